@@ -1,0 +1,1100 @@
+// g4b_paged.cu -- a batch of sequences over a paged f16 KV cache: the plan of the batch, the append of its new
+// keys and values with norm and rotation, and its attention, with a prefix that all sequences share read once.
+//
+// The cache is [num_pages, nkv, page_size, hd] f16: the engine's per-head cache rows (src/vk_engine.py:281-282)
+// cut into pages.  The arithmetic per token and head is that of vk/prepkv.comp and vk/attn.comp.
+#include <algorithm>
+
+#include "g4b_paged.cuh"
+#include "g4b_tcgen05.cuh"   // mbar_wait_drain
+
+namespace g4b {
+namespace pg {
+
+constexpr float kEps = 1e-6f;    // vk/attn.comp:25, vk/prepkv.comp:21
+__device__ unsigned g_status_paged;
+
+// ------------------------------------------------------------------ sizes
+static unsigned sig_of(const Dims& d) {
+    unsigned h = 2166136261u;
+    for (int v : {d.T, d.B, d.nH, d.nkv, d.hd, d.ps, d.own_pages, d.pre_pages, d.window, d.ctas[0], d.ctas[1]})
+        h = (h ^ (unsigned)v) * 16777619u;
+    return h | 1u;
+}
+
+static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+// CTAs of the few-rows kernel per SM: two where the stages of two fit an SM's shared memory (hd 128, 256)
+static int few_per_sm(int hd) { return hd == 512 ? 1 : 2; }
+
+// Checks the sizes and lays the plan out for `sms` SMs.  No device is needed: a caller that will launch asks
+// check_device() last, when every argument has been looked at.
+static int make_dims(const char* op, int T, int B, int nH, int nkv, int hd, int ps, int own_pages, int pre_pages,
+                     int window, Dims& d) {
+    G4B_REQUIRE(T >= 1 && B >= 1 && B <= kMaxSeqs, G4B_E_SHAPE, "%s: T=%d tokens, B=%d sequences (1 to %d)", op, T, B,
+                kMaxSeqs);
+    G4B_REQUIRE(nkv >= 1 && nkv <= 65535 && nH >= nkv && nH % nkv == 0 && (hd == 128 || hd == 256 || hd == 512),
+                G4B_E_SHAPE, "%s: nH=%d nkv=%d hd=%d (nH a multiple of nkv, hd 128, 256 or 512)", op, nH, nkv, hd);
+    G4B_REQUIRE(ps >= 16 && ps <= 1024 && (ps & (ps - 1)) == 0, G4B_E_SHAPE,
+                "%s: page_size=%d (a power of two from 16 to 1024)", op, ps);
+    G4B_REQUIRE(own_pages >= 1 && pre_pages >= 0 && window >= 0 &&
+                    ((long long)own_pages + pre_pages) * ps <= 0x40000000LL,
+                G4B_E_SHAPE, "%s: table of %d pages, prefix of %d, page_size %d, window %d (at most 2^30 positions)",
+                op, own_pages, pre_pages, ps, window);
+    G4B_REQUIRE((long long)T * nH <= 0x20000000LL, G4B_E_SHAPE, "%s: T=%d tokens of %d heads are too many", op, T, nH);
+    int sms = 148;
+    if (check_device(&sms) != G4B_OK) sms = 148;
+    clear_error();
+    d = Dims{};
+    d.T = T;
+    d.B = B;
+    d.nH = nH;
+    d.nkv = nkv;
+    d.G = nH / nkv;
+    d.hd = hd;
+    d.ps = ps;
+    d.own_pages = own_pages;
+    d.pre_pages = pre_pages;
+    d.window = window;
+    d.ctas[0] = sms * few_per_sm(hd);
+    d.ctas[1] = sms;
+    const int rows = T * d.G;
+    const bool many = many_rows(hd);
+    // tiles of sequences (one more each for the last, partial one) and of the prefix
+    d.max_tiles[0] = (many ? 0 : 2 * (rows / kRowsS)) + B + 1;
+    d.max_tiles[1] = many ? 2 * (rows / kRowsP) + B + 1 : 0;
+    size_t o = up256(sizeof(Hdr));
+    auto take = [&](size_t bytes) {
+        const size_t at = o;
+        o += up256(bytes);
+        return at;
+    };
+    d.tok_seq = take((size_t)T * 4);
+    d.tok_pos = take((size_t)T * 4);
+    d.row_own = take((size_t)rows * 4);
+    d.row_pre = take((size_t)rows * 4);
+    for (int k = 0; k < 2; k++) {
+        d.start[k] = take((size_t)d.ctas[k] * sizeof(Start));
+        d.tiles[k] = take((size_t)d.max_tiles[k] * sizeof(Tile));
+    }
+    d.bytes = o;
+    d.sig = sig_of(d);
+    return G4B_OK;
+}
+
+static size_t work_bytes(const Dims& d, char* base, Work* w) {
+    size_t o = 0;
+    auto take = [&](size_t bytes) {
+        const size_t at = o;
+        o += up256(bytes);
+        return base + at;
+    };
+    Work x{};
+    for (int k = 0; k < 2; k++) {
+        if (k == 1 && !many_rows(d.hd)) continue;
+        const size_t rows = (size_t)d.ctas[k] * 2 * (k ? kRowsP : kRowsS);
+        x.edge[k] = reinterpret_cast<float*>(take(rows * d.hd * 4));
+        x.edge_ml[k] = reinterpret_cast<float2*>(take(rows * 8));
+    }
+    if (d.pre_pages > 0) {
+        const size_t rows = (size_t)d.T * d.nH * 2;
+        x.row = reinterpret_cast<float*>(take(rows * d.hd * 4));
+        x.row_ml = reinterpret_cast<float2*>(take(rows * 8));
+    }
+    if (w) *w = x;
+    return o;
+}
+
+// ------------------------------------------------------------------ plan
+// Every CTA reads the sequences into shared memory and makes its share of the per-token and per-row
+// arrays; CTA 0 makes the tiles, whose offsets are one running sum.  Nothing the caller's lengths say is
+// trusted with an address: starts are made non-decreasing and cut to [0, T], lengths to the tables'
+// capacity.
+constexpr int kPlanThreads = 1024;
+
+struct PlanArgs {
+    const int* q_start;
+    const int* kv_len;
+    const int* prefix_len;
+    void* plan;
+    Dims d;
+    int many;
+};
+
+__device__ __forceinline__ int seq_of(const int* st, int B, int t) {   // the last b with st[b] <= t
+    int lo = 0, hi = B;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (st[m] <= t) lo = m;
+        else hi = m;
+    }
+    return lo;
+}
+
+template <typename X, typename F>
+__device__ X block_scan(X v, X init, X* warp_buf, X* total, F op) {   // exclusive; total: of the whole block
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    X inc = v;
+    #pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const X u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc = op(u, inc);
+    }
+    X exc = __shfl_up_sync(0xffffffffu, inc, 1);
+    if (lane == 0) exc = init;
+    __syncthreads();
+    if (lane == 31) warp_buf[warp] = inc;
+    __syncthreads();
+    X before = init, all = init;
+    for (int w = 0; w < kPlanThreads / 32; w++) {
+        if (w == warp) before = all;
+        all = op(all, warp_buf[w]);
+    }
+    *total = all;
+    return op(before, exc);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
+    extern __shared__ int sm[];
+    __shared__ long long wbuf[kPlanThreads / 32];
+    __shared__ int ibuf[kPlanThreads / 32];
+    const Dims& d = a.d;
+    const int B = d.B, G = d.G, tid = threadIdx.x;
+    int* st = sm;                    // [B + 1] first row of each sequence
+    int* len = st + B + 1;           // [B] tokens it holds
+    int* base = len + B;             // [B] first tile of each sequence among its kind's; the kind in bit 31
+    const int pl = a.prefix_len ? min(max(__ldg(a.prefix_len), 0), d.pre_pages * d.ps) : 0;
+    const int cap = pl + d.own_pages * d.ps;
+    // starts: running maximum of the given ones, within [0, T]
+    {
+        int run = 0;
+        for (int i0 = 0; i0 <= B; i0 += kPlanThreads) {
+            const int i = i0 + tid;
+            const int v = i <= B ? min(max(__ldg(a.q_start + i), 0), d.T) : 0;
+            int all;
+            const int exc = block_scan(v, 0, ibuf, &all, [](int x, int y) { return max(x, y); });
+            if (i <= B) st[i] = max(run, max(exc, v));
+            run = max(run, all);
+        }
+        for (int i = tid; i < B; i += kPlanThreads) len[i] = min(max(__ldg(a.kv_len + i), 0), cap);
+    }
+    __syncthreads();
+    const int r_lo = st[0] * G, r_hi = st[B] * G;
+    const bool pre_many = a.many && r_hi - r_lo > kRowsS;
+    const int pre_rows = pre_many ? kRowsP : kRowsS;
+    const int pre_tiles = pl > 0 ? (r_hi - r_lo + pre_rows - 1) / pre_rows : 0;
+    auto many_of = [&](int b) { return a.many && (st[b + 1] - st[b]) * G > kRowsS; };
+    // first tile of each sequence: the prefix's come first
+    int nt[2] = {pre_many ? 0 : pre_tiles, pre_many ? pre_tiles : 0};
+    for (int i0 = 0; i0 < B; i0 += kPlanThreads) {
+        const int b = i0 + tid;
+        const int rows = b < B ? (st[b + 1] - st[b]) * G : 0;
+        const bool many = b < B && many_of(b);
+        int all0, all1;
+        const auto add = [](int x, int y) { return x + y; };
+        const int e0 = block_scan(many ? 0 : (rows + kRowsS - 1) / kRowsS, 0, ibuf, &all0, add);
+        const int e1 = block_scan(many ? (rows + kRowsP - 1) / kRowsP : 0, 0, ibuf, &all1, add);
+        if (b < B) base[b] = many ? (int)(0x80000000u | (unsigned)(nt[1] + e1)) : nt[0] + e0;
+        nt[0] += all0;
+        nt[1] += all1;
+    }
+    __syncthreads();
+
+    // ---- per token and per row
+    const int gtid = blockIdx.x * kPlanThreads + tid, gn = gridDim.x * kPlanThreads;
+    for (int t = gtid; t < d.T; t += gn) {
+        const bool live = t >= st[0] && t < st[B];
+        int b = -1, pos = -1;
+        if (live) {
+            b = seq_of(st, B, t);
+            pos = len[b] - st[b + 1] + t;
+        }
+        at<int>(a.plan, d.tok_seq)[t] = b;
+        at<int>(a.plan, d.tok_pos)[t] = pos;
+    }
+    for (int r = gtid; r < d.T * G; r += gn) {
+        int own = -1, pre = -1;
+        if (r >= r_lo && r < r_hi) {
+            const int b = seq_of(st, B, r / G);
+            const unsigned kind = (unsigned)base[b] & 0x80000000u;
+            own = (int)(kind | (((unsigned)base[b] & 0x7fffffffu) +
+                                (unsigned)((r - st[b] * G) / (kind ? kRowsP : kRowsS))));
+            if (pre_tiles) pre = (int)((pre_many ? 0x80000000u : 0u) | (unsigned)((r - r_lo) / pre_rows));
+        }
+        at<int>(a.plan, d.row_own)[r] = own;
+        at<int>(a.plan, d.row_pre)[r] = pre;
+    }
+    if (blockIdx.x != 0) return;
+
+    // ---- the tiles, by CTA 0
+    auto first_key = [&](int pos) { return d.window > 0 ? max(0, pos + 1 - d.window) : 0; };
+    for (int i = tid; i < pre_tiles; i += kPlanThreads) {
+        Tile t{};
+        t.row0 = r_lo + i * pre_rows;
+        t.nrows = min(pre_rows, r_hi - t.row0);
+        t.seq = -1;
+        // the positions of its rows: within a sequence they rise
+        const int t0 = t.row0 / G, t1 = (t.row0 + t.nrows - 1) / G;
+        int lo = 0x7fffffff, hi = 0;
+        for (int b = seq_of(st, B, t0); b < B && st[b] <= t1; b++) {
+            const int f = max(t0, st[b]), l = min(t1, st[b + 1] - 1);
+            if (l < f) continue;
+            lo = min(lo, first_key(len[b] - st[b + 1] + f));
+            hi = max(hi, len[b] - st[b + 1] + l + 1);
+        }
+        t.lo = lo / kUnit * kUnit;
+        t.hi = min(pl, hi);
+        t.n = max(0, (t.hi - t.lo + kUnit - 1) / kUnit);
+        at<Tile>(a.plan, d.tiles[pre_many ? 1 : 0])[i] = t;
+    }
+    // each sequence names its tiles (a warp per sequence: a long prompt has many)
+    for (int b = tid >> 5; b < B; b += kPlanThreads / 32) {
+        const bool many = many_of(b);
+        const int br = many ? kRowsP : kRowsS, n = ((st[b + 1] - st[b]) * G + br - 1) / br;
+        Tile* tiles = at<Tile>(a.plan, d.tiles[many ? 1 : 0]) + ((unsigned)base[b] & 0x7fffffffu);
+        for (int k = tid & 31; k < n; k += 32) tiles[k].seq = b;
+    }
+    __syncthreads();
+    Hdr* h = reinterpret_cast<Hdr*>(a.plan);
+    for (int kind = 0; kind < 2; kind++) {
+        Tile* tiles = at<Tile>(a.plan, d.tiles[kind]);
+        const int br = kind ? kRowsP : kRowsS;
+        const bool pre_here = pre_tiles > 0 && (kind == 1) == pre_many;
+        long long run = 0;
+        for (int i0 = 0; i0 < nt[kind]; i0 += kPlanThreads) {
+            const int i = i0 + tid;
+            Tile t{};
+            if (i < nt[kind]) {
+                if (pre_here && i < pre_tiles) {
+                    t = tiles[i];
+                } else {
+                    const int b0 = tiles[i].seq;
+                    const int lr = (i - (int)((unsigned)base[b0] & 0x7fffffffu)) * br;
+                    t.seq = b0;
+                    t.row0 = st[b0] * G + lr;
+                    t.nrows = min(br, (st[b0 + 1] - st[b0]) * G - lr);
+                    const int p0 = len[b0] - st[b0 + 1] + t.row0 / G;
+                    const int p1 = len[b0] - st[b0 + 1] + (t.row0 + t.nrows - 1) / G;
+                    t.lo = max(0, first_key(p0) - pl) / kUnit * kUnit;
+                    t.hi = p1 + 1 - pl;
+                    t.n = max(0, (t.hi - t.lo + kUnit - 1) / kUnit);
+                    t.solo = 1;
+                    if (pre_tiles) {
+                        const Tile* pt = at<Tile>(a.plan, d.tiles[pre_many ? 1 : 0]);
+                        for (int j = (t.row0 - r_lo) / pre_rows; j <= (t.row0 + t.nrows - 1 - r_lo) / pre_rows; j++)
+                            if (pt[j].n > 0) t.solo = 0;
+                    }
+                }
+            }
+            long long all;
+            const long long exc = block_scan((long long)t.n, 0LL, wbuf, &all,
+                                             [](long long x, long long y) { return x + y; });
+            if (i < nt[kind]) {
+                t.off = run + exc;
+                tiles[i] = t;
+            }
+            run += all;
+        }
+        __syncthreads();
+        // equal stretches of the line of all heads' units
+        const long long total = run * d.nkv;
+        const long long u = max(1LL, (total + d.ctas[kind] - 1) / d.ctas[kind]);
+        if (tid == 0) {
+            h->nt[kind] = nt[kind];
+            h->wt[kind] = run;
+            h->u[kind] = u;
+        }
+        for (int c = tid; c < d.ctas[kind]; c += kPlanThreads) {
+            Start s{-1, 0, 0, 0};
+            const long long at0 = (long long)c * u;
+            if (at0 < total) {
+                const long long rem = at0 % run;
+                s.head = (int)(at0 / run);
+                int lo = 0, hi = nt[kind];       // the last tile with off <= rem; of equal ones it is the one with units
+                while (hi - lo > 1) {
+                    const int m = (lo + hi) >> 1;
+                    if (tiles[m].off <= rem) lo = m;
+                    else hi = m;
+                }
+                s.tile = lo;
+                s.unit = (int)(rem - tiles[lo].off);
+            }
+            at<Start>(a.plan, d.start[kind])[c] = s;
+        }
+    }
+    if (tid == 0) {
+        h->sig = d.sig;
+        h->prefix_len = pl;
+        h->tok_lo = st[0];
+        h->tok_hi = st[B];
+    }
+}
+
+// ------------------------------------------------------------------ append
+struct AppendArgs {
+    const void* plan;
+    const void* qkv;
+    const float* qnw;
+    const float* knw;
+    const float* cos_t;
+    const float* sin_t;
+    uint16_t* kc;
+    uint16_t* vc;
+    const int* table;
+    uint16_t* q_out;
+    long long row_stride, q_stride;
+    int koff, voff, num_pages;
+    Dims d;
+};
+
+constexpr int kAppendThreads = 256;
+
+template <int N, bool F32>
+__device__ __forceinline__ void load_n(const void* base, long long e, float (&v)[N]) {
+    if constexpr (F32) {
+        const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + e);
+        #pragma unroll
+        for (int j = 0; j < N / 4; j++) {
+            const float4 x = __ldg(p + j);
+            v[4 * j] = x.x; v[4 * j + 1] = x.y; v[4 * j + 2] = x.z; v[4 * j + 3] = x.w;
+        }
+    } else {
+        const uint2* p = reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(base) + e);
+        #pragma unroll
+        for (int j = 0; j < N / 4; j++) {
+            const uint2 u = __ldg(p + j);
+            v[4 * j] = h_lo(u.x); v[4 * j + 1] = h_hi(u.x); v[4 * j + 2] = h_lo(u.y); v[4 * j + 3] = h_hi(u.y);
+        }
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void store_half(uint16_t* p, const float (&v)[N]) {
+    #pragma unroll
+    for (int j = 0; j < N / 4; j++) {
+        uint2 u;
+        u.x = pack_half2(__float2half_rn(v[4 * j]), __float2half_rn(v[4 * j + 1]));
+        u.y = pack_half2(__float2half_rn(v[4 * j + 2]), __float2half_rn(v[4 * j + 3]));
+        reinterpret_cast<uint2*>(p)[j] = u;
+    }
+}
+
+// One warp per head, the heads of a token spread over the warps of its CTAs (blockIdx.y).  Lane l holds
+// elements l * PER ..; element i's rotation partner i +- hd/2 is in lane l ^ 16.
+template <int HD, bool XF32>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
+    constexpr int PER = HD / 32;
+    const Dims& d = a.d;
+    const Hdr* h = hdr_of(a.plan);
+    if (h->sig != d.sig) {
+        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(&g_status_paged, kStatusPlan);
+        return;
+    }
+    const int t = blockIdx.x, lane = threadIdx.x & 31;
+    const int warps = gridDim.y * (kAppendThreads / 32), w0 = blockIdx.y * (kAppendThreads / 32) + (threadIdx.x >> 5);
+    const int b = __ldg(at<int>(a.plan, d.tok_seq) + t), pos = __ldg(at<int>(a.plan, d.tok_pos) + t);
+    if (b < 0 || pos < 0) return;    // behind the last sequence; or more new tokens than its length says
+    const int own = pos - h->prefix_len;
+    int slot = -1;                   // the token's row of the cache for KV head 0
+    if (own >= 0)
+        slot = cache_row(__ldg(a.table + (size_t)b * d.own_pages + own / d.ps), a.num_pages, d.nkv, d.ps, 0, own);
+    float cs[PER], sn[PER];
+    load_n<PER, true>(a.cos_t, (long long)pos * HD + lane * PER, cs);
+    load_n<PER, true>(a.sin_t, (long long)pos * HD + lane * PER, sn);
+    const int heads = d.nH + 2 * d.nkv;
+    for (int j = w0; j < heads; j += warps) {
+        const bool is_q = j < d.nH, is_v = j >= d.nH + d.nkv;
+        const int kv = is_v ? j - d.nH - d.nkv : j - d.nH;
+        if (!is_q && slot < 0) continue;
+        const long long e = (long long)t * a.row_stride + lane * PER +
+                            (is_q ? (long long)j * HD : (is_v ? a.voff : a.koff) + (long long)kv * HD);
+        float v[PER];
+        load_n<PER, XF32>(a.qkv, e, v);
+        float ss = 0.f;
+        #pragma unroll
+        for (int i = 0; i < PER; i++) ss = fmaf(v[i], v[i], ss);
+        #pragma unroll
+        for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+        const float r = rsqrtf(ss / (float)HD + kEps);
+        if (is_v) {
+            #pragma unroll
+            for (int i = 0; i < PER; i++) v[i] *= r;
+        } else {
+            float g[PER];
+            load_n<PER, true>(is_q ? a.qnw : a.knw, lane * PER, g);
+            #pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const float n = v[i] * r * g[i];
+                const float o = __shfl_xor_sync(0xffffffffu, n, 16);
+                v[i] = n * cs[i] + (lane < 16 ? -o : o) * sn[i];
+            }
+        }
+        uint16_t* dst = is_q ? a.q_out + (long long)t * a.q_stride + (long long)j * HD
+                             : (is_v ? a.vc : a.kc) + ((long long)slot + kv * d.ps) * HD;
+        store_half<PER>(dst + lane * PER, v);
+    }
+}
+
+// ------------------------------------------------------------------ attention, few rows
+// A tile of up to 8 rows (the query heads of a token or two) over a stretch of keys, HBM-bound on them.  The
+// products are transposed so that the rows are the n = 8 of m16n8k16 and the keys or the head's elements
+// the m = 16:
+//   S^T [16 keys x 8 rows] = K [16 x hd] Q^T,   O^T [hd x 8] += V^T [hd x 16 keys] P^T
+// K and V fragments come from shared memory by ldmatrix (transposed for V), Q stays in registers, and P^T
+// gets from its accumulator layout to an operand's by movmatrix.  P enters as f16 hi + lo, since these
+// MMAs are not what bounds the kernel.  The four warps of a CTA take every fourth block of 16 keys, each
+// with its own ring of TMA-filled buffers, its own running maximum and sum: no CTA barrier until the
+// partials of the warps are added at a piece's end.
+constexpr int kFewWarps = 4;
+constexpr int kBlk = 16;             // keys per block (one page always holds a block: page_size >= 16)
+
+template <int HD>
+struct FewCfg {
+    static constexpr int ENTRY = kBlk * HD * 2;               // bytes of a block of K or of V
+    static constexpr int NST = HD == 128 ? 6 : 3;             // ring entries per warp: 24 / 24 / 48 KB
+    static constexpr int SMEM = kFewWarps * NST * ENTRY + 1024;   // + alignment
+    static constexpr int PITCH = HD + 4;                      // floats per row of the merge buffer
+    static_assert(kRowsS * PITCH * 4 <= NST * ENTRY, "a warp's partial fits its ring");
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t movm_t(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+template <int HD>
+__global__ void __launch_bounds__(32 * kFewWarps, HD == 512 ? 1 : 2)
+few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    using C = FewCfg<HD>;
+    constexpr int KK = HD / 16;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[kFewWarps][C::NST];
+    __shared__ float s_m[kFewWarps][kRowsS], s_l[kFewWarps][kRowsS];
+    __shared__ int s_abort;
+    const Dims& d = a.d;
+    const Hdr* h = hdr_of(a.plan);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+    pdl_launch_dependents();
+    if (h->sig != d.sig) {
+        if (blockIdx.x == 0 && tid == 0) atomicOr(&g_status_paged, kStatusPlan);
+        return;
+    }
+    const Start st = at<Start>(a.plan, d.start[0])[blockIdx.x];
+    if (st.head < 0) return;
+    const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + (uint32_t)(warp * C::NST * C::ENTRY);
+    uint8_t* ring_p = smem_raw + (ring - smem_u32(smem_raw));
+    const uint32_t bar0 = smem_u32(&bars[warp][0]);
+    if (lane == 0) {
+        for (int i = 0; i < C::NST; i++) mbar_init(bar0 + 8 * i, 1);
+        fence_mbar_init();
+    }
+    if (tid == 0) s_abort = 0;
+    __syncthreads();
+    volatile int* abort = &s_abort;
+    const int pl = h->prefix_len, G = d.G;
+    const long long wt = h->wt[0], u_all = h->u[0];
+    const int ntiles = h->nt[0];
+    const Tile* tiles = at<Tile>(a.plan, d.tiles[0]);
+    const int* tok_pos = at<int>(a.plan, d.tok_pos);
+    long long left = min(u_all, wt * d.nkv - (long long)blockIdx.x * u_all);
+    int head = st.head, ti = st.tile, unit = st.unit;
+    int entry = 0;                       // ring position of the next entry to consume; runs on over pieces
+    uint32_t phase = 0;                  // parity bit per ring position
+
+    while (left > 0) {
+        if (ti == ntiles) {
+            ti = 0;
+            head++;
+        }
+        const Tile t = tiles[ti];
+        if (t.n == 0) {
+            ti++;
+            unit = 0;
+            continue;
+        }
+        const int nu = (int)min((long long)(t.n - unit), left);
+        const int key0 = t.lo + unit * kUnit, key1 = min(t.hi, key0 + nu * kUnit);
+        const int kbase = t.seq < 0 ? 0 : pl;                        // position of the segment's key 0
+        const int* table = t.seq < 0 ? a.pre_table : a.table + (size_t)t.seq * d.own_pages;
+        const int table_n = t.seq < 0 ? d.pre_pages : d.own_pages;
+        // this thread's rows: 2 * q4 and 2 * q4 + 1 of the scores; row g of Q
+        int vlo[2], vhi[2], all_lo = 0, all_hi = 0x7fffffff;         // keys that a row sees; that all rows see
+        #pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = 2 * q4 + i;
+            const int pos = __ldg(tok_pos + (t.row0 + min(r, t.nrows - 1)) / G);
+            vhi[i] = pos + 1 - kbase;
+            vlo[i] = d.window > 0 ? pos + 1 - d.window - kbase : 0;
+            all_lo = max(all_lo, vlo[i]);
+            all_hi = min(all_hi, vhi[i]);
+        }
+        #pragma unroll
+        for (int m = 1; m <= 2; m <<= 1) {
+            all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, m));
+            all_hi = min(all_hi, __shfl_xor_sync(0xffffffffu, all_hi, m));
+        }
+        const int tok_a = t.row0 / G, tok_b = (t.row0 + t.nrows - 1) / G;
+        uint32_t qf[KK][2];
+        {
+            const bool live = g < t.nrows;
+            const int row = t.row0 + (live ? g : 0);
+            const uint16_t* qp = a.q + (long long)(row / G) * a.q_stride + (long long)(head * G + row % G) * HD + 2 * q4;
+            #pragma unroll
+            for (int k = 0; k < KK; k++) {
+                qf[k][0] = live ? __ldg(reinterpret_cast<const uint32_t*>(qp + 16 * k)) : 0u;
+                qf[k][1] = live ? __ldg(reinterpret_cast<const uint32_t*>(qp + 16 * k + 8)) : 0u;
+            }
+        }
+        float o[KK][4];
+        #pragma unroll
+        for (int k = 0; k < KK; k++) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+        // this warp's blocks: key0 + 16 * (warp + 4 n)
+        const int nblk_all = (key1 - key0 + kBlk - 1) / kBlk;
+        const int nblk = (nblk_all - warp + kFewWarps - 1) / kFewWarps;
+        const int total = 2 * max(nblk, 0);      // entries: K and V of each block in turn
+        uint32_t valid = 0;                      // bit n % 32: block n's page exists
+        int ids = 0, ids_at = -32;               // page ids of 32 blocks, one per lane
+        int eslot = entry, issued = 0;
+        auto issue = [&](int e) {                // whole warp; e counts the piece's entries
+            const int n = e >> 1;
+            if (n >= ids_at + 32) {
+                ids_at = n;
+                const int key = key0 + kBlk * (warp + kFewWarps * (n + lane));
+                const int page = key / d.ps;
+                ids = key < key1 && page < table_n ? __ldg(table + page) : -1;
+            }
+            const int key = key0 + kBlk * (warp + kFewWarps * n);
+            const int page = __shfl_sync(0xffffffffu, ids, n - ids_at);
+            const int at_row = cache_row(page, a.num_pages, d.nkv, d.ps, head, key);
+            const bool ok = at_row >= 0;
+            if (!(e & 1)) valid = (valid & ~(1u << (n & 31))) | ((ok ? 1u : 0u) << (n & 31));
+            // a page that is not there: past the map's last row, which TMA fills with zeros
+            const int row = ok ? at_row : a.num_pages * d.nkv * d.ps;
+            if (lane == 0) {
+                const uint32_t bar = bar0 + 8 * eslot, dst = ring + (uint32_t)(eslot * C::ENTRY);
+                mbar_arrive_expect_tx(bar, C::ENTRY);
+                #pragma unroll
+                for (int c = 0; c < HD / 64; c++)
+                    tma_2d(dst + c * (kBlk * 128), (e & 1) ? &vmap : &kmap, 64 * c, row, bar);
+            }
+            eslot = eslot + 1 == C::NST ? 0 : eslot + 1;
+            issued++;
+        };
+        const int ahead = min(C::NST, total);
+        for (int e = 0; e < ahead; e++) issue(e);
+        bool ok = true;
+        int done = 0;                            // entries consumed
+        auto next = [&]() {                      // wait for the next entry; its address
+            ok = __all_sync(0xffffffffu, mbar_wait(bar0 + 8 * entry, (phase >> entry) & 1u, abort, &g_status_paged));
+            if (ok) phase ^= 1u << entry;
+            return ring + (uint32_t)(entry * C::ENTRY);
+        };
+        auto release = [&]() {                   // the entry just read may be filled again
+            __syncwarp();
+            entry = entry + 1 == C::NST ? 0 : entry + 1;
+            done++;
+            if (done + C::NST - 1 < total) issue(done + C::NST - 1);
+        };
+        for (int n = 0; n < nblk; n++) {
+            const int key = key0 + kBlk * (warp + kFewWarps * n);
+            const uint32_t kb = next();
+            if (!ok) break;
+            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};   // two chains
+            {
+                const int row = (lane & 7) + 8 * ((lane >> 3) & 1);
+                #pragma unroll
+                for (int k = 0; k < KK; k++) {
+                    uint32_t f[4];
+                    const int un = 2 * k + (lane >> 4);
+                    ldsm4(kb + (un >> 3) * (kBlk * 128) + row * 128 + (((un & 7) ^ (row & 7)) << 4), f);
+                    mma8(s[k & 1], f, qf[k][0], qf[k][1]);
+                }
+            }
+            const bool there = (valid >> (n & 31)) & 1u;
+            release();
+            // keys g and g + 8 of rows 2 q4 and 2 q4 + 1
+            float x[4];
+            #pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = (s[0][e] + s[1][e]) * a.scale;
+            const bool edge = !there || key < all_lo || key + kBlk > min(all_hi, key1);
+            if (edge) {
+                #pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int j = key + g + 8 * (e >> 1);
+                    if (!there || j >= key1 || j < vlo[e & 1] || j >= vhi[e & 1]) x[e] = -INFINITY;
+                }
+            }
+            float corr[2];
+            #pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float mx = fmaxf(x[i], x[2 + i]);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float mn = fmaxf(m[i], mx);
+                const float mu = mn == -INFINITY ? 0.f : mn;     // nothing seen yet: weights 2^-inf = 0
+                corr[i] = exp2_approx(m[i] - mu);
+                m[i] = mn;
+                x[i] = exp2_approx(x[i] - mu);
+                x[2 + i] = exp2_approx(x[2 + i] - mu);
+                l[i] = fmaf(l[i], corr[i], x[i] + x[2 + i]);
+            }
+            const __half2 h0 = __floats2half2_rn(x[0], x[1]), h1 = __floats2half2_rn(x[2], x[3]);
+            const __half2 r0 = __floats2half2_rn(x[0] - __low2float(h0), x[1] - __high2float(h0));
+            const __half2 r1 = __floats2half2_rn(x[2] - __low2float(h1), x[3] - __high2float(h1));
+            const uint32_t ph0 = movm_t(*reinterpret_cast<const uint32_t*>(&h0));
+            const uint32_t ph1 = movm_t(*reinterpret_cast<const uint32_t*>(&h1));
+            const uint32_t pw0 = movm_t(*reinterpret_cast<const uint32_t*>(&r0));
+            const uint32_t pw1 = movm_t(*reinterpret_cast<const uint32_t*>(&r1));
+            if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+                #pragma unroll
+                for (int k = 0; k < KK; k++) {
+                    o[k][0] *= corr[0];
+                    o[k][1] *= corr[1];
+                    o[k][2] *= corr[0];
+                    o[k][3] *= corr[1];
+                }
+            }
+            const uint32_t vb = next();
+            if (!ok) break;
+            const int row = (lane & 7) + 8 * (lane >> 4);
+            auto vfrag = [&](int k, uint32_t (&f)[4]) {
+                const int un = 2 * k + ((lane >> 3) & 1);
+                ldsm4t(vb + (un >> 3) * (kBlk * 128) + row * 128 + (((un & 7) ^ (row & 7)) << 4), f);
+            };
+            if (!edge) {
+                #pragma unroll
+                for (int k = 0; k < KK; k++) {
+                    uint32_t f[4];
+                    vfrag(k, f);
+                    mma8(o[k], f, ph0, ph1);
+                    mma8(o[k], f, pw0, pw1);
+                }
+            } else {
+                // A value behind the mask may be anything, NaN included, and 0 x NaN is not 0: the values a
+                // token does not see are cleared.  Rows of several tokens see different keys, so each token
+                // then has products of its own, of which only its rows are added.
+                for (int tok = tok_a; tok <= tok_b; tok++) {
+                    const int pos = __ldg(tok_pos + tok);
+                    const int th = min(key1, pos + 1 - kbase), tl = d.window > 0 ? pos + 1 - d.window - kbase : 0;
+                    auto keep = [&](int j) { return there && j >= tl && j < th; };
+                    const int j0 = key + 2 * q4;
+                    const uint32_t k0 = (keep(j0) ? 0xffffu : 0u) | (keep(j0 + 1) ? 0xffff0000u : 0u);
+                    const uint32_t k1 = (keep(j0 + 8) ? 0xffffu : 0u) | (keep(j0 + 9) ? 0xffff0000u : 0u);
+                    const bool c0 = (t.row0 + 2 * q4) / G == tok, c1 = (t.row0 + 2 * q4 + 1) / G == tok;
+                    #pragma unroll
+                    for (int k = 0; k < KK; k++) {
+                        uint32_t f[4];
+                        vfrag(k, f);
+                        f[0] &= k0;
+                        f[1] &= k0;
+                        f[2] &= k1;
+                        f[3] &= k1;
+                        float e4[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma8(e4, f, ph0, ph1);
+                        mma8(e4, f, pw0, pw1);
+                        if (c0) o[k][0] += e4[0];
+                        if (c1) o[k][1] += e4[1];
+                        if (c0) o[k][2] += e4[2];
+                        if (c1) o[k][3] += e4[3];
+                    }
+                }
+            }
+            release();
+        }
+        // the sums of a row lie in the lanes of its column
+        #pragma unroll
+        for (int i = 0; i < 2; i++) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 8);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
+        }
+        if (g == 0) {
+            s_m[warp][2 * q4] = m[0];
+            s_m[warp][2 * q4 + 1] = m[1];
+            s_l[warp][2 * q4] = l[0];
+            s_l[warp][2 * q4 + 1] = l[1];
+        }
+        if (!ok) {
+            // a wait ran out: the copies still in flight land (bounded) before shared memory is given up
+            for (; done < issued; done++) {
+                mbar_wait_drain(bar0 + 8 * entry, (phase >> entry) & 1u, &g_status_paged);
+                phase ^= 1u << entry;
+                entry = entry + 1 == C::NST ? 0 : entry + 1;
+            }
+        }
+        // the ring is empty now: it takes the warp's partial
+        float* mine = reinterpret_cast<float*>(ring_p);
+        #pragma unroll
+        for (int k = 0; k < KK; k++) {
+            mine[(2 * q4) * C::PITCH + 16 * k + g] = o[k][0];
+            mine[(2 * q4 + 1) * C::PITCH + 16 * k + g] = o[k][1];
+            mine[(2 * q4) * C::PITCH + 16 * k + g + 8] = o[k][2];
+            mine[(2 * q4 + 1) * C::PITCH + 16 * k + g + 8] = o[k][3];
+        }
+        __syncthreads();
+        if (*abort) break;                       // the same for the whole CTA: it is set before the barrier only
+        const bool whole = nu == t.n;
+        const bool direct = whole && t.solo;
+        const float* parts = reinterpret_cast<const float*>(ring_p - warp * C::NST * C::ENTRY);
+        constexpr int WP = C::NST * C::ENTRY / 4;    // floats between two warps' partials
+        for (int e = tid; e < t.nrows * (HD / 4); e += 32 * kFewWarps) {
+            const int r = e / (HD / 4), c = 4 * (e % (HD / 4));
+            float M = s_m[0][r];
+            #pragma unroll
+            for (int w = 1; w < kFewWarps; w++) M = fmaxf(M, s_m[w][r]);
+            const float mu = M == -INFINITY ? 0.f : M;
+            float L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+            #pragma unroll
+            for (int w = 0; w < kFewWarps; w++) {
+                const float f = exp2_approx(s_m[w][r] - mu);
+                L = fmaf(s_l[w][r], f, L);
+                const float4 p = *reinterpret_cast<const float4*>(parts + w * WP + r * C::PITCH + c);
+                v[0] = fmaf(p.x, f, v[0]);
+                v[1] = fmaf(p.y, f, v[1]);
+                v[2] = fmaf(p.z, f, v[2]);
+                v[3] = fmaf(p.w, f, v[3]);
+            }
+            const int row = t.row0 + r, tok = row / G, hq = head * G + row % G;
+            if (direct) {
+                const float inv = L == 0.f ? 0.f : 1.f / L;
+                const long long at0 = (long long)tok * a.out_stride + (long long)hq * HD + c;
+                if (a.out_f32) {
+                    *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at0) =
+                        make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                } else {
+                    uint2 p;
+                    p.x = pack_half2(__float2half_rn(v[0] * inv), __float2half_rn(v[1] * inv));
+                    p.y = pack_half2(__float2half_rn(v[2] * inv), __float2half_rn(v[3] * inv));
+                    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(a.out) + at0) = p;
+                }
+            } else {
+                // whole: the row's own slot; else this CTA's edge slot: 1 for the tile's first piece, 0 for a later
+                const size_t slot = whole ? ((size_t)(t.seq < 0 ? 0 : 1) * d.T + tok) * d.nH + hq
+                                          : ((size_t)blockIdx.x * 2 + (unit == 0 ? 1 : 0)) * kRowsS + r;
+                float* dst = (whole ? a.w.row : a.w.edge[0]) + slot * HD + c;
+                *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+                if (c == 0) (whole ? a.w.row_ml : a.w.edge_ml[0])[slot] = make_float2(M, L);
+            }
+        }
+        // the ring was written and read by threads; the next piece's copies come behind that
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+        left -= nu;
+        unit += nu;
+        if (unit == t.n) {
+            unit = 0;
+            ti++;
+        }
+    }
+    // the join reads what this grid and the one before it wrote: done only when that one is
+    pdl_wait();
+}
+
+// ------------------------------------------------------------------ join
+// One warp per (token, query head): out = sum_p V_p 2^(m_p - M) / sum_p l_p 2^(m_p - M) over the partials
+// of its prefix tile and its own tile.  A row whose own whole tile wrote it is left; a row with no key at
+// all becomes zeros.
+constexpr int kJoinThreads = 128;
+
+template <int HD>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
+    constexpr int PER = HD / 32;
+    const Dims& d = a.d;
+    const Hdr* h = hdr_of(a.plan);
+    pdl_wait();
+    if (h->sig != d.sig) return;
+    const int lane = threadIdx.x & 31;
+    const long long w = (long long)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
+    if (w >= (long long)d.T * d.nH) return;
+    const int tok = (int)(w / d.nH), hq = (int)(w % d.nH), head = hq / d.G, row = tok * d.G + hq % d.G;
+    if (tok < h->tok_lo || tok >= h->tok_hi) return;   // not a row of any sequence: left as it was
+    float M = -INFINITY, L = 0.f, v[PER];
+    #pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = 0.f;
+    auto add = [&](const float* p, float2 ml) {
+        const float mn = fmaxf(M, ml.x), mu = mn == -INFINITY ? 0.f : mn;
+        const float f0 = exp2_approx(M - mu), f1 = exp2_approx(ml.x - mu);
+        M = mn;
+        L = L * f0 + ml.y * f1;
+        #pragma unroll
+        for (int i = 0; i < PER; i += 4) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(p + lane * PER + i));
+            v[i] = v[i] * f0 + x.x * f1;
+            v[i + 1] = v[i + 1] * f0 + x.y * f1;
+            v[i + 2] = v[i + 2] * f0 + x.z * f1;
+            v[i + 3] = v[i + 3] * f0 + x.w * f1;
+        }
+    };
+    #pragma unroll 1
+    for (int seg = 0; seg < 2; seg++) {      // 0 prefix, 1 own
+        const int ref = at<int>(a.plan, seg ? d.row_own : d.row_pre)[row];
+        if (seg == 0 && ref == -1) continue;
+        const int kind = (unsigned)ref >> 31;
+        const Tile& t = at<Tile>(a.plan, d.tiles[kind])[ref & 0x7fffffff];
+        if (t.n == 0) continue;
+        const Span sp = span_of(h, kind, t.off, t.n, head);
+        if (sp.c0 == sp.c1) {
+            if (t.solo) return;              // written by its tile
+            const size_t slot = ((size_t)seg * d.T + tok) * d.nH + hq;
+            add(a.w.row + slot * HD, __ldcg(a.w.row_ml + slot));
+        } else {
+            const int br = kind ? kRowsP : kRowsS, r = row - t.row0;
+            #pragma unroll 4
+            for (int c = sp.c0; c <= sp.c1; c++) {
+                const size_t slot = ((size_t)c * 2 + (c == sp.c0 ? 1 : 0)) * br + r;
+                add(a.w.edge[kind] + slot * HD, __ldcg(a.w.edge_ml[kind] + slot));
+            }
+        }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const long long o = (long long)tok * a.out_stride + (long long)hq * HD + lane * PER;
+    #pragma unroll
+    for (int i = 0; i < PER; i++) v[i] *= inv;
+    if (a.out_f32) {
+        #pragma unroll
+        for (int i = 0; i < PER; i += 4)
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o + i) =
+                make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else {
+        store_half<PER>(reinterpret_cast<uint16_t*>(a.out) + o, v);
+    }
+}
+
+// a launch that may begin while the kernel before it in the stream finishes
+template <typename K, typename... A>
+static cudaError_t launch_pdl(K k, dim3 grid, int threads, size_t smem, cudaStream_t s, const A&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
+template <int HD>
+static cudaError_t launch_few(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+    using C = FewCfg<HD>;
+    cudaError_t e = cudaFuncSetAttribute(few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    few_kernel<HD><<<a.d.ctas[0], 32 * kFewWarps, C::SMEM, s>>>(a, km, vm);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    const long long rows = (long long)a.d.T * a.d.nH, per = kJoinThreads / 32;
+    return launch_pdl(join_kernel<HD>, dim3((unsigned)((rows + per - 1) / per)), kJoinThreads, 0, s, a);
+}
+
+template <bool XF32>
+static void launch_append(const AppendArgs& a, dim3 grid, cudaStream_t s) {
+    if (a.d.hd == 128) append_kernel<128, XF32><<<grid, kAppendThreads, 0, s>>>(a);
+    else if (a.d.hd == 256) append_kernel<256, XF32><<<grid, kAppendThreads, 0, s>>>(a);
+    else append_kernel<512, XF32><<<grid, kAppendThreads, 0, s>>>(a);
+}
+
+bool many_rows(int) { return false; }
+}  // namespace pg
+
+unsigned read_status_paged() {
+    unsigned v = 0;
+    if (cudaMemcpyFromSymbol(&v, pg::g_status_paged, sizeof(v)) != cudaSuccess) return 0xffffffffu;
+    if (v) {
+        const unsigned zero = 0;
+        cudaMemcpyToSymbol(pg::g_status_paged, &zero, sizeof(zero));
+    }
+    return v;
+}
+
+}  // namespace g4b
+
+using namespace g4b;
+using namespace g4b::pg;
+
+extern "C" {
+
+size_t g4b_paged_plan_bytes(int T, int B, int nH, int nkv, int hd, int page_size, int table_pages, int prefix_pages,
+                            int window) {
+    Dims d;
+    clear_error();
+    return make_dims("paged_plan_bytes", T, B, nH, nkv, hd, page_size, table_pages, prefix_pages, window, d) == G4B_OK
+               ? d.bytes
+               : 0;
+}
+
+size_t g4b_paged_workspace_bytes(int T, int B, int nH, int nkv, int hd, int page_size, int table_pages,
+                                 int prefix_pages, int window) {
+    Dims d;
+    clear_error();
+    return make_dims("paged_workspace_bytes", T, B, nH, nkv, hd, page_size, table_pages, prefix_pages, window, d) ==
+                   G4B_OK
+               ? work_bytes(d, nullptr, nullptr)
+               : 0;
+}
+
+int g4b_paged_plan(const int* q_start, const int* kv_len, const int* prefix_len, int T, int B, int nH, int nkv, int hd,
+                   int page_size, int table_pages, int prefix_pages, int window, void* plan, size_t plan_bytes,
+                   g4b_stream_t stream) {
+    G4B_ENTRY("paged_plan");
+    G4B_REQUIRE(q_start && kv_len && plan, G4B_E_ARG, "paged_plan: NULL pointer");
+    G4B_REQUIRE(prefix_pages == 0 || prefix_len, G4B_E_ARG, "paged_plan: %d prefix pages without prefix_len",
+                prefix_pages);
+    PlanArgs a{};
+    int st = make_dims("paged_plan", T, B, nH, nkv, hd, page_size, table_pages, prefix_pages, window, a.d);
+    if (st != G4B_OK) return st;
+    G4B_REQUIRE(aligned16(plan), G4B_E_ALIGN, "paged_plan: the plan must be 16-byte aligned");
+    G4B_REQUIRE(plan_bytes >= a.d.bytes, G4B_E_WORKSPACE, "paged_plan: needs %zu bytes, got %zu", a.d.bytes,
+                plan_bytes);
+    st = check_device(nullptr);
+    if (st != G4B_OK) return st;
+    a.q_start = q_start;
+    a.kv_len = kv_len;
+    a.prefix_len = prefix_pages > 0 ? prefix_len : nullptr;
+    a.plan = plan;
+    a.many = many_rows(hd) ? 1 : 0;
+    const int smem = (3 * B + 1) * 4;
+    cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return fail(G4B_E_CUDA, "paged_plan: %s", cudaGetErrorString(e));
+    const int rows = T * a.d.G;
+    const int grid = std::min(64, (rows + 4 * kPlanThreads - 1) / (4 * kPlanThreads));
+    plan_kernel<<<grid, kPlanThreads, smem, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+    count_launch();
+    return launch_status("paged_plan");
+}
+
+int g4b_paged_append(const void* qkv, int dtype, long long row_stride, const float* qnw, const float* knw,
+                     const float* cos_tab, const float* sin_tab, int n_pos, uint16_t* kc, uint16_t* vc, int num_pages,
+                     const int* table, uint16_t* q_out, long long q_stride, int T, int B, int nH, int nkv, int hd,
+                     int koff, int voff, int page_size, int table_pages, int prefix_pages, int window,
+                     const void* plan, g4b_stream_t stream) {
+    G4B_ENTRY("paged_append");
+    G4B_REQUIRE(qkv && qnw && knw && cos_tab && sin_tab && kc && vc && table && q_out && plan, G4B_E_ARG,
+                "paged_append: NULL pointer");
+    G4B_REQUIRE(dtype == G4B_DT_F32 || dtype == G4B_DT_F16, G4B_E_ARG, "paged_append: bad dtype %d", dtype);
+    AppendArgs a{};
+    int st = make_dims("paged_append", T, B, nH, nkv, hd, page_size, table_pages, prefix_pages, window, a.d);
+    if (st != G4B_OK) return st;
+    G4B_REQUIRE(num_pages >= 1 && (long long)num_pages * nkv * page_size <= 0x7fff0000LL, G4B_E_SHAPE,
+                "paged_append: %d pages of %d rows of %d heads", num_pages, page_size, nkv);
+    G4B_REQUIRE(n_pos >= (table_pages + prefix_pages) * page_size, G4B_E_SHAPE,
+                "paged_append: rotations of %d positions, the tables hold %d", n_pos,
+                (table_pages + prefix_pages) * page_size);
+    G4B_REQUIRE(koff >= 0 && voff >= 0 && koff % 8 == 0 && voff % 8 == 0 && row_stride % 8 == 0 && q_stride % 8 == 0 &&
+                    q_stride >= (long long)nH * hd && row_stride >= (long long)nH * hd &&
+                    row_stride >= (long long)koff + (long long)nkv * hd && row_stride >= (long long)voff + (long long)nkv * hd,
+                G4B_E_SHAPE, "paged_append: row_stride=%lld q_stride=%lld koff=%d voff=%d (multiples of 8, rows inside)",
+                row_stride, q_stride, koff, voff);
+    G4B_REQUIRE(aligned16(qkv) && aligned16(qnw) && aligned16(knw) && aligned16(cos_tab) && aligned16(sin_tab) &&
+                    aligned16(kc) && aligned16(vc) && aligned16(q_out) && aligned16(plan),
+                G4B_E_ALIGN, "paged_append: qkv, the weights, the rotations, the caches, q_out and the plan must be "
+                "16-byte aligned");
+    a.plan = plan;
+    a.qkv = qkv;
+    a.qnw = qnw;
+    a.knw = knw;
+    a.cos_t = cos_tab;
+    a.sin_t = sin_tab;
+    a.kc = kc;
+    a.vc = vc;
+    a.table = table;
+    a.q_out = q_out;
+    a.row_stride = row_stride;
+    a.q_stride = q_stride;
+    a.koff = koff;
+    a.voff = voff;
+    a.num_pages = num_pages;
+    st = check_device(nullptr);
+    if (st != G4B_OK) return st;
+    // few tokens: one head per warp; many: a token per CTA, whose warps keep the rotation for their heads
+    const int heads = nH + 2 * nkv, per = kAppendThreads / 32;
+    const int y = T >= 256 ? 1 : std::min(65535, (heads + per - 1) / per);
+    const dim3 grid(T, y);
+    if (dtype == G4B_DT_F32) launch_append<true>(a, grid, reinterpret_cast<cudaStream_t>(stream));
+    else launch_append<false>(a, grid, reinterpret_cast<cudaStream_t>(stream));
+    count_launch();
+    return launch_status("paged_append");
+}
+
+int g4b_paged_attn(const uint16_t* q, long long q_stride, const uint16_t* kc, const uint16_t* vc, int num_pages,
+                   const int* table, const int* prefix_table, void* out, int out_dtype, long long out_stride,
+                   float scale, int T, int B, int nH, int nkv, int hd, int page_size, int table_pages,
+                   int prefix_pages, int window, const void* plan, void* workspace, size_t ws_bytes,
+                   g4b_stream_t stream) {
+    G4B_ENTRY("paged_attn");
+    G4B_REQUIRE(q && kc && vc && table && out && plan, G4B_E_ARG, "paged_attn: NULL pointer");
+    G4B_REQUIRE(prefix_pages == 0 || prefix_table, G4B_E_ARG, "paged_attn: %d prefix pages without prefix_table",
+                prefix_pages);
+    G4B_REQUIRE(out_dtype == G4B_DT_F32 || out_dtype == G4B_DT_F16, G4B_E_ARG, "paged_attn: bad out_dtype %d",
+                out_dtype);
+    G4B_REQUIRE(scale > 0.f && scale < 1e30f, G4B_E_ARG, "paged_attn: scale=%g (positive and finite)", (double)scale);
+    Args a{};
+    int st = make_dims("paged_attn", T, B, nH, nkv, hd, page_size, table_pages, prefix_pages, window, a.d);
+    if (st != G4B_OK) return st;
+    G4B_REQUIRE(num_pages >= 1 && (long long)num_pages * nkv * page_size <= 0x7fff0000LL, G4B_E_SHAPE,
+                "paged_attn: %d pages of %d rows of %d heads", num_pages, page_size, nkv);
+    G4B_REQUIRE(q_stride >= (long long)nH * hd && out_stride >= (long long)nH * hd && q_stride % 8 == 0 &&
+                    out_stride % 8 == 0,
+                G4B_E_SHAPE, "paged_attn: q_stride=%lld out_stride=%lld (multiples of 8, >= nH * hd)", q_stride,
+                out_stride);
+    G4B_REQUIRE(aligned16(q) && aligned16(kc) && aligned16(vc) && aligned16(out) && aligned16(plan), G4B_E_ALIGN,
+                "paged_attn: q, the caches, out and the plan must be 16-byte aligned");
+    const size_t need = work_bytes(a.d, nullptr, nullptr);
+    G4B_REQUIRE(workspace && aligned16(workspace) && ws_bytes >= need, G4B_E_WORKSPACE,
+                "paged_attn: needs a 16-byte aligned workspace of %zu bytes, got %zu", need, ws_bytes);
+    work_bytes(a.d, reinterpret_cast<char*>(workspace), &a.w);
+    a.plan = plan;
+    a.q = q;
+    a.kc = kc;
+    a.vc = vc;
+    a.table = table;
+    a.pre_table = prefix_table;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.scale = scale * 1.4426950408889634f;
+    a.out_f32 = out_dtype == G4B_DT_F32;
+    a.num_pages = num_pages;
+    st = check_device(nullptr);
+    if (st != G4B_OK) return st;
+    CUtensorMap km, vm;
+    const uint64_t rows = (uint64_t)num_pages * nkv * page_size;
+    for (int i = 0; i < 2; i++) {
+        st = tensor_map_2d(i ? &vm : &km, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, i ? vc : kc, hd, rows, (uint64_t)hd * 2, 64,
+                           kBlk, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (st != G4B_OK) return st;
+    }
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e = hd == 128 ? launch_few<128>(a, km, vm, s)
+                  : hd == 256 ? launch_few<256>(a, km, vm, s)
+                              : launch_few<512>(a, km, vm, s);
+    if (e != cudaSuccess) return fail(G4B_E_CUDA, "paged_attn: launch: %s", cudaGetErrorString(e));
+    count_launch(2);
+    return launch_status("paged_attn");
+}
+
+}  // extern "C"

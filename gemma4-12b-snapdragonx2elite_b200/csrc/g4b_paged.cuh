@@ -1,0 +1,114 @@
+// g4b_paged.cuh -- what the paged-cache kernels share: the plan of a ragged batch, its layout in the
+// caller's buffer, the walk over its pieces, and where a piece's partial result goes.
+//
+// A batch is B sequences with their new tokens back to back in rows [q_start[b], q_start[b + 1]) of the
+// token buffers.  Sequence b holds kv_len[b] tokens once its new ones are appended; its token i has
+// position kv_len[b] - n_b + i.  Positions below prefix_len live in the pages of one prefix table that all
+// sequences share, the others in the sequence's own table row.
+//
+// The attention of a KV head reads "segments": the prefix's keys for the rows of all sequences, and every
+// sequence's own keys for its own rows (row = token * G + query head of the group).  A segment is cut
+// into tiles of kRowsS or kRowsP rows; a tile is n units of 64 keys.  The units of all tiles and KV heads
+// form one line that is cut into equal lengths, one per CTA, whatever the lengths of the sequences: a CTA
+// walks its stretch piece by piece.  A tile that lies in one CTA's stretch is finished there; one that
+// crosses a border leaves a partial (running maximum, sum, weighted values) in the edge slots of each CTA,
+// and the join kernel adds them.
+#pragma once
+
+#include "g4b_common.cuh"
+#include "g4b_pages.h"
+
+namespace g4b {
+namespace pg {
+
+constexpr int kUnit = 64;        // keys per unit of work
+constexpr int kRowsS = 8;        // rows of a tile of the few-rows kernel (the n of m16n8k16)
+constexpr int kRowsP = 128;      // rows of a tile of the many-rows kernel (tensor memory lanes)
+constexpr int kMaxSeqs = 4096;   // the plan kernel keeps the sequences in shared memory
+constexpr unsigned kStatusPlan = 2u;   // a plan made for other sizes (or never made) was passed
+
+struct Tile {
+    int row0;        // first row: token * G + g
+    int nrows;       // rows of the tile
+    int seq;         // sequence whose own keys it reads; -1: the shared prefix
+    int lo, hi;      // keys [lo, hi) of the segment; lo is a multiple of kUnit
+    int n;           // units
+    int solo;        // its rows have keys in no other segment: a whole tile writes the output itself
+    int pad;
+    long long off;   // units of the tiles before it
+    long long pad2;
+};
+
+struct Start {       // where a CTA's stretch begins
+    int head, tile, unit, pad;
+};
+
+struct Hdr {
+    unsigned sig;                    // of the sizes the plan was made for
+    int prefix_len;
+    int tok_lo, tok_hi;              // rows of the token buffers that belong to a sequence
+    int nt[2];                       // tiles: [0] few rows, [1] many rows
+    int pad[2];
+    long long wt[2];                 // units of one KV head
+    long long u[2];                  // units per CTA
+};
+
+// sizes fixed on the host, and the offsets of the arrays in the plan buffer that follow from them
+struct Dims {
+    int T, B, nH, nkv, G, hd, ps, own_pages, pre_pages, window;
+    int ctas[2];                     // stretches per kind
+    int max_tiles[2];
+    size_t tok_seq, tok_pos, row_own, row_pre, start[2], tiles[2], bytes;
+    unsigned sig;
+};
+
+__host__ __device__ inline const Hdr* hdr_of(const void* plan) { return reinterpret_cast<const Hdr*>(plan); }
+template <typename X>
+__host__ __device__ inline X* at(void* plan, size_t off) {
+    return reinterpret_cast<X*>(reinterpret_cast<char*>(plan) + off);
+}
+template <typename X>
+__host__ __device__ inline const X* at(const void* plan, size_t off) {
+    return reinterpret_cast<const X*>(reinterpret_cast<const char*>(plan) + off);
+}
+
+// The workspace: edge slots of both kinds ([cta][2][rows][hd] sums, then [cta][2][rows] (max, sum)), then,
+// where there is a prefix, one slot per (segment kind, token, head) for whole tiles.
+struct Work {
+    float* edge[2];
+    float2* edge_ml[2];
+    float* row;        // [2][T * nH][hd]: 0 prefix, 1 own
+    float2* row_ml;
+};
+
+struct Args {
+    const void* plan;
+    const uint16_t* q;
+    const uint16_t* kc;
+    const uint16_t* vc;
+    const int* table;
+    const int* pre_table;
+    void* out;
+    Work w;
+    long long q_stride, out_stride;
+    float scale;       // times log2(e): scores are kept in powers of two
+    int out_f32, num_pages;
+    Dims d;
+};
+
+__device__ __forceinline__ Span span_of(const Hdr* h, int kind, long long off, int n, int head) {
+    return span_of((long long)head * h->wt[kind] + off, n, h->u[kind]);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// many-rows tiles are for these head widths (the kernel of g4b_paged_mma.cu)
+bool many_rows(int hd);
+int launch_many(const Args& a, cudaStream_t s);
+
+}  // namespace pg
+}  // namespace g4b

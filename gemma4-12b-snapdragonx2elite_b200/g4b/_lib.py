@@ -50,6 +50,7 @@ _P = C.c_void_p
 _I = C.c_int
 _F = C.c_float
 _Z = C.c_size_t
+_LL = C.c_longlong
 class GemmSeg(C.Structure):
     """g4b_gemm_seg: one weight of g4b_gemm_i4_fused."""
     _fields_ = [("wp", C.c_void_p), ("scales_f16", C.c_void_p), ("y", C.c_void_p), ("N", C.c_int)]
@@ -97,6 +98,12 @@ SIGNATURES = {
                                     _P, _P, _Z, _P]),
     "g4b_rows_rmsnorm": (_I, [_P, _I, _P, _P, _I, _I, _I, _P]),
     "g4b_rows_normadd": (_I, [_P, _I, _P, _P, _I, _I, _F, _P]),
+    "g4b_rows_normadd_i8": (_I, [_P, _I, _P, _P, _P, _F, _P, _P, _P, _I, _I, _P]),
+    "g4b_paged_plan_bytes": (_Z, [_I] * 9),
+    "g4b_paged_plan": (_I, [_P, _P, _P] + [_I] * 9 + [_P, _Z, _P]),
+    "g4b_paged_append": (_I, [_P, _I, _LL, _P, _P, _P, _P, _I, _P, _P, _I, _P, _P, _LL] + [_I] * 11 + [_P, _P]),
+    "g4b_paged_workspace_bytes": (_Z, [_I] * 9),
+    "g4b_paged_attn": (_I, [_P, _LL, _P, _P, _I, _P, _P, _P, _I, _LL, _F] + [_I] * 9 + [_P, _P, _Z, _P]),
     "g4b_gelumul": (_I, [_P, _P, _I, _P, _I, _Z, _P]),
     "g4b_attn_prefill_prepkv": (_I, [_P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P]),
     "g4b_attn_prefill": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P]),

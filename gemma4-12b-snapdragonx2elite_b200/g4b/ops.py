@@ -37,6 +37,36 @@ def _need(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must be contiguous")
 
 
+class _on:
+    """The device of a call's tensors as the current one, and `stream` as the current stream, for as long as the
+    call allocates and launches: what it allocates is then ordered with the stream that uses it."""
+    __slots__ = ("dev", "stream")
+
+    def __init__(self, device: torch.device, stream: Optional[torch.cuda.Stream]):
+        index = torch.cuda.current_device() if device.index is None else device.index
+        self.dev = torch.cuda.device(index) if index != torch.cuda.current_device() else None
+        self.stream = None if stream is None else torch.cuda.stream(stream)
+
+    def __enter__(self):
+        if self.dev is not None:
+            self.dev.__enter__()
+        if self.stream is not None:
+            self.stream.__enter__()
+
+    def __exit__(self, *exc):
+        if self.stream is not None:
+            self.stream.__exit__(*exc)
+        if self.dev is not None:
+            self.dev.__exit__(*exc)
+
+
+def _rows_shape(op: str, t: torch.Tensor, name: str):
+    _need(t, name)
+    if t.dim() != 2 or t.dtype != torch.float32:
+        raise ValueError(f"{op}: {name} must be [rows, D] f32, got {tuple(t.shape)} {t.dtype}")
+    return t.shape
+
+
 @dataclass
 class DeviceWeight:
     """One packed linear layer resident in HBM (the reference's Buf set for a layer)."""
@@ -592,3 +622,35 @@ def gelumul(gate: torch.Tensor, up: torch.Tensor, out: Optional[torch.Tensor] = 
         _ptr(gate), _ptr(up), _DT[gate.dtype], _ptr(out), _DT[out.dtype], gate.numel(),
         _stream_handle(stream, gate.device)))
     return out
+
+
+def rows_normadd_i8(x: Optional[torch.Tensor], h: torch.Tensor, w: torch.Tensor, w_post: Optional[torch.Tensor] = None,
+                    scl: float = 1.0, h_out: Optional[torch.Tensor] = None, A8: Optional[torch.Tensor] = None,
+                    sa: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None):
+    """rows_normadd, the next rows_rmsnorm and cast_i8 in one pass over the rows of h [M, D] (f32):
+    h' = (h + rmsnorm(x) * w_post) * scl (w_post None: (h + x) * scl; x None: h * scl) and
+    (A8, sa) = cast_i8(rmsnorm(h') * w), gemm_w8a8's operand.  Returns (A8 [M, D] int8, sa [M] f32).
+
+    h' is written to h_out, or to h where none is given."""
+    M, D = _rows_shape("rows_normadd_i8", h, "h")
+    for t, n, shape in ((x, "x", (M, D)), (w, "w", (D,)), (w_post, "w_post", (D,)), (h_out, "h_out", (M, D)),
+                        (A8, "A8", (M, D)), (sa, "sa", (M,))):
+        if t is None:
+            continue
+        _need(t, n)
+        if t.device != h.device or tuple(t.shape) != shape:
+            raise ValueError(f"rows_normadd_i8: {n} is {tuple(t.shape)} on {t.device}, want {shape} on {h.device}")
+        want = {"x": (torch.float32, torch.float16), "A8": (torch.int8,)}.get(n, (torch.float32,))
+        if t.dtype not in want:
+            raise TypeError(f"rows_normadd_i8: {n} is {t.dtype}")
+    with _on(h.device, stream):
+        if A8 is None:
+            A8 = torch.empty((M, D), dtype=torch.int8, device=h.device)
+        if sa is None:
+            sa = torch.empty((M,), dtype=torch.float32, device=h.device)
+        if h_out is None and (x is not None or scl != 1.0):
+            h_out = h
+        L.check("g4b_rows_normadd_i8", L.load().g4b_rows_normadd_i8(
+            _ptr(x), L.DT_F32 if x is None else _DT[x.dtype], _ptr(w_post), _ptr(h), _ptr(h_out), float(scl), _ptr(w),
+            _ptr(A8), _ptr(sa), M, D, _stream_handle(stream, h.device)))
+    return A8, sa

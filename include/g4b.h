@@ -70,8 +70,10 @@ typedef struct CUstream_st* g4b_stream_t;
 #define G4B_Q_LAUNCHES       3  /* kernels this process has launched through g4b   */
 #define G4B_Q_FAULT_COUNTER  4  /* calls seen by the fault injector                */
 #define G4B_Q_KERNEL_STATUS  5  /* read-and-clear the kernels' device status word:
-                                   0 = clean, 1 = a bounded wait timed out (the
-                                   kernel gave up and its outputs are invalid);
+                                   0 = clean, bit 0 = a bounded wait timed out (the
+                                   kernel gave up and its outputs are invalid),
+                                   bit 1 = a paged call was given a plan made for
+                                   other sizes, or none (it wrote nothing);
                                    synchronises the device */
 
 /* --------------------------------------------------------------- utilities */
@@ -517,6 +519,67 @@ G4B_API int g4b_attn_prefill(const void* q, int dtype, int q_stride, int M, cons
                              int out_stride, int nH, int nkv, int hd, int stride, int window, const int* p0_dev,
                              g4b_stream_t stream);
 
+/* ------------------------------------------------------------ batches over a paged KV cache */
+/* The engine serves one sequence from a contiguous cache (src/vk_engine.py:281-282, 416-417).  These calls
+ * serve a ragged batch of B sequences whose caches are made of pages, with a prefix that all of them share
+ * kept, and read, once.
+ *
+ *   cache         kc, vc [num_pages, nkv, page_size, hd] f16; page_size a power of two, 16 to 1024
+ *   tokens        the sequences' new tokens back to back: sequence b has rows q_start[b] .. q_start[b+1] - 1
+ *                 of the token buffers (T rows; rows outside q_start[0] .. q_start[B] - 1 are padding and
+ *                 are neither read into a result nor written).  A sequence may have no new token.
+ *   positions     kv_len[b] counts the tokens sequence b holds with its new ones, the shared prefix
+ *                 included: its token i of n has position kv_len[b] - n + i
+ *   pages         position p < *prefix_len is in page prefix_table[p / page_size], any other in page
+ *                 table[b][(p - *prefix_len) / page_size], at p's (p - *prefix_len's) remainder.  The prefix
+ *                 may end inside a page.  table is [B, table_pages], prefix_table [prefix_pages], int32.
+ *                 An id outside [0, num_pages) is a page that is not there: nothing is written to it and
+ *                 its keys are not attended to.
+ *   device data   q_start, kv_len, *prefix_len and the tables are int32 in device memory, so a captured
+ *                 graph serves every step.  q_start is read as its running maximum within [0, T], lengths
+ *                 are cut to [0, capacity of the tables]: no value of theirs makes a call leave its buffers.
+ *
+ * A step first makes a plan of the batch, which all its layers of one kind (same heads and window) use:
+ * g4b_paged_plan reads q_start, kv_len and *prefix_len once and lays the work of the attention out over the
+ * SMs.  The later calls take the same sizes; given a plan of other sizes they write nothing and raise
+ * G4B_Q_KERNEL_STATUS bit 1.  Sizes: hd 128, 256 or 512; nH a multiple of nkv; B <= 4096;
+ * (table_pages + prefix_pages) * page_size <= 2^30; window 0 (none) or the keys a token sees, itself included. */
+G4B_API size_t g4b_paged_plan_bytes(int T, int B, int nH, int nkv, int hd, int page_size, int table_pages,
+                                    int prefix_pages, int window);
+G4B_API int g4b_paged_plan(const int* q_start, const int* kv_len, const int* prefix_len, int T, int B, int nH, int nkv,
+                           int hd, int page_size, int table_pages, int prefix_pages, int window, void* plan,
+                           size_t plan_bytes, g4b_stream_t stream);
+
+/* The new tokens' keys and values into their pages and their queries ready for g4b_paged_attn, the prepkv
+ * dispatch (vk/prepkv.comp:14-31) and the query half of attn (vk/attn.comp:22-28) for a batch: for the token
+ * in row t, at position p,
+ *   k = RoPE_p(rmsnorm(qkv[t, koff + h*hd ..], knw)),  v = qkv[t, voff + h*hd ..] * rsqrt(mean(v^2) + 1e-6)
+ *     -> f16 at p's place in kc / vc   (koff == voff: v is the unrotated k, attention_k_eq_v),
+ *   q_out[t, h*hd ..] = f16(RoPE_p(rmsnorm(qkv[t, h*hd ..], qnw)))       (q heads at offset 0)
+ * with the rotation rows p of cos_tab / sin_tab [n_pos, hd] f32, n_pos >= the tables' positions.  Keys and
+ * values at positions below *prefix_len are not written (the shared pages hold them).  qkv f32 or f16 with
+ * row_stride elements between rows, q_out f16 with q_stride; strides and offsets multiples of 8.  No two
+ * tokens of a call may have the same place in the cache. */
+G4B_API int g4b_paged_append(const void* qkv, int dtype, long long row_stride, const float* qnw, const float* knw,
+                             const float* cos_tab, const float* sin_tab, int n_pos, uint16_t* kc, uint16_t* vc,
+                             int num_pages, const int* table, uint16_t* q_out, long long q_stride, int T, int B, int nH,
+                             int nkv, int hd, int koff, int voff, int page_size, int table_pages, int prefix_pages,
+                             int window, const void* plan, g4b_stream_t stream);
+
+/* Attention of the new tokens over their sequences' pages: for the token in row t at position p, query head h,
+ *   out[t, h*hd ..] = sum_j softmax_j(scale * q_t,h . k_j) v_j over the positions j <= p, j > p - window if window > 0.
+ * The prefix's keys and values are read once for the rows of all sequences, a sequence's own once for its rows.
+ * A token that sees no key gets zeros.  q f16 [T, q_stride]; out f16 or f32 [T, out_stride]; strides multiples of 8.
+ * f32 scores, maxima, sums and accumulators.  The workspace (g4b_paged_workspace_bytes) needs no
+ * initialisation; calls that share one, or a plan, must be ordered. */
+G4B_API size_t g4b_paged_workspace_bytes(int T, int B, int nH, int nkv, int hd, int page_size, int table_pages,
+                                         int prefix_pages, int window);
+G4B_API int g4b_paged_attn(const uint16_t* q, long long q_stride, const uint16_t* kc, const uint16_t* vc, int num_pages,
+                           const int* table, const int* prefix_table, void* out, int out_dtype, long long out_stride,
+                           float scale, int T, int B, int nH, int nkv, int hd, int page_size, int table_pages,
+                           int prefix_pages, int window, const void* plan, void* workspace, size_t ws_bytes,
+                           g4b_stream_t stream);
+
 /* ------------------------------------------------------------ prefill element-wise rows */
 /* The prefill layer's norm and activation dispatches over [M, D] token rows
  * (src/vk_engine.py:413-424), one CTA per row for the norms:
@@ -532,6 +595,17 @@ G4B_API int g4b_rows_normadd(const void* x, int x_dtype, const float* w, float* 
                              g4b_stream_t stream);
 G4B_API int g4b_gelumul(const void* gate, const void* up, int dtype, void* out, int out_dtype, size_t n,
                         g4b_stream_t stream);
+
+/* The residual's update, the next norm and the int8 quantiser in one pass over [M, D] rows: what
+ * g4b_rows_normadd, g4b_rows_rmsnorm and g4b_cast_i8 do between two W8A8 GEMMs (src/vk_engine.py:392-394, 413-424):
+ *   h' = (h + x * rsqrt(mean(x^2) + 1e-6) * w_post) * scl     (w_post NULL: (h + x) * scl;  x NULL: h * scl)
+ *   y  = h' * rsqrt(mean(h'^2) + 1e-6) * w
+ *   sa[m] = max(max_k |y[m,k]| / 127, 1e-12),  A8[m,k] = clamp(round_half_even(y[m,k] / sa[m]), -127, 127)
+ * x f32 or f16; h, w_post, w f32.  h' goes to h_out, which may be h itself (in place) but not overlap it
+ * otherwise; NULL: it is not stored.  The codes are formed without rounding y first, so one may differ by a
+ * step from the three calls' where y / sa is next to a half.  D is a multiple of 16. */
+G4B_API int g4b_rows_normadd_i8(const void* x, int x_dtype, const float* w_post, const float* h, float* h_out, float scl,
+                                const float* w, int8_t* A8, float* sa, int M, int D, g4b_stream_t stream);
 
 /* ------------------------------------------------------------ tensor parallel */
 /* The all-reduce after the row-parallel o and down GEMVs of a tensor-parallel

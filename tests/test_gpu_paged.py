@@ -1,0 +1,482 @@
+"""Batches over a paged KV cache (g4b_paged_plan, g4b_paged_append, g4b_paged_attn) against the definitions in
+64 bits, computed with plain torch one sequence at a time.
+
+Every cache starts as NaN; only the places that the batch may read hold numbers, so a value taken from behind a
+mask, from another page or from a row that is not there shows at once.  Tolerances count roundings:
+  append  an output is rounded to f16 once (2^-11 of its value, 2^-25 below the normal range); its f32 path
+          makes under 16 roundings of terms no larger than |n cos| + |partner sin|: 2^-20 of that sum.
+  attend  the output's rounding (2^-11 f16, 2^-24 f32), and on every weight: its own rounding to f16 (2^-11, where
+          many rows share a tile), the exponential (2^-21), and twice the error of a score, which is at most
+          hd 2^-23 of sum |q_i k_i| scale (f32 sums of exact products, truncated or rounded, in any order).  An error of d on
+          every weight moves an output by at most 2 d sum_j p_j |v_j|."""
+import numpy as np
+import pytest
+import torch
+
+from g4b import _lib as L
+from g4b import ops
+from g4b.paged import PagedPlan
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F64 = torch.float64
+
+
+class Batch:
+    """A ragged batch: new[b] tokens for sequence b, total[b] held with them, `prefix` of those shared."""
+
+    def __init__(self, nH, nkv, hd, page, new, total, prefix=0, window=0, seed=0, front=0, back=0, spare_pages=5,
+                 prefix_pages=None):
+        self.nH, self.nkv, self.hd, self.page, self.window, self.prefix = nH, nkv, hd, page, window, prefix
+        self.new, self.total, self.B = list(new), list(total), len(new)
+        self.start = np.concatenate([[0], np.cumsum(new)]).astype(np.int64) + front
+        self.T = int(self.start[-1]) + back
+        rng = np.random.default_rng(seed)
+        self.pre_pages = -(-prefix // page) if prefix_pages is None else prefix_pages
+        self.own_pages = max([1] + [-(-(t - prefix) // page) for t in total])
+        self.pages = self.pre_pages + self.B * self.own_pages + spare_pages
+        order = rng.permutation(self.pages).astype(np.int32)
+        self.pre_ids = order[:self.pre_pages]
+        self.ids = order[self.pre_pages:self.pre_pages + self.B * self.own_pages].reshape(self.B, self.own_pages)
+        self.g = torch.Generator(device=DEV).manual_seed(seed)
+        t32 = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(DEV)  # noqa: E731
+        self.q_start, self.kv_len, self.table = t32(self.start), t32(self.total), t32(self.ids)
+        self.prefix_table = t32(self.pre_ids) if self.pre_pages else None
+        self.prefix_len = t32([prefix]) if self.pre_pages else None
+        self.kc = torch.full((self.pages, nkv, page, hd), float("nan"), dtype=torch.float16, device=DEV)
+        self.vc = torch.full_like(self.kc, float("nan"))
+
+    def place(self, b, p):
+        """(page, slot) of position p of sequence b."""
+        if p < self.prefix:
+            return int(self.pre_ids[p // self.page]), p % self.page
+        return int(self.ids[b, (p - self.prefix) // self.page]), (p - self.prefix) % self.page
+
+    def places(self, b, n):
+        at = [self.place(b, p) for p in range(n)]
+        return (torch.tensor([x[0] for x in at], dtype=torch.long, device=DEV),
+                torch.tensor([x[1] for x in at], dtype=torch.long, device=DEV))
+
+    def randn(self, *s, dtype=torch.float32):
+        return torch.randn(*s, generator=self.g, device=DEV, dtype=dtype)
+
+    def fill(self):
+        """Numbers at every position that a token may see."""
+        done = 0
+        for b in sorted(range(self.B), key=lambda b: -self.total[b]):
+            n = self.total[b]
+            lo = min(done, self.prefix)       # the longest sequence fills the prefix
+            pg, sl = self.places(b, n)
+            pg, sl = pg[lo:], sl[lo:]
+            self.kc[pg, :, sl] = self.randn(len(pg), self.nkv, self.hd, dtype=torch.float16)
+            self.vc[pg, :, sl] = self.randn(len(pg), self.nkv, self.hd, dtype=torch.float16)
+            done = max(done, min(n, self.prefix))
+        return self
+
+    def queries(self, std=4.0):
+        return self.randn(self.T, self.nH * self.hd, dtype=torch.float16) * (std * self.hd ** -0.5)
+
+    def plan(self, T=None):
+        p = PagedPlan(self.T, self.B, self.nH, self.nkv, self.hd, self.page, self.own_pages, self.pre_pages,
+                      self.window, DEV)
+        p.update(self.q_start, self.kv_len, self.prefix_len)
+        return p
+
+    def reference(self, q, scale=1.0, bad_pages=()):
+        """(out, tolerance without the output's rounding) [T, nH, hd] in 64 bits; padding rows are NaN."""
+        out = torch.full((self.T, self.nH, self.hd), float("nan"), dtype=F64, device=DEV)
+        tol = torch.zeros_like(out)
+        G = self.nH // self.nkv
+        for b in range(self.B):
+            n, t0, total = self.new[b], int(self.start[b]), self.total[b]
+            if n == 0:
+                continue
+            pg, sl = self.places(b, total)
+            k, v = self.kc[pg, :, sl].to(F64), self.vc[pg, :, sl].to(F64)      # [total, nkv, hd]
+            j = torch.arange(total, device=DEV)
+            there = torch.ones(total, dtype=torch.bool, device=DEV)
+            for x in bad_pages:
+                there &= pg != x
+            for i0 in range(0, n, 128):
+                m = min(128, n - i0)
+                pos = torch.arange(total - n + i0, total - n + i0 + m, device=DEV)
+                see = (j[None] <= pos[:, None]) & there[None]
+                if self.window:
+                    see &= j[None] > pos[:, None] - self.window
+                qq = q[t0 + i0:t0 + i0 + m].to(F64).view(m, self.nkv, G, self.hd)
+                used = see.any(0)
+                kk = torch.where(used[:, None, None], k, torch.zeros_like(k))
+                vv = torch.where(used[:, None, None], v, torch.zeros_like(v))
+                s = torch.einsum("mkgd,jkd->mkgj", qq, kk) * scale
+                s = torch.where(see[:, None, None], s, torch.full_like(s, float("-inf")))
+                top = s.amax(-1, keepdim=True) if total else s.new_zeros(m, self.nkv, G, 1)
+                p = torch.exp(s - torch.where(torch.isinf(top), torch.zeros_like(top), top))
+                den = p.sum(-1, keepdim=True)
+                p = p / torch.where(den == 0, torch.ones_like(den), den)
+                mag = torch.einsum("mkgd,jkd->mkgj", qq.abs(), kk.abs()) * scale
+                mag = torch.where(see[:, None, None], mag, torch.zeros_like(mag)).amax(-1, keepdim=True) if total else 0
+                d = 2.0 ** -11 + 2.0 ** -21 + 2 * self.hd * 2.0 ** -23 * mag
+                o = torch.einsum("mkgj,jkd->mkgd", p, vv)
+                a = torch.einsum("mkgj,jkd->mkgd", p, vv.abs())
+                out[t0 + i0:t0 + i0 + m] = o.reshape(m, self.nH, self.hd)
+                tol[t0 + i0:t0 + i0 + m] = (2 * d * a).reshape(m, self.nH, self.hd)
+        return out, tol
+
+    def check(self, got, q, scale=1.0, bad_pages=()):
+        ref, tol = self.reference(q, scale, bad_pages)
+        got64 = got.to(F64).view(self.T, self.nH, self.hd)
+        eps = torch.finfo(got.dtype).eps / 2
+        lo, hi = int(self.start[0]), int(self.start[-1])
+        err = (got64 - ref).abs()[lo:hi]
+        lim = (tol + eps * ref.abs() + 2.0 ** -25)[lo:hi]
+        assert torch.isfinite(got64[lo:hi]).all()
+        worst = (err - lim).max().item() if err.numel() else 0.0
+        assert worst <= 0, f"off by {err.max().item():.3e}, {(err / lim).max().item():.2f} of the tolerance"
+        assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+def _attend(bt, q, plan=None, out_dtype=torch.float16, scale=1.0, out=None):
+    plan = plan or bt.plan()
+    if out is None:
+        out = torch.full((bt.T, bt.nH * bt.hd), 7.0, dtype=out_dtype, device=DEV)
+    plan.attend(q, bt.kc, bt.vc, bt.table, bt.prefix_table, out=out, scale=scale)
+    torch.cuda.synchronize()
+    return out
+
+
+HEADS = [(16, 8, 256), (8, 1, 128), (4, 2, 512), (6, 2, 128), (3, 3, 256), (16, 1, 512)]
+
+
+@pytest.mark.parametrize("nH,nkv,hd", HEADS)
+@pytest.mark.parametrize("page,new,total,prefix,window", [
+    (64, [1], [1], 0, 0),                                     # one token, one key
+    (64, [1], [700], 0, 0),
+    (16, [1, 1, 1], [5, 64, 65], 0, 0),
+    (32, [1, 1, 1, 1], [130, 101, 377, 102], 100, 0),         # the prefix ends inside a page
+    (128, [1] * 9, [200 + 37 * i for i in range(9)], 150, 64),  # a window that begins in the prefix for some only
+    (64, [2, 1, 4, 3], [300, 260, 259, 500], 256, 0),         # a few proposed tokens each
+])
+def test_decode_batches(nH, nkv, hd, page, new, total, prefix, window):
+    bt = Batch(nH, nkv, hd, page, new, total, prefix, window, seed=hd + nH).fill()
+    q = bt.queries()
+    bt.check(_attend(bt, q), q)
+
+
+@pytest.mark.parametrize("nH,nkv,hd", HEADS)
+@pytest.mark.parametrize("page,new,total,prefix,window", [
+    (64, [70], [70], 0, 0),                                   # a first prompt
+    (16, [33, 90], [40, 333], 0, 0),
+    (32, [130, 17, 1], [400, 217, 260], 200, 0),              # chunks behind a prefix, and a decode among them
+    (64, [150, 60], [391, 460], 230, 100),                    # window
+    (128, [65], [1300], 0, 129),
+])
+def test_prompt_chunks(nH, nkv, hd, page, new, total, prefix, window):
+    bt = Batch(nH, nkv, hd, page, new, total, prefix, window, seed=hd + page).fill()
+    q = bt.queries()
+    bt.check(_attend(bt, q), q)
+
+
+@pytest.mark.parametrize("nH,nkv,hd", [(16, 8, 256), (8, 1, 128)])
+def test_long_ragged_batch_over_a_prefix(nH, nkv, hd):
+    rng = np.random.default_rng(3)
+    new = [1] * 70
+    total = [5000 + int(x) for x in rng.integers(1, 900, 70)]
+    bt = Batch(nH, nkv, hd, 64, new, total, prefix=5000, seed=1).fill()
+    q = bt.queries()
+    bt.check(_attend(bt, q), q)
+
+
+@pytest.mark.parametrize("hd,nH,nkv", [(256, 16, 8), (512, 4, 2)])
+def test_f32_output_scale_and_strides(hd, nH, nkv):
+    bt = Batch(nH, nkv, hd, 32, [1, 40, 3], [90, 140, 33], 30, seed=5, back=2).fill()
+    wide = bt.randn(bt.T, nH * hd + 24, dtype=torch.float16)
+    q = wide[:, 8:8 + nH * hd]
+    out = torch.full((bt.T, nH * hd + 16), 7.0, dtype=torch.float32, device=DEV)
+    view = out[:, 8:8 + nH * hd]
+    _attend(bt, q, out=view, scale=hd ** -0.5)
+    bt.check(view, q, scale=hd ** -0.5)
+    assert (out[:, :8] == 7).all() and (out[:, 8 + nH * hd:] == 7).all() and (view[-2:] == 7).all()
+
+
+def test_rows_outside_the_sequences_are_left():
+    bt = Batch(16, 8, 256, 64, [1, 0, 20, 0], [65, 10, 90, 0], 0, seed=6, front=3, back=4).fill()
+    q = bt.queries()
+    out = _attend(bt, q)
+    bt.check(out, q)
+    assert (out[:3] == 7).all() and (out[-4:] == 7).all()
+
+
+@pytest.mark.parametrize("hd,nH,nkv", [(256, 16, 8), (512, 4, 2)])
+def test_tokens_without_keys_give_zeros(hd, nH, nkv):
+    """More new tokens than the length says (positions below 0), and a sequence whose only pages are not there."""
+    bt = Batch(nH, nkv, hd, 16, [1, 1, 2], [20, 16, 40], 0, seed=7).fill()
+    bt.table[1, 0] = -1                                  # all of sequence 1's keys
+    bt.kv_len[2] = 1                                     # its first token has position -1
+    q = bt.queries()
+    out = _attend(bt, q).view(bt.T, nH, hd)
+    assert (out[1] == 0).all() and (out[2] == 0).all()
+    bt.total[2], bt.new[2] = 1, 1
+    bt.start[2] = 3
+    ref, _ = bt.reference(q)                             # token 3 sees its one key
+    assert (out[3].to(F64) - ref[3]).abs().max() < 1e-2
+    bt.total[1] = 0
+    assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+@pytest.mark.parametrize("hd,nH,nkv,new", [(256, 16, 8, [1, 1]), (128, 8, 1, [20, 3]), (512, 4, 2, [5, 2])])
+@pytest.mark.parametrize("bad", [-1, 10**9, None])
+def test_pages_that_are_not_there(hd, nH, nkv, new, bad):
+    bt = Batch(nH, nkv, hd, 16, new, [150, 120], 50, seed=8).fill()
+    q = bt.queries()
+    gone = [int(bt.ids[0, 1]), int(bt.ids[1, 3]), int(bt.pre_ids[1])]
+    bad = bt.pages if bad is None else bad               # the first id that is too large
+    bt.table[0, 1] = bad
+    bt.table[1, 3] = bad
+    bt.prefix_table[1] = bad
+    bt.check(_attend(bt, q), q, bad_pages=gone)
+
+
+def test_prefix_of_length_zero_and_short_sequences():
+    """Prefix pages with a prefix of no token; a sequence that ends inside the prefix."""
+    bt = Batch(16, 8, 256, 32, [1, 3], [70, 41], 0, seed=9, prefix_pages=4).fill()
+    q = bt.queries()
+    bt.check(_attend(bt, q), q)
+    bt = Batch(16, 8, 256, 32, [1, 3, 2], [170, 41, 1 + 100], 100, seed=9).fill()
+    q = bt.queries()
+    bt.check(_attend(bt, q), q)
+
+
+@pytest.mark.parametrize("hd,nH,nkv,new", [(256, 16, 8, 4), (512, 4, 2, 3), (128, 8, 1, 2), (256, 16, 8, 30), (128, 8, 1, 40)])
+def test_values_behind_the_mask_do_not_reach_a_row(hd, nH, nkv, new):
+    """The last token's key and value are infinite: the tokens before it must not notice."""
+    bt = Batch(nH, nkv, hd, 16, [new, 1], [new + 21, 50], 0, seed=10).fill()
+    q = bt.queries()
+    clean = _attend(bt, q).clone()
+    pg, sl = bt.place(0, new + 20)
+    bt.kc[pg, :, sl] = float("inf")
+    bt.vc[pg, :, sl] = float("-inf")
+    out = _attend(bt, q)
+    assert torch.equal(out[:new - 1], clean[:new - 1]) and torch.equal(out[new:], clean[new:])
+    assert not torch.isfinite(out[new - 1]).any()
+
+
+def test_scores_of_the_lowest_values():
+    """Scores near the largest negative finite ones still give weights; equal scores give equal weights."""
+    bt = Batch(16, 8, 256, 64, [1], [300], 0, seed=11).fill()
+    q = bt.queries()
+    bt.kc.copy_(torch.where(torch.isnan(bt.kc), bt.kc, torch.full_like(bt.kc, -60000.0)))
+    q.copy_(torch.full_like(q, 200.0))
+    out = _attend(bt, q)
+    pg, sl = bt.places(0, 300)
+    mean = bt.vc[pg, :, sl].to(F64).mean(0).repeat_interleave(2, 0)
+    a = bt.vc[pg, :, sl].to(F64).abs().mean(0).repeat_interleave(2, 0)
+    assert ((out.view(16, 256).to(F64) - mean).abs() <= 2.0 ** -11 * mean.abs() + 2 * (2.0 ** -11 + 2.0 ** -20) * a).all()
+
+
+def test_lengths_that_lie_stay_inside_the_buffers():
+    """Starts that fall and run past T, lengths past the tables: cut as the header says, no row outside is touched."""
+    bt = Batch(16, 8, 256, 16, [2, 3, 1], [40, 33, 48], 0, seed=12, back=2).fill()
+    bt.kc.nan_to_num_(0.5)
+    bt.vc.nan_to_num_(0.5)
+    q = bt.queries()
+    bt.q_start.copy_(torch.tensor([-5, 4, 1, 9999], dtype=torch.int32))
+    bt.kv_len.copy_(torch.tensor([-3, 10**9, 2**31 - 1], dtype=torch.int32))
+    out = _attend(bt, q)
+    assert torch.isfinite(out).all() and L.query(L.Q_KERNEL_STATUS) == 0
+    assert (out[:4] == 0).all()                          # sequence 0: no key
+    # sequence 2 has rows 4.. of all T, its length cut to its three pages
+    bt.start, bt.new, bt.total = np.array([0, 4, 4, bt.T]), [4, 0, bt.T - 4], [0, 48, 48]
+    ref, tol = bt.reference(q)
+    err = (out.view(bt.T, 16, 256).to(F64) - ref)[4:].abs()
+    assert (err <= tol[4:] + 2.0 ** -11 * ref[4:].abs() + 2.0 ** -25).all()
+
+
+def test_a_plan_of_other_sizes_writes_nothing():
+    bt = Batch(16, 8, 256, 64, [1, 1], [65, 90], 0, seed=13).fill()
+    q = bt.queries()
+    plan = PagedPlan(bt.T, bt.B, 16, 8, 256, 64, bt.own_pages, 0, 0, DEV)    # never updated
+    out = torch.full((bt.T, 4096), 7.0, dtype=torch.float16, device=DEV)
+    plan.attend(q, bt.kc, bt.vc, bt.table, out=out)
+    torch.cuda.synchronize()
+    assert (out == 7).all()
+    assert L.query(L.Q_KERNEL_STATUS) == 2 and L.query(L.Q_KERNEL_STATUS) == 0
+    other = Batch(16, 8, 256, 64, [1, 1, 1], [65, 90, 4], 0, seed=13)
+    plan._plan = torch.cat((other.plan()._plan, torch.zeros(1 << 20, dtype=torch.uint8, device=DEV)))
+    qkv = bt.randn(bt.T, 8192)
+    kc = bt.kc.clone()
+    w = torch.ones(256, device=DEV)
+    rot = torch.ones(bt.own_pages * 64, 256, device=DEV)
+    plan.append(qkv, w, w, rot, rot, bt.kc, bt.vc, bt.table, 4096, 6144, q_out=out)
+    torch.cuda.synchronize()
+    assert (out == 7).all() and torch.equal(bt.kc.view(torch.int16), kc.view(torch.int16))
+    assert L.query(L.Q_KERNEL_STATUS) == 2
+
+
+def test_python_refusals():
+    bt = Batch(16, 8, 256, 64, [1, 1], [65, 90], 0, seed=13).fill()
+    plan, q = bt.plan(), bt.queries()
+    with pytest.raises(ValueError):
+        plan.attend(q, bt.kc, bt.vc, bt.table, prefix_table=bt.table[0])
+    with pytest.raises(TypeError):
+        plan.attend(q.float(), bt.kc, bt.vc, bt.table)
+    with pytest.raises(ValueError):
+        plan.attend(q[:1], bt.kc, bt.vc, bt.table)
+    with pytest.raises(ValueError):
+        plan.attend(q, bt.kc[:, :, :32], bt.vc[:, :, :32], bt.table)
+    with pytest.raises(ValueError):
+        plan.attend(q, bt.kc.cpu(), bt.vc, bt.table)
+    with pytest.raises(ValueError):
+        plan.update(bt.q_start[:2], bt.kv_len)
+    with pytest.raises(L.G4BError):
+        PagedPlan(1, 1, 16, 8, 96, 64, 1)
+
+
+def _append_reference(bt, qkv, qnw, knw, cos, sin, koff, voff):
+    """(value, magnitude of the rotation's terms) of q [T, nH, hd], k and v [T, nkv, hd], positions [T]."""
+    pos = torch.full((bt.T,), -1, dtype=torch.long, device=DEV)
+    for b in range(bt.B):
+        s, n = int(bt.start[b]), bt.new[b]
+        pos[s:s + n] = torch.arange(bt.total[b] - n, bt.total[b], device=DEV)
+    x = qkv.to(F64)
+    c, s = cos[pos.clamp(min=0)].to(F64)[:, None], sin[pos.clamp(min=0)].to(F64)[:, None]
+
+    def normed(off, heads):
+        y = x[:, off:off + heads * bt.hd].reshape(bt.T, heads, bt.hd)
+        return y * (y.pow(2).mean(-1, keepdim=True) + 1e-6).rsqrt()
+
+    def turn(y):
+        h = bt.hd // 2
+        o = torch.cat((-y[..., h:], y[..., :h]), -1)
+        return y * c + o * s, (y * c).abs() + (o * s).abs()
+
+    v = normed(voff, bt.nkv)
+    return turn(normed(0, bt.nH) * qnw.to(F64)), turn(normed(koff, bt.nkv) * knw.to(F64)), (v, v.abs()), pos
+
+
+def _close16(got, ref, mag, what):
+    lim = 2.0 ** -11 * ref.abs() + 2.0 ** -20 * mag + 2.0 ** -25
+    err = (got.to(F64) - ref).abs()
+    assert (err <= lim).all(), f"{what}: {(err / lim).max().item():.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("nH,nkv,hd", HEADS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("page,new,total,prefix,keqv", [
+    (64, [1], [1], 0, False),
+    (16, [1, 0, 1, 2], [33, 7, 50, 49], 32, False),
+    (32, [1, 1, 1], [131, 129, 140], 128, True),
+    (128, [300, 5, 90], [311, 77, 90], 0, False),
+    (64, [20, 40], [30, 45], 25, False),                      # the first chunk begins inside the prefix: not written there
+])
+def test_append(nH, nkv, hd, dtype, page, new, total, prefix, keqv):
+    bt = Batch(nH, nkv, hd, page, new, total, prefix, seed=hd + page + nH, front=1, back=2)
+    nq, nk = nH * hd, nkv * hd
+    koff, voff = nq, nq if keqv else nq + nk
+    wide = (bt.randn(bt.T, nq + 2 * nk + 16) * torch.exp(bt.randn(bt.T, 1))).to(dtype)
+    qkv = wide[:, 8:]
+    if qkv.data_ptr() % 16:
+        qkv = wide[:, :-16]
+    qnw, knw = 1 + 0.2 * bt.randn(hd), 1 + 0.2 * bt.randn(hd)
+    n_pos = (bt.own_pages + bt.pre_pages) * page
+    inv = 10000.0 ** (-torch.arange(0, hd, 2, device=DEV, dtype=F64) / hd)
+    ang = torch.arange(n_pos, device=DEV, dtype=F64)[:, None] * torch.cat((inv, inv))
+    cos, sin = ang.cos().float(), ang.sin().float()
+    q_out = torch.full((bt.T, nq), 7.0, dtype=torch.float16, device=DEV)
+    bt.plan().append(qkv, qnw, knw, cos, sin, bt.kc, bt.vc, bt.table, koff, voff, q_out=q_out)
+    torch.cuda.synchronize()
+    (q, qm), (k, km), (v, vm), pos = _append_reference(bt, qkv, qnw, knw, cos, sin, koff, voff)
+    lo, hi = int(bt.start[0]), int(bt.start[-1])
+    _close16(q_out.view(bt.T, nH, hd)[lo:hi], q[lo:hi], qm[lo:hi], "q")
+    assert (q_out[:lo] == 7).all() and (q_out[hi:] == 7).all()
+    written = torch.zeros(bt.pages, page, dtype=torch.bool, device=DEV)
+    for b in range(bt.B):
+        for i in range(new[b]):
+            t = int(bt.start[b]) + i
+            p = int(pos[t])
+            if p < prefix:
+                continue
+            pg, sl = bt.place(b, p)
+            written[pg, sl] = True
+            _close16(bt.kc[pg, :, sl], k[t], km[t], "k")
+            _close16(bt.vc[pg, :, sl], v[t], vm[t], "v")
+    for c in (bt.kc, bt.vc):
+        kept = c.permute(0, 2, 1, 3)[~written]
+        assert torch.isnan(kept).all()                       # every other place as it was
+    assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+def test_append_skips_pages_that_are_not_there():
+    bt = Batch(16, 8, 256, 16, [20, 1], [20, 5], 0, seed=20)
+    bt.table[0, 0] = -7
+    bt.table[1, 0] = bt.pages
+    w, rot = torch.ones(256, device=DEV), torch.ones(bt.own_pages * 16, 256, device=DEV)
+    bt.plan().append(bt.randn(bt.T, 8192), w, w, rot, rot, bt.kc, bt.vc, bt.table, 4096, 6144)
+    torch.cuda.synchronize()
+    pg, _ = bt.place(0, 16)
+    mask = torch.ones(bt.pages, dtype=torch.bool, device=DEV)
+    mask[pg] = False
+    assert torch.isnan(bt.kc[mask]).all() and torch.isfinite(bt.kc[pg, :, :4]).all() and torch.isnan(bt.kc[pg, :, 4:]).all()
+    assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+def test_caches_past_two_to_the_31_elements():
+    nkv, hd, page = 8, 256, 64
+    pages = (1 << 31) // (nkv * hd * page) + 3
+    bt = Batch(16, nkv, hd, page, [1, 30], [100, 64], 0, seed=21)
+    kc = torch.zeros(pages, nkv, page, hd, dtype=torch.float16, device=DEV)
+    vc = torch.zeros_like(kc)
+    last = list(range(pages - bt.B * bt.own_pages, pages))
+    bt.ids = np.array(last[::-1], dtype=np.int32).reshape(bt.B, bt.own_pages)
+    bt.table.copy_(torch.from_numpy(bt.ids))
+    bt.kc, bt.vc, bt.pages = kc, vc, pages
+    bt.fill()
+    q = bt.queries()
+    bt.check(_attend(bt, q), q)
+    w, rot = torch.ones(256, device=DEV), torch.ones(bt.own_pages * page, 256, device=DEV)
+    before = kc[:64].clone()
+    bt.plan().append(bt.randn(bt.T, 8192), w, w, rot, rot, kc, vc, bt.table, 4096, 6144)
+    pg, sl = bt.place(0, 99)
+    assert (kc[pg, :, sl] != 0).any() and torch.equal(kc[:64], before)
+
+
+def test_graph_replays_follow_the_lengths():
+    bt = Batch(16, 8, 256, 64, [1, 1, 1], [100, 300, 161], 64, seed=22).fill()
+    q = bt.queries()
+    plan = bt.plan()
+    out = torch.full((bt.T, 4096), 7.0, dtype=torch.float16, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        plan.update(bt.q_start, bt.kv_len, bt.prefix_len)
+        plan.attend(q, bt.kc, bt.vc, bt.table, bt.prefix_table, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.update(bt.q_start, bt.kv_len, bt.prefix_len)
+        plan.attend(q, bt.kc, bt.vc, bt.table, bt.prefix_table, out=out)
+    for total in ([100, 300, 161], [65, 140, 161], [64, 299, 90]):
+        bt.kv_len.copy_(torch.tensor(total, dtype=torch.int32))
+        bt.total = total
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        bt.check(out, q)
+
+
+def test_two_plans_at_once_on_two_streams():
+    a = Batch(16, 8, 256, 64, [1] * 40, [2000 + i for i in range(40)], 1900, seed=23).fill()
+    b = Batch(8, 1, 128, 16, [60, 1, 5], [900, 700, 300], 200, seed=24).fill()
+    qa, qb = a.queries(), b.queries()
+    pa, pb = a.plan(), b.plan()
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(4):
+        oa = pa.attend(qa, a.kc, a.vc, a.table, a.prefix_table, stream=sa)
+        ob = pb.attend(qb, b.kc, b.vc, b.table, b.prefix_table, stream=sb)
+        outs.append((oa, ob))
+    torch.cuda.synchronize()
+    for oa, ob in outs:
+        a.check(oa, qa)
+        b.check(ob, qb)
+        assert torch.equal(oa, outs[0][0]) and torch.equal(ob, outs[0][1])    # the same bits every time
