@@ -56,6 +56,7 @@ static int make_dims(const char* op, int T, int B, int nH, int nkv, int hd, int 
     d.own_pages = own_pages;
     d.pre_pages = pre_pages;
     d.window = window;
+    d.cs = hd == 512 ? 2 : 1;
     d.ctas[0] = sms * few_per_sm(hd);
     d.ctas[1] = sms;
     const int rows = T * d.G;
@@ -93,13 +94,13 @@ static size_t work_bytes(const Dims& d, char* base, Work* w) {
     for (int k = 0; k < 2; k++) {
         if (k == 1 && !many_rows(d.hd)) continue;
         const size_t rows = (size_t)d.ctas[k] * 2 * (k ? kRowsP : kRowsS);
-        x.edge[k] = reinterpret_cast<float*>(take(rows * d.hd * 4));
+        x.edge[k] = reinterpret_cast<float*>(take(rows * (k ? d.hd / d.cs : d.hd) * 4));
         x.edge_ml[k] = reinterpret_cast<float2*>(take(rows * 8));
     }
     if (d.pre_pages > 0) {
         const size_t rows = (size_t)d.T * d.nH * 2;
         x.row = reinterpret_cast<float*>(take(rows * d.hd * 4));
-        x.row_ml = reinterpret_cast<float2*>(take(rows * 8));
+        x.row_ml = reinterpret_cast<float2*>(take(rows * 2 * 8));
     }
     if (w) *w = x;
     return o;
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         }
         __syncthreads();
         // equal stretches of the line of all heads' units
-        const long long total = run * d.nkv;
+        const long long total = run * d.nkv * (kind ? d.cs : 1);
         const long long u = max(1LL, (total + d.ctas[kind] - 1) / d.ctas[kind]);
         if (tid == 0) {
             h->nt[kind] = nt[kind];
@@ -497,10 +498,14 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
     pdl_launch_dependents();
     if (h->sig != d.sig) {
         if (blockIdx.x == 0 && tid == 0) atomicOr(&g_status_paged, kStatusPlan);
+        pdl_wait();
         return;
     }
     const Start st = at<Start>(a.plan, d.start[0])[blockIdx.x];
-    if (st.head < 0) return;
+    if (st.head < 0) {
+        pdl_wait();
+        return;
+    }
     const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + (uint32_t)(warp * C::NST * C::ENTRY);
     uint8_t* ring_p = smem_raw + (ring - smem_u32(smem_raw));
     const uint32_t bar0 = smem_u32(&bars[warp][0]);
@@ -796,7 +801,7 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
                                           : ((size_t)blockIdx.x * 2 + (unit == 0 ? 1 : 0)) * kRowsS + r;
                 float* dst = (whole ? a.w.row : a.w.edge[0]) + slot * HD + c;
                 *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-                if (c == 0) (whole ? a.w.row_ml : a.w.edge_ml[0])[slot] = make_float2(M, L);
+                if (c == 0) *(whole ? a.w.row_ml + 2 * slot : a.w.edge_ml[0] + slot) = make_float2(M, L);
             }
         }
         // the ring was written and read by threads; the next piece's copies come behind that
@@ -841,13 +846,14 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
         L = L * f0 + ml.y * f1;
         #pragma unroll
         for (int i = 0; i < PER; i += 4) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(p + lane * PER + i));
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(p + i));
             v[i] = v[i] * f0 + x.x * f1;
             v[i + 1] = v[i + 1] * f0 + x.y * f1;
             v[i + 2] = v[i + 2] * f0 + x.z * f1;
             v[i + 3] = v[i + 3] * f0 + x.w * f1;
         }
     };
+    bool done = false;
     #pragma unroll 1
     for (int seg = 0; seg < 2; seg++) {      // 0 prefix, 1 own
         const int ref = at<int>(a.plan, seg ? d.row_own : d.row_pre)[row];
@@ -855,20 +861,24 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
         const int kind = (unsigned)ref >> 31;
         const Tile& t = at<Tile>(a.plan, d.tiles[kind])[ref & 0x7fffffff];
         if (t.n == 0) continue;
-        const Span sp = span_of(h, kind, t.off, t.n, head);
-        if (sp.c0 == sp.c1) {
-            if (t.solo) return;              // written by its tile
+        // a many-rows tile of a wide head is walked once per part of the columns: this lane's is `part`
+        const int width = kind ? HD / d.cs : HD, part = lane * PER / width, col = lane * PER % width;
+        const Span sp = span_of(h, kind, t.off, t.n, kind ? head * d.cs + part : head);
+        if (sp.c0 == sp.c1 && t.solo) {      // written by its tile
+            done = true;
+        } else if (sp.c0 == sp.c1) {
             const size_t slot = ((size_t)seg * d.T + tok) * d.nH + hq;
-            add(a.w.row + slot * HD, __ldcg(a.w.row_ml + slot));
+            add(a.w.row + slot * HD + lane * PER, __ldcg(a.w.row_ml + 2 * slot + part));
         } else {
             const int br = kind ? kRowsP : kRowsS, r = row - t.row0;
             #pragma unroll 4
             for (int c = sp.c0; c <= sp.c1; c++) {
                 const size_t slot = ((size_t)c * 2 + (c == sp.c0 ? 1 : 0)) * br + r;
-                add(a.w.edge[kind] + slot * HD, __ldcg(a.w.edge_ml[kind] + slot));
+                add(a.w.edge[kind] + slot * width + col, __ldcg(a.w.edge_ml[kind] + slot));
             }
         }
     }
+    if (done) return;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const long long o = (long long)tok * a.out_stride + (long long)hq * HD + lane * PER;
     #pragma unroll
@@ -900,12 +910,19 @@ static cudaError_t launch_pdl(K k, dim3 grid, int threads, size_t smem, cudaStre
 }
 
 template <int HD>
-static cudaError_t launch_few(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+static cudaError_t launch_few(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, bool after_many,
+                              cudaStream_t s) {
     using C = FewCfg<HD>;
     cudaError_t e = cudaFuncSetAttribute(few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
-    few_kernel<HD><<<a.d.ctas[0], 32 * kFewWarps, C::SMEM, s>>>(a, km, vm);
-    e = cudaGetLastError();
+    // Behind the many-rows kernel its CTAs may begin as that one's end: they read nothing of it, and what both read was
+    // complete before that one began (it is an ordinary launch).  Each waits for it before it ends.
+    if (after_many) {
+        e = launch_pdl(few_kernel<HD>, dim3(a.d.ctas[0]), 32 * kFewWarps, C::SMEM, s, a, km, vm);
+    } else {
+        few_kernel<HD><<<a.d.ctas[0], 32 * kFewWarps, C::SMEM, s>>>(a, km, vm);
+        e = cudaGetLastError();
+    }
     if (e != cudaSuccess) return e;
     const long long rows = (long long)a.d.T * a.d.nH, per = kJoinThreads / 32;
     return launch_pdl(join_kernel<HD>, dim3((unsigned)((rows + per - 1) / per)), kJoinThreads, 0, s, a);
@@ -918,17 +935,17 @@ static void launch_append(const AppendArgs& a, dim3 grid, cudaStream_t s) {
     else append_kernel<512, XF32><<<grid, kAppendThreads, 0, s>>>(a);
 }
 
-bool many_rows(int) { return false; }
 }  // namespace pg
 
 unsigned read_status_paged() {
+    const unsigned m = pg::read_status_paged_mma();
     unsigned v = 0;
     if (cudaMemcpyFromSymbol(&v, pg::g_status_paged, sizeof(v)) != cudaSuccess) return 0xffffffffu;
     if (v) {
         const unsigned zero = 0;
         cudaMemcpyToSymbol(pg::g_status_paged, &zero, sizeof(zero));
     }
-    return v;
+    return v | m;
 }
 
 }  // namespace g4b
@@ -1089,9 +1106,15 @@ int g4b_paged_attn(const uint16_t* q, long long q_stride, const uint16_t* kc, co
         if (st != G4B_OK) return st;
     }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e = hd == 128 ? launch_few<128>(a, km, vm, s)
-                  : hd == 256 ? launch_few<256>(a, km, vm, s)
-                              : launch_few<512>(a, km, vm, s);
+    // no tile of many rows: neither a sequence nor the prefix has more rows than the batch
+    const bool many = many_rows(hd) && T * a.d.G > kRowsS;
+    if (many) {
+        st = launch_many(a, s);
+        if (st != G4B_OK) return st;
+    }
+    cudaError_t e = hd == 128 ? launch_few<128>(a, km, vm, many, s)
+                  : hd == 256 ? launch_few<256>(a, km, vm, many, s)
+                              : launch_few<512>(a, km, vm, many, s);
     if (e != cudaSuccess) return fail(G4B_E_CUDA, "paged_attn: launch: %s", cudaGetErrorString(e));
     count_launch(2);
     return launch_status("paged_attn");

@@ -56,6 +56,7 @@ struct Hdr {
 // sizes fixed on the host, and the offsets of the arrays in the plan buffer that follow from them
 struct Dims {
     int T, B, nH, nkv, G, hd, ps, own_pages, pre_pages, window;
+    int cs;                          // walks per many-rows tile: parts of hd's output columns
     int ctas[2];                     // stretches per kind
     int max_tiles[2];
     size_t tok_seq, tok_pos, row_own, row_pre, start[2], tiles[2], bytes;
@@ -72,13 +73,13 @@ __host__ __device__ inline const X* at(const void* plan, size_t off) {
     return reinterpret_cast<const X*>(reinterpret_cast<const char*>(plan) + off);
 }
 
-// The workspace: edge slots of both kinds ([cta][2][rows][hd] sums, then [cta][2][rows] (max, sum)), then,
+// The workspace: edge slots of both kinds ([cta][2][rows][columns of a walk] sums, [cta][2][rows] (max, sum)), then,
 // where there is a prefix, one slot per (segment kind, token, head) for whole tiles.
 struct Work {
     float* edge[2];
     float2* edge_ml[2];
     float* row;        // [2][T * nH][hd]: 0 prefix, 1 own
-    float2* row_ml;
+    float2* row_ml;    // [2][T * nH][2]: one per walk of the tile (the few-rows kernel's only one first)
 };
 
 struct Args {
@@ -106,9 +107,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// many-rows tiles are for these head widths (the kernel of g4b_paged_mma.cu)
+// the many-rows kernel (g4b_paged_mma.cu): the head widths it has, its launch, its status word
 bool many_rows(int hd);
 int launch_many(const Args& a, cudaStream_t s);
+unsigned read_status_paged_mma();
 
 }  // namespace pg
 }  // namespace g4b

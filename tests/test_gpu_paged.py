@@ -129,7 +129,7 @@ class Batch:
         lo, hi = int(self.start[0]), int(self.start[-1])
         err = (got64 - ref).abs()[lo:hi]
         lim = (tol + eps * ref.abs() + 2.0 ** -25)[lo:hi]
-        assert torch.isfinite(got64[lo:hi]).all()
+        assert bool(torch.isfinite(got64[lo:hi]).all())
         worst = (err - lim).max().item() if err.numel() else 0.0
         assert worst <= 0, f"off by {err.max().item():.3e}, {(err / lim).max().item():.2f} of the tolerance"
         assert L.query(L.Q_KERNEL_STATUS) == 0
