@@ -112,6 +112,7 @@ static size_t work_bytes(const Dims& d, char* base, Work* w) {
 // trusted with an address: starts are made non-decreasing and cut to [0, T], lengths to the tables'
 // capacity.
 constexpr int kPlanThreads = 1024;
+constexpr long long kPieceCostS = 2, kPieceCostP = 3;
 
 struct PlanArgs {
     const int* q_start;
@@ -261,7 +262,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         Tile* tiles = at<Tile>(a.plan, d.tiles[kind]);
         const int br = kind ? kRowsP : kRowsS;
         const bool pre_here = pre_tiles > 0 && (kind == 1) == pre_many;
-        long long run = 0;
+        const auto add = [](long long x, long long y) { return x + y; };
+        const int heads = d.nkv * (kind ? d.cs : 1), ctas = d.ctas[kind];
+        long long work = 0;                  // units of one head
         for (int i0 = 0; i0 < nt[kind]; i0 += kPlanThreads) {
             const int i = i0 + tid;
             Tile t{};
@@ -287,26 +290,60 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
                     }
                 }
             }
+            if (i < nt[kind]) tiles[i] = t;
             long long all;
-            const long long exc = block_scan((long long)t.n, 0LL, wbuf, &all,
-                                             [](long long x, long long y) { return x + y; });
+            block_scan((long long)t.n, 0LL, wbuf, &all, add);
+            work += all;
+        }
+        __syncthreads();
+        // Equal stretches of the line of all heads' units, wherever their borders fall; or, if every tile can have
+        // CTAs of its own, the shortest stretch for which they suffice when each tile starts at a border.  A border
+        // inside a tile costs its CTA another start and another partial, about kPieceCost units.
+        long long u = max(1LL, (work * heads + ctas - 1) / ctas);
+        bool aligned = false;
+        {
+            auto stretches = [&](long long len) {
+                long long n = 0;
+                for (int i = tid; i < nt[kind]; i += kPlanThreads) n += (tiles[i].n + len - 1) / len;
+                long long all;
+                block_scan(n, 0LL, wbuf, &all, add);
+                return all * heads;
+            };
+            const long long most = u + (kind ? kPieceCostP : kPieceCostS);
+            if (work > 0 && stretches(most) <= ctas) {
+                long long lo = u, hi = most;
+                while (lo < hi) {
+                    const long long m = (lo + hi) / 2;
+                    if (stretches(m) <= ctas) hi = m;
+                    else lo = m + 1;
+                }
+                u = lo;
+                aligned = true;
+            }
+        }
+        long long run = 0;
+        for (int i0 = 0; i0 < nt[kind]; i0 += kPlanThreads) {
+            const int i = i0 + tid;
+            const int n = i < nt[kind] ? tiles[i].n : 0;
+            const int idle = aligned ? (int)((u - n % u) % u) : 0;
+            long long all;
+            const long long exc = block_scan((long long)n + idle, 0LL, wbuf, &all, add);
             if (i < nt[kind]) {
-                t.off = run + exc;
-                tiles[i] = t;
+                tiles[i].off = run + exc;
+                tiles[i].idle = idle;
             }
             run += all;
         }
         __syncthreads();
-        // equal stretches of the line of all heads' units
-        const long long total = run * d.nkv * (kind ? d.cs : 1);
-        const long long u = max(1LL, (total + d.ctas[kind] - 1) / d.ctas[kind]);
+        const long long total = run * heads;
         if (tid == 0) {
             h->nt[kind] = nt[kind];
             h->wt[kind] = run;
             h->u[kind] = u;
         }
         for (int c = tid; c < d.ctas[kind]; c += kPlanThreads) {
-            Start s{-1, 0, 0, 0};
+            Start s{};
+            s.head = -1;
             const long long at0 = (long long)c * u;
             if (at0 < total) {
                 const long long rem = at0 % run;
@@ -319,6 +356,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
                 }
                 s.tile = lo;
                 s.unit = (int)(rem - tiles[lo].off);
+                s.t = tiles[lo];
             }
             at<Start>(a.plan, d.start[kind])[c] = s;
         }
@@ -501,7 +539,9 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
         pdl_wait();
         return;
     }
-    const Start st = at<Start>(a.plan, d.start[0])[blockIdx.x];
+    const Start& st = at<Start>(a.plan, d.start[0])[blockIdx.x];
+    Tile t = st.t;
+    bool first = true;
     if (st.head < 0) {
         pdl_wait();
         return;
@@ -531,7 +571,8 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
             ti = 0;
             head++;
         }
-        const Tile t = tiles[ti];
+        if (!first) t = tiles[ti];
+        first = false;
         if (t.n == 0) {
             ti++;
             unit = 0;
@@ -597,13 +638,12 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
             if (!(e & 1)) valid = (valid & ~(1u << (n & 31))) | ((ok ? 1u : 0u) << (n & 31));
             // a page that is not there: past the map's last row, which TMA fills with zeros
             const int row = ok ? at_row : a.num_pages * d.nkv * d.ps;
-            if (lane == 0) {
-                const uint32_t bar = bar0 + 8 * eslot, dst = ring + (uint32_t)(eslot * C::ENTRY);
-                mbar_arrive_expect_tx(bar, C::ENTRY);
-                #pragma unroll
-                for (int c = 0; c < HD / 64; c++)
-                    tma_2d(dst + c * (kBlk * 128), (e & 1) ? &vmap : &kmap, 64 * c, row, bar);
-            }
+            // one box of 64 columns per lane: one instruction of the warp issues the entry
+            const uint32_t bar = bar0 + 8 * eslot;
+            if (lane == 0) mbar_arrive_expect_tx(bar, C::ENTRY);
+            __syncwarp();
+            if (lane < HD / 64)
+                tma_2d(ring + (uint32_t)(eslot * C::ENTRY + lane * (kBlk * 128)), (e & 1) ? &vmap : &kmap, 64 * lane, row, bar);
             eslot = eslot + 1 == C::NST ? 0 : eslot + 1;
             issued++;
         };
@@ -612,7 +652,7 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
         bool ok = true;
         int done = 0;                            // entries consumed
         auto next = [&]() {                      // wait for the next entry; its address
-            ok = __all_sync(0xffffffffu, mbar_wait(bar0 + 8 * entry, (phase >> entry) & 1u, abort, &g_status_paged));
+            ok = __all_sync(0xffffffffu, wait_short(bar0 + 8 * entry, (phase >> entry) & 1u, abort, &g_status_paged));
             if (ok) phase ^= 1u << entry;
             return ring + (uint32_t)(entry * C::ENTRY);
         };
@@ -810,6 +850,7 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
         left -= nu;
         unit += nu;
         if (unit == t.n) {
+            left -= t.idle;
             unit = 0;
             ti++;
         }
@@ -829,56 +870,93 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
     constexpr int PER = HD / 32;
     const Dims& d = a.d;
     const Hdr* h = hdr_of(a.plan);
-    pdl_wait();
-    if (h->sig != d.sig) return;
     const int lane = threadIdx.x & 31;
     const long long w = (long long)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
-    if (w >= (long long)d.T * d.nH) return;
+    const bool mine = h->sig == d.sig && w < (long long)d.T * d.nH && w >= (long long)h->tok_lo * d.nH &&
+                      w < (long long)h->tok_hi * d.nH;
+    if (!mine) {          // not a row of any sequence: left as it was
+        pdl_wait();       // (a grid that ends is taken for the end of the one it depends on, too)
+        return;
+    }
     const int tok = (int)(w / d.nH), hq = (int)(w % d.nH), head = hq / d.G, row = tok * d.G + hq % d.G;
-    if (tok < h->tok_lo || tok >= h->tok_hi) return;   // not a row of any sequence: left as it was
-    float M = -INFINITY, L = 0.f, v[PER];
-    #pragma unroll
-    for (int i = 0; i < PER; i++) v[i] = 0.f;
-    auto add = [&](const float* p, float2 ml) {
-        const float mn = fmaxf(M, ml.x), mu = mn == -INFINITY ? 0.f : mn;
-        const float f0 = exp2_approx(M - mu), f1 = exp2_approx(ml.x - mu);
-        M = mn;
-        L = L * f0 + ml.y * f1;
-        #pragma unroll
-        for (int i = 0; i < PER; i += 4) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(p + i));
-            v[i] = v[i] * f0 + x.x * f1;
-            v[i + 1] = v[i + 1] * f0 + x.y * f1;
-            v[i + 2] = v[i + 2] * f0 + x.z * f1;
-            v[i + 3] = v[i + 3] * f0 + x.w * f1;
-        }
-    };
+    // where the partials are: from the plan, which no kernel before this one writes
+    const float* part[2] = {nullptr, nullptr};         // of segment 0 (prefix) and 1 (own): first partial,
+    const float2* ml[2] = {nullptr, nullptr};
+    int n[2] = {0, 0}, next[2] = {0, 0}, part_width[2] = {HD, HD};   // how many; slots between the later ones; floats of a slot
     bool done = false;
-    #pragma unroll 1
-    for (int seg = 0; seg < 2; seg++) {      // 0 prefix, 1 own
-        const int ref = at<int>(a.plan, seg ? d.row_own : d.row_pre)[row];
-        if (seg == 0 && ref == -1) continue;
+    #pragma unroll
+    for (int seg = 0; seg < 2; seg++) {
+        const int ref = __ldg(at<int>(a.plan, seg ? d.row_own : d.row_pre) + row);
+        if (ref == -1 && seg == 0) continue;
         const int kind = (unsigned)ref >> 31;
         const Tile& t = at<Tile>(a.plan, d.tiles[kind])[ref & 0x7fffffff];
         if (t.n == 0) continue;
-        // a many-rows tile of a wide head is walked once per part of the columns: this lane's is `part`
-        const int width = kind ? HD / d.cs : HD, part = lane * PER / width, col = lane * PER % width;
-        const Span sp = span_of(h, kind, t.off, t.n, kind ? head * d.cs + part : head);
-        if (sp.c0 == sp.c1 && t.solo) {      // written by its tile
-            done = true;
-        } else if (sp.c0 == sp.c1) {
+        // a many-rows tile of a wide head is walked once per part of the columns: this lane's is `walk`
+        const int width = kind ? HD / d.cs : HD, walk = lane * PER / width, col = lane * PER % width;
+        const Span sp = span_of(h, kind, t.off, t.n, kind ? head * d.cs + walk : head);
+        n[seg] = sp.c1 - sp.c0 + 1;
+        if (sp.c0 == sp.c1) {
+            done = t.solo;                             // written by its tile
             const size_t slot = ((size_t)seg * d.T + tok) * d.nH + hq;
-            add(a.w.row + slot * HD + lane * PER, __ldcg(a.w.row_ml + 2 * slot + part));
+            part[seg] = a.w.row + slot * HD + lane * PER;
+            ml[seg] = a.w.row_ml + 2 * slot + walk;
         } else {
-            const int br = kind ? kRowsP : kRowsS, r = row - t.row0;
-            #pragma unroll 4
-            for (int c = sp.c0; c <= sp.c1; c++) {
-                const size_t slot = ((size_t)c * 2 + (c == sp.c0 ? 1 : 0)) * br + r;
-                add(a.w.edge[kind] + slot * width + col, __ldcg(a.w.edge_ml[kind] + slot));
+            // edge slots: 1 in the tile's first CTA, 0 in the ones behind it
+            const int br = kind ? kRowsP : kRowsS;
+            const size_t slot = ((size_t)sp.c0 * 2 + 1) * br + (row - t.row0);
+            part[seg] = a.w.edge[kind] + slot * width + col;
+            ml[seg] = a.w.edge_ml[kind] + slot;
+            next[seg] = 2 * br;
+        }
+        part_width[seg] = width;
+    }
+    pdl_wait();
+    if (done) return;
+    float M = -INFINITY, L = 0.f, v[PER];
+    #pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = 0.f;
+    #pragma unroll
+    for (int seg = 0; seg < 2; seg++) {
+        // up to four partials at once: their loads are independent, their sums are not
+        for (int k0 = 0; k0 < n[seg]; k0 += 4) {
+            float2 w2[4];
+            float x[4][PER];
+            #pragma unroll
+            for (int k = 0; k < 4; k++) {
+                // slot of partial k0 + k from the first one's: -br + k 2 br behind the first
+                const long long s = k0 + k == 0 ? 0 : (long long)(k0 + k) * next[seg] - next[seg] / 2;
+                w2[k] = make_float2(-INFINITY, 0.f);
+                if (k0 + k < n[seg]) {
+                    w2[k] = __ldcg(ml[seg] + s);
+                    #pragma unroll
+                    for (int i = 0; i < PER; i += 4) {
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(part[seg] + s * part_width[seg] + i));
+                        x[k][i] = y.x;
+                        x[k][i + 1] = y.y;
+                        x[k][i + 2] = y.z;
+                        x[k][i + 3] = y.w;
+                    }
+                } else {
+                    #pragma unroll
+                    for (int i = 0; i < PER; i++) x[k][i] = 0.f;
+                }
+            }
+            const float mn = fmaxf(fmaxf(fmaxf(M, w2[0].x), fmaxf(w2[1].x, w2[2].x)), w2[3].x);
+            const float mu = mn == -INFINITY ? 0.f : mn;
+            const float f = exp2_approx(M - mu);
+            M = mn;
+            L *= f;
+            #pragma unroll
+            for (int i = 0; i < PER; i++) v[i] *= f;
+            #pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float g = exp2_approx(w2[k].x - mu);
+                L = fmaf(w2[k].y, g, L);
+                #pragma unroll
+                for (int i = 0; i < PER; i++) v[i] = fmaf(x[k][i], g, v[i]);
             }
         }
     }
-    if (done) return;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const long long o = (long long)tok * a.out_stride + (long long)hq * HD + lane * PER;
     #pragma unroll

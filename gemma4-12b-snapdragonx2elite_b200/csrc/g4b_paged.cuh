@@ -10,7 +10,7 @@
 // sequence's own keys for its own rows (row = token * G + query head of the group).  A segment is cut
 // into tiles of kRowsS or kRowsP rows; a tile is n units of 64 keys.  The units of all tiles and KV heads
 // form one line that is cut into equal lengths, one per CTA, whatever the lengths of the sequences: a CTA
-// walks its stretch piece by piece.  A tile that lies in one CTA's stretch is finished there; one that
+// walks its stretch piece by piece.  Where that costs no more (few tiles, many CTAs) every tile starts at a border.  A tile that lies in one CTA's stretch is finished there; one that
 // crosses a border leaves a partial (running maximum, sum, weighted values) in the edge slots of each CTA,
 // and the join kernel adds them.
 #pragma once
@@ -34,13 +34,13 @@ struct Tile {
     int lo, hi;      // keys [lo, hi) of the segment; lo is a multiple of kUnit
     int n;           // units
     int solo;        // its rows have keys in no other segment: a whole tile writes the output itself
-    int pad;
-    long long off;   // units of the tiles before it
-    long long pad2;
+    int idle;        // units behind it that are nobody's work: they align the next tile with a stretch's start
+    long long off;   // units of the tiles before it, their idle ones included
 };
 
 struct Start {       // where a CTA's stretch begins
-    int head, tile, unit, pad;
+    int head, tile, unit, pad;   // head: KV head * walks per tile + walk; -1: nothing to do
+    Tile t;                      // tiles[tile]
 };
 
 struct Hdr {
@@ -99,6 +99,15 @@ struct Args {
 
 __device__ __forceinline__ Span span_of(const Hdr* h, int kind, long long off, int n, int head) {
     return span_of((long long)head * h->wt[kind] + off, n, h->u[kind]);
+}
+
+// mbar_wait whose first tries do not read the timer: in these kernels most waits are short and lie on the path
+// from one unit to the next.
+__device__ __forceinline__ bool wait_short(uint32_t bar, uint32_t parity, volatile int* abort, unsigned* status) {
+    #pragma unroll 1
+    for (int i = 0; i < 64; i++)
+        if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait(bar, parity, abort, status);
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {

@@ -4,14 +4,15 @@
 // A tile is 128 rows (token, query head of the group) of one KV head, a row per tensor memory lane; units of 64
 // keys stream past it.  Per unit
 //   S [128 x 64] = Q K^T      (tcgen05, Q in tensor memory, K from shared memory)
-//   P = 2^(S scale - m)       (one thread per row: no reduction leaves the thread)
+//   P = 2^(S scale - m)       (two threads per row: a row's maximum takes one exchange through shared memory)
 //   O [128 x hd] += P V       (tcgen05, P in tensor memory over S's columns, V from shared memory)
 // S is double buffered, so the tensor core makes unit i + 1's scores while the softmax warps work on unit i.
-// m is the maximum seen when it was last set: O is rescaled only where a row's maximum has risen by more than
-// 2^8 since (weights up to 256 are exact enough in f16: their relative rounding does not change).
+// m is a base, 2^4 under the maximum seen when it was set: O is rescaled only where a row's weights would pass
+// 2^15, the last power of two of f16 (a larger weight's relative rounding is the same; the 2^4 keep weights down
+// to 2^-18 of the maximum out of f16's subnormals).
 // K and V units come by TMA through one ring of 64-key buffers, issued ahead across pieces.
 //
-// Warps: 0-3 softmax, the mask, the rows' Q and the result; 4 TMA; 5 MMA issue.
+// Warps: 0-7 softmax, the mask, the rows' Q and the result; 8 TMA; 9 MMA issue.
 // At hd 512 the 512 output columns of O would fill tensor memory, so a tile is walked once for each half of
 // them (the scores are made twice), and half of Q stays in shared memory.
 //
@@ -25,9 +26,10 @@ namespace pg {
 
 __device__ unsigned g_status_paged_mma;
 
-constexpr int kManyThreads = 192;
-constexpr int kPieceRowsMin = 16;       // smallest page: rows of a TMA box
-constexpr float kLazy = 8.f;            // log2 of how far weights may rise before O is rescaled
+constexpr int kSoft = 256;              // softmax threads: two per row
+constexpr int kManyThreads = kSoft + 64;
+constexpr float kLift = 4.f;            // log2 of the weight that a row's maximum gets when its base is set
+constexpr float kMost = 15.f;           // log2 of the largest weight before the base is set anew (f16: below 2^16)
 
 template <int HD>
 struct ManyCfg {
@@ -37,11 +39,25 @@ struct ManyCfg {
     static constexpr int KE = HD / QT;                  // ring entries per unit of K
     static constexpr int ENTRY = kUnit * DV * 2;        // bytes of a ring entry: 64 keys x DV elements
     static constexpr int QS_BYTES = kRowsP * (HD - QT) * 2;
-    static constexpr int NST = HD == 128 ? 12 : HD == 256 ? 7 : 5;
-    static constexpr int SMEM = NST * ENTRY + QS_BYTES + 1024;
+    // a warp's 32 rows x 128 bytes on their way between rows in memory and rows in lanes; at hd 512 they lie in
+    // the shared half of Q, which is idle then
+    static constexpr int STAGE = 32 * 128;
+    static constexpr int NST = HD == 128 ? 12 : HD == 256 ? 6 : 5;
+    static constexpr int BUF = NST * ENTRY + (QS_BYTES ? QS_BYTES : 8 * STAGE);
     static constexpr int O_COL = 0, S_COL = DV, Q_COL = DV + 2 * kUnit;
     static_assert(Q_COL + QT / 2 <= 512, "tensor memory columns");
-    static_assert(SMEM <= 226 * 1024, "shared memory");
+    // Everything else that is shared, behind the buffers: no static shared memory, so that the buffers begin where the
+    // CTA's window does, at a multiple of 1024 (the kernel checks).
+    struct Small {
+        uint64_t bars[2 * NST + 8];
+        unsigned long long odd;            // keys of the unit with a value that is not finite
+        float top[2][2][kRowsP];           // [unit % 2][half][row]
+        int red[4][4];
+        uint32_t tmem;
+        int abort, acc;
+    };
+    static constexpr int SMEM = BUF + (int)sizeof(Small);
+    static_assert(SMEM <= 227 * 1024, "shared memory");
     static_assert(KE * 2 + 1 <= NST, "the units issued before the first release");
 };
 
@@ -59,17 +75,39 @@ __device__ __forceinline__ uint32_t ld_tmem_x1(uint32_t taddr) {
     return v;
 }
 
+// or of all softmax threads' flags
+__device__ __forceinline__ bool any_soft(bool v) {
+    int r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+        : "=r"(r) : "r"((int)v) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void st_shared(uint32_t at, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+// bit 15 of a half is set where the f16 value is not finite (its exponent field overflows by one)
+__device__ __forceinline__ uint32_t not_finite(uint32_t v) { return (v & 0x7fff7fffu) + 0x04000400u; }
+
 // The pieces of a CTA's stretch, walked alike by every role.
 struct Walk {
     const Tile* tiles;
     long long left;
     int ntiles, head, ti, unit;   // head: KV head * CS + column part
+    bool first;
     Tile t;
     int nu, key0, key1;
 
     __device__ __forceinline__ bool init(const Args& a) {
         const Hdr* h = hdr_of(a.plan);
-        const Start st = at<Start>(a.plan, a.d.start[1])[blockIdx.x];
+        const Start& st = at<Start>(a.plan, a.d.start[1])[blockIdx.x];
+        t = st.t;
+        first = true;
         if (st.head < 0) return false;
         tiles = at<Tile>(a.plan, a.d.tiles[1]);
         ntiles = h->nt[1];
@@ -85,7 +123,8 @@ struct Walk {
                 ti = 0;
                 head++;
             }
-            t = tiles[ti];
+            if (!first) t = tiles[ti];
+            first = false;
             if (t.n > 0) break;
             ti++;
             unit = 0;
@@ -100,6 +139,7 @@ struct Walk {
         left -= nu;
         unit += nu;
         if (unit == t.n) {
+            left -= t.idle;
             unit = 0;
             ti++;
         }
@@ -112,11 +152,8 @@ template <int HD>
 __global__ void __launch_bounds__(kManyThreads, 1)
 many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using C = ManyCfg<HD>;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * C::NST + 8];
-    __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_acc, s_red[4][4];
-    __shared__ unsigned long long s_odd;         // keys of the unit with a value that is not finite
+    extern __shared__ __align__(1024) uint8_t smem[];
+    auto& sm = *reinterpret_cast<typename C::Small*>(smem + C::BUF);
     const Dims& d = a.d;
     const Hdr* h = hdr_of(a.plan);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -128,10 +165,13 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
     }
     Walk w;
     if (!w.init(a)) return;
-    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* ring_p = smem_raw + (ring - smem_u32(smem_raw));
-    const uint32_t qs = ring + C::NST * C::ENTRY;                    // hd 512: the second half of Q
-    const uint32_t bar0 = smem_u32(bars);
+    const uint32_t ring = smem_u32(smem);
+    if (ring & 1023u) {                      // the swizzled tiles need it; never the case
+        if (tid == 0) atomicOr(&g_status_paged_mma, kStatusTimeout);
+        return;
+    }
+    const uint32_t qs = ring + C::NST * C::ENTRY;                    // hd 512: the second half of Q; else the stages
+    const uint32_t bar0 = smem_u32(sm.bars);
     auto full = [&](int s) { return bar0 + 8u * s; };
     auto empty = [&](int s) { return bar0 + 8u * (C::NST + s); };
     const uint32_t b_s = bar0 + 8u * (2 * C::NST);                   // [2] scores of a unit are there
@@ -143,73 +183,72 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         for (int i = 0; i < 2 * C::NST; i++) mbar_init(bar0 + 8u * i, 1);
         mbar_init(b_s, 1);
         mbar_init(b_s + 8, 1);
-        mbar_init(b_p, 128);
-        mbar_init(b_p + 8, 128);
+        mbar_init(b_p, kSoft);
+        mbar_init(b_p + 8, kSoft);
         mbar_init(b_pv, 1);
         mbar_init(b_pv + 8, 1);
-        mbar_init(b_q, 128);
+        mbar_init(b_q, kSoft);
         mbar_init(b_drain, 1);
         fence_mbar_init();
-        s_abort = 0;
+        sm.abort = 0;
     }
-    if (warp == 5) {
-        tc::tmem_alloc(smem_u32(&s_tmem), 512);
+    if (warp == 9) {
+        tc::tmem_alloc(smem_u32(&sm.tmem), 512);
         tc::tmem_relinquish();
     }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    const uint32_t tmem = s_tmem;
-    volatile int* abort = &s_abort;
+    const uint32_t tmem = sm.tmem;
+    volatile int* abort = &sm.abort;
     unsigned* status = &g_status_paged_mma;
     const int pl = h->prefix_len, G = d.G;
 
-    if (warp == 4) {
+    if (warp == 8) {
         // ---------------------------------------------------------------- TMA
-        long long e = 0;                          // entries issued
+        int slot = 0, used = 0;                   // the next entry's slot; slots that were ever filled
+        uint32_t turn = 0;                        // parity of the ring's round
         bool ok = true;
         while (ok && w.next()) {
             const int head = w.head / C::CS, part = w.head % C::CS;
             const int* table = w.t.seq < 0 ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
             const int table_n = w.t.seq < 0 ? d.pre_pages : d.own_pages;
-            const int box = min(d.ps, kUnit), boxes = kUnit / box;   // rows of a box, boxes per unit
+            // An entry is DV / 64 column chunks of `boxes` boxes of `box` rows.  Each lane has one box of it: one
+            // instruction of the warp issues them all (one thread's loop over them took longer than the units' MMAs).
+            const int box = min(d.ps, kUnit), boxes = kUnit / box, lboxes = __ffs(boxes) - 1;
+            const int my_p = lane & (boxes - 1), my_c = lane >> lboxes;
+            const bool issues = my_c < C::DV / 64;
+            const uint32_t my_dst = ring + my_c * (kUnit * 128) + my_p * box * 128;
             int ids = -1, ids_at = -64;
             // unit u of the piece: K (all of hd) or V (this walk's columns)
             auto load = [&](int u, bool is_v) {
                 const int key = w.key0 + u * kUnit;
-                int row[kUnit / kPieceRowsMin];
-                #pragma unroll
-                for (int p = 0; p < kUnit / kPieceRowsMin; p++) {
-                    row[p] = 0;
-                    if (p < boxes) {
-                        const int k = key + p * box, idx = k / d.ps;
-                        if (idx < ids_at || idx >= ids_at + 32) {
-                            // 32 page ids ahead; from the unit before on, whose V may still be to come
-                            ids_at = max(w.key0, key - kUnit) / d.ps;
-                            ids = ids_at + lane < table_n ? __ldg(table + ids_at + lane) : -1;
-                        }
-                        const int id = __shfl_sync(0xffffffffu, ids, idx - ids_at);
-                        const int r = cache_row(id, a.num_pages, d.nkv, d.ps, head, k);
-                        row[p] = r < 0 ? a.num_pages * d.nkv * d.ps : r;   // past the map: zeros
-                    }
+                const int last = (key + kUnit - 1) / d.ps;
+                if (key / d.ps < ids_at || last >= ids_at + 32) {
+                    // 32 page ids ahead; from the unit before on, whose V may still be to come
+                    ids_at = max(w.key0, key - kUnit) / d.ps;
+                    ids = ids_at + lane < table_n ? __ldg(table + ids_at + lane) : -1;
                 }
+                const int k = key + my_p * box;
+                const int id = __shfl_sync(0xffffffffu, ids, k / d.ps - ids_at);
+                const int at_row = cache_row(id, a.num_pages, d.nkv, d.ps, head, k);
+                const int row = at_row < 0 ? a.num_pages * d.nkv * d.ps : at_row;   // past the map: zeros
                 for (int part_e = 0; part_e < (is_v ? 1 : C::KE); part_e++) {
-                    const int s = (int)(e % C::NST);
-                    const uint32_t use = (uint32_t)(e / C::NST);
-                    if (use > 0 && !mbar_wait(empty(s), (use - 1) & 1u, abort, status)) ok = false;
+                    const int s = slot;
+                    // from the second round on: the slot's products of the round before are done
+                    if (used == C::NST && !wait_short(empty(s), turn ^ 1u, abort, status)) ok = false;
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) return;
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(full(s), C::ENTRY);
-                        const int x0 = (is_v ? part : part_e) * C::DV;
-                        for (int c = 0; c < C::DV / 64; c++)
-                            #pragma unroll
-                            for (int p = 0; p < kUnit / kPieceRowsMin; p++)
-                                if (p < boxes)
-                                    tma_box(ring + s * C::ENTRY + c * (kUnit * 128) + p * box * 128, is_v ? &vmap : &kmap,
-                                            x0 + 64 * c, row[p], full(s));
+                    if (lane == 0) mbar_arrive_expect_tx(full(s), C::ENTRY);
+                    __syncwarp();
+                    if (issues)
+                        tma_box(my_dst + s * C::ENTRY, is_v ? &vmap : &kmap, (is_v ? part : part_e) * C::DV + 64 * my_c, row,
+                                full(s));
+                    used = max(used, s + 1);
+                    if (++slot == C::NST) {
+                        slot = 0;
+                        turn ^= 1u;
                     }
-                    e++;
                 }
             };
             load(0, false);
@@ -222,24 +261,31 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         __syncwarp();
         // every copy lands before the CTA gives up its shared memory
         if (*abort)
-            for (int s = 0; s < C::NST; s++) {
-                const long long uses = e > s ? (e - s - 1) / C::NST + 1 : 0;
-                if (uses > 0) mbar_wait_drain(full(s), (uint32_t)((uses - 1) & 1), status);
-            }
-    } else if (warp == 5) {
+            for (int s = 0; s < used; s++)        // the slots before the next one were filled in this round
+                mbar_wait_drain(full(s), s < slot ? turn : turn ^ 1u, status);
+    } else if (warp == 9) {
         // ---------------------------------------------------------------- MMA
         if (lane == 0) {
             constexpr uint32_t id_s = tc::idesc(1, 0, 0, 0, 0, kUnit, kRowsP);
             constexpr uint32_t id_o = tc::idesc(1, 0, 0, 0, 1, C::DV, kRowsP);
-            long long e = 0;
+            int slot = 0;                          // the next entry's
+            uint32_t turn = 0;                     // parity of the ring's round
             uint32_t it = 0, piece = 0;            // units and pieces so far
             bool ok = true;
             auto entry = [&](int& s) {             // the next entry, once it has landed
-                s = (int)(e % C::NST);
-                ok = ok && mbar_wait(full(s), (uint32_t)(e / C::NST) & 1u, abort, status);
-                e++;
+                s = slot;
+                ok = ok && wait_short(full(s), turn, abort, status);
+                if (++slot == C::NST) {
+                    slot = 0;
+                    turn ^= 1u;
+                }
                 return ok;
             };
+            // A descriptor's address field counts 16 bytes and has room for all of shared memory: the descriptors of an
+            // entry's tiles are its first one's plus a constant, one addition each.  (This thread's instructions
+            // between two MMAs of 32 clocks are what bounds the rate.)
+            const uint64_t k_desc = tc::sdesc_sw128(ring, 16, 1024), v_desc = tc::sdesc_sw128(ring, kUnit * 128, 1024);
+            const uint64_t q_desc = tc::sdesc_sw128(qs, 16, 1024);
             auto scores = [&](uint32_t i) {
                 const uint32_t ds = tmem + C::S_COL + (i & 1u) * kUnit;
                 #pragma unroll
@@ -247,39 +293,36 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     int s;
                     if (!entry(s)) return;
                     tc::fence_after();
+                    const uint64_t kd = k_desc + (uint64_t)(s * (C::ENTRY / 16));
                     #pragma unroll
                     for (int k = 0; k < C::QT / 16; k++) {
-                        const uint64_t bd = tc::sdesc_sw128(ring + s * C::ENTRY + (k / 4) * (kUnit * 128), 16, 1024) +
-                                            (uint64_t)((k % 4) * 2);
-                        if (pe == 0) {
+                        const uint64_t bd = kd + (uint64_t)((k / 4) * (kUnit * 128 / 16) + (k % 4) * 2);
+                        if (pe == 0)
                             tc::mma_f16_ts(ds, tmem + C::Q_COL + 8 * k, bd, id_s, k > 0);
-                        } else {
-                            const uint64_t ad = tc::sdesc_sw128(qs + (k / 4) * (kRowsP * 128), 16, 1024) +
-                                                (uint64_t)((k % 4) * 2);
-                            tc::mma_f16_ss(ds, ad, bd, id_s, 1);
-                        }
+                        else
+                            tc::mma_f16_ss(ds, q_desc + (uint64_t)((k / 4) * (kRowsP * 128 / 16) + (k % 4) * 2), bd, id_s, 1);
                     }
                     tc::commit(empty(s));
                 }
                 tc::commit(b_s + 8u * (i & 1u));
             };
             while (ok && w.next()) {
-                ok = mbar_wait(b_q, piece & 1u, abort, status);
+                ok = wait_short(b_q, piece & 1u, abort, status);
                 piece++;
                 tc::fence_after();
                 if (ok) scores(it);
                 for (int u = 0; ok && u < w.nu; u++) {
                     if (u + 1 < w.nu) scores(it + 1);
-                    ok = ok && mbar_wait(b_p + 8u * (it & 1u), (it >> 1) & 1u, abort, status);
+                    ok = ok && wait_short(b_p + 8u * (it & 1u), (it >> 1) & 1u, abort, status);
                     int s;
                     if (!ok || !entry(s)) break;
                     tc::fence_after();
-                    const int acc = u > 0 || *(volatile int*)&s_acc;
+                    const int acc = u > 0 || *(volatile int*)&sm.acc;
+                    const uint64_t vd = v_desc + (uint64_t)(s * (C::ENTRY / 16));
                     #pragma unroll
-                    for (int k = 0; k < kUnit / 16; k++)
+                    for (int k = 0; k < kUnit / 16; k++)      // 16 keys: two groups of 8 rows of 128 bytes
                         tc::mma_f16_ts(tmem + C::O_COL, tmem + C::S_COL + (it & 1u) * kUnit + 8 * k,
-                                       tc::sdesc_sw128(ring + s * C::ENTRY + k * 2048, kUnit * 128, 1024), id_o,
-                                       acc || k > 0);
+                                       vd + (uint64_t)(k * (2048 / 16)), id_o, acc || k > 0);
                     tc::commit(empty(s));
                     tc::commit(b_pv + 8u * (it & 1u));
                     it++;
@@ -293,15 +336,22 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         }
         __syncwarp();
     } else {
-        // ---------------------------------------------------------------- softmax: thread = row
-        const uint32_t tl = tmem + ((uint32_t)(warp * 32) << 16);    // this warp's lanes
+        // ---------------------------------------------------------------- softmax: two threads per row
+        // Thread `half` of row `r` takes 32 of a unit's 64 keys, half of Q's and of O's columns; the two rows of warps
+        // that share tensor memory lanes meet at a barrier of their own once per unit, for the row's maximum.
+        const int half = warp >> 2, wq = warp & 3, r0 = wq * 32 + lane;
+        const uint32_t tl = tmem + ((uint32_t)(wq * 32) << 16);      // this warp's lanes
+        constexpr int DH = C::DV / 2;                                // this half's columns of O
+        const uint32_t to = tl + C::O_COL + half * DH;
+        auto pair_sync = [&]() { named_bar_sync(2 + wq, 64); };
+        const uint32_t stage = qs + warp * C::STAGE;
         uint32_t it = 0;                          // units so far
         long long e0 = 0;                         // ring entries of the pieces before
-        // A wait that ran out clears ok.  The warp then walks on without waiting, so that the four warps meet at
+        // A wait that ran out clears ok.  The warp then walks on without waiting, so that the warps meet at
         // the same named barriers to the end; it writes no result.
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity, abort, status));
+            ok = __all_sync(0xffffffffu, ok && wait_short(bar, parity, abort, status));
         };
         // The product of a unit is added.  A parity tells a barrier's last two phases apart only: units alternate
         // between two barriers, and every unit u waits for unit u - 2's, so neither runs ahead unseen.
@@ -311,33 +361,59 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         };
         while (w.next()) {
             const int head = w.head / C::CS, part = w.head % C::CS;
-            const bool live = tid < w.t.nrows;
-            const int row = w.t.row0 + min(tid, w.t.nrows - 1);
+            const bool live = r0 < w.t.nrows;
+            const int row = w.t.row0 + min(r0, w.t.nrows - 1);
             const int tok = row / G, hq = head * G + row % G;
-            // Q's row into tensor memory (two elements per column) and, past QT, shared memory
+            // Q's rows into tensor memory (two elements per column) and, past QT, shared memory.  Eight lanes read 128
+            // bytes of a row; the stage turns rows over lanes into a row per lane.
             {
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + (long long)tok * a.q_stride + (long long)hq * HD);
+                const long long mine = ((long long)tok * a.q_stride + (long long)hq * HD) * 2;
+                const char* qb = reinterpret_cast<const char*>(a.q) + (lane & 7) * 16;
+                auto fetch = [&](int c, uint4 (&x)[8]) {       // chunk c: 64 elements of rows 4 i + lane / 8
+                    #pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int r = 4 * i + (lane >> 3);
+                        const long long o = __shfl_sync(0xffffffffu, mine, r);
+                        x[i] = wq * 32 + r < w.t.nrows ? __ldg(reinterpret_cast<const uint4*>(qb + o + c * 128))
+                                                         : make_uint4(0, 0, 0, 0);
+                    }
+                };
+                constexpr int CH = C::QT / 128;                // chunks of this half
+                uint4 x[CH][8];
                 #pragma unroll
-                for (int c = 0; c < C::QT / 64; c++) {
+                for (int c = 0; c < CH; c++) fetch(half * CH + c, x[c]);
+                #pragma unroll
+                for (int c = 0; c < CH; c++) {
+                    #pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int r = 4 * i + (lane >> 3);
+                        st_shared(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4), x[c][i]);
+                    }
+                    __syncwarp();
                     uint32_t v[32];
                     #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        const uint4 x = live ? __ldg(src + c * 8 + j) : make_uint4(0, 0, 0, 0);
-                        v[4 * j] = x.x;
-                        v[4 * j + 1] = x.y;
-                        v[4 * j + 2] = x.z;
-                        v[4 * j + 3] = x.w;
+                        const uint4 y = ld_shared(stage + lane * 128 + ((j ^ (lane & 7)) << 4));
+                        v[4 * j] = y.x;
+                        v[4 * j + 1] = y.y;
+                        v[4 * j + 2] = y.z;
+                        v[4 * j + 3] = y.w;
                     }
-                    tc::st_32x32b_x32(tl + C::Q_COL + 32 * c, v);
+                    tc::st_32x32b_x32(tl + C::Q_COL + 32 * (half * CH + c), v);
+                    __syncwarp();
                 }
                 if constexpr (HD > C::QT) {
-                    #pragma unroll 8
-                    for (int j = 0; j < (HD - C::QT) / 8; j++) {
-                        const uint4 x = live ? __ldg(src + C::QT / 8 + j) : make_uint4(0, 0, 0, 0);
-                        const uint32_t dst = qs + (j / 8) * (kRowsP * 128) + tid * 128 + (((j & 7) ^ (tid & 7)) << 4);
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(x.x), "r"(x.y), "r"(x.z),
-                                     "r"(x.w) : "memory");
-                    }
+                    constexpr int CR = (HD - C::QT) / 128;
+                    #pragma unroll
+                    for (int c = 0; c < CR; c++) fetch(C::QT / 64 + half * CR + c, x[c]);
+                    named_bar_sync(1, kSoft);   // the stages lie where the rest of Q goes
+                    #pragma unroll
+                    for (int c = 0; c < CR; c++)
+                        #pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const int r = wq * 32 + 4 * i + (lane >> 3);
+                            st_shared(qs + (half * CR + c) * (kRowsP * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4), x[c][i]);
+                        }
                     tc::fence_proxy_async_smem();
                 }
                 tc::wait_st();
@@ -352,23 +428,23 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             // keys that all rows see, keys that any row sees
             int all_lo = __reduce_max_sync(0xffffffffu, vlo), all_hi = __reduce_min_sync(0xffffffffu, vhi);
             int any_lo = __reduce_min_sync(0xffffffffu, vlo), any_hi = __reduce_max_sync(0xffffffffu, vhi);
-            named_bar_sync(1, 128);               // the piece before has been read out of s_red
-            if (lane == 0) {
-                s_red[warp][0] = all_lo;
-                s_red[warp][1] = all_hi;
-                s_red[warp][2] = any_lo;
-                s_red[warp][3] = any_hi;
+            named_bar_sync(1, kSoft);             // the piece before has been read out of sm.red
+            if (lane == 0 && half == 0) {
+                sm.red[wq][0] = all_lo;
+                sm.red[wq][1] = all_hi;
+                sm.red[wq][2] = any_lo;
+                sm.red[wq][3] = any_hi;
             }
-            named_bar_sync(1, 128);
+            named_bar_sync(1, kSoft);
             #pragma unroll
             for (int i = 0; i < 4; i++) {
-                all_lo = max(all_lo, s_red[i][0]);
-                all_hi = min(all_hi, s_red[i][1]);
-                any_lo = min(any_lo, s_red[i][2]);
-                any_hi = max(any_hi, s_red[i][3]);
+                all_lo = max(all_lo, sm.red[i][0]);
+                all_hi = min(all_hi, sm.red[i][1]);
+                any_lo = min(any_lo, sm.red[i][2]);
+                any_hi = max(any_hi, sm.red[i][3]);
             }
             // page ids of a unit, one per box, in the first lanes; fetched a unit ahead
-            const int box = min(d.ps, kUnit), boxes = kUnit / box, lbox = __ffs(box) - 1;
+            const int box = min(d.ps, kUnit), boxes = kUnit / box;
             auto page_of = [&](int u) {
                 const int k = w.key0 + u * kUnit + (lane & 3) * box, idx = k / d.ps;
                 return lane < boxes && u < w.nu && idx < table_n ? __ldg(table + idx) : -1;
@@ -384,92 +460,110 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 if (it >= 2) wait_pv(it - 2);
                 tc::fence_after();
                 const uint32_t ts = tl + C::S_COL + (it & 1u) * kUnit;
-                uint32_t x0[32], x1[32];
-                tc::ld_32x32b_x32(ts, x0);
-                tc::ld_32x32b_x32(ts + 32, x1);
+                uint32_t x[32];
+                tc::ld_32x32b_x32(ts + half * 32, x);
                 tc::wait_ld();
                 if (edge) {
+                    // the keys that this row sees, one bit each
+                    auto below = [&](int k) { return k >= kUnit ? ~0ull : k <= 0 ? 0ull : (1ull << k) - 1; };
+                    unsigned long long bits = below(vhi - key) & ~below(vlo - key);
+                    if (there != (1u << boxes) - 1)
+                        for (int b = 0; b < boxes; b++)
+                            if (!((there >> b) & 1u)) bits &= ~(below((b + 1) * box) & ~below(b * box));
+                    const uint32_t mine = (uint32_t)(bits >> (32 * half));
                     #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const bool ta = (there >> (j >> lbox)) & 1u, tb = (there >> ((j + 32) >> lbox)) & 1u;
-                        if (!ta || key + j < vlo || key + j >= vhi) x0[j] = 0xff800000u;
-                        if (!tb || key + j + 32 < vlo || key + j + 32 >= vhi) x1[j] = 0xff800000u;
-                    }
+                    for (int j = 0; j < 32; j++)
+                        if (!((mine >> j) & 1u)) x[j] = 0xff800000u;
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 #pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    mx[0] = fmaxf(mx[0], __uint_as_float(x0[j]));
-                    mx[1] = fmaxf(mx[1], __uint_as_float(x0[j + 1]));
-                    mx[2] = fmaxf(mx[2], __uint_as_float(x1[j]));
-                    mx[3] = fmaxf(mx[3], __uint_as_float(x1[j + 1]));
-                }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
-                // units so far of this piece are in O: rescale it where a row's maximum has left its base behind
+                for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(x[j]));
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                sm.top[it & 1][half][r0] = top;
+                tc::fence_before();
+                pair_sync();          // both have read their scores, too: P goes over them
+                tc::fence_after();
+                top = fmaxf(top, sm.top[it & 1][half ^ 1][r0]) * a.scale;
+                // Units so far of this piece are in O: rescale it where a row's maximum has left its base behind.
+                // A row that saw nothing yet has zeros there and in l.
                 if (u == 0) {
-                    m = top;
+                    m = top - kLift;
                 } else {
-                    const bool rise = top > m + kLazy || (m == -INFINITY && top > m);
-                    if (__any_sync(0xffffffffu, rise)) {
-                        const float f = rise ? exp2_approx(m - top) : 1.f;     // m = -inf: nothing was added yet
-                        if (rise) m = top;
+                    const bool set = top > m + kMost, scale = set && m != -INFINITY;
+                    if (__any_sync(0xffffffffu, scale)) {
+                        const float f = scale ? exp2_approx(m - (top - kLift)) : 1.f;
                         l *= f;
                         wait_pv(it - 1);
                         #pragma unroll
-                        for (int c = 0; c < C::DV; c += 32) {
+                        for (int c = 0; c < DH; c += 32) {
                             uint32_t o[32];
-                            tc::ld_32x32b_x32(tl + C::O_COL + c, o);
+                            tc::ld_32x32b_x32(to + c, o);
                             tc::wait_ld();
                             #pragma unroll
                             for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                            tc::st_32x32b_x32(tl + C::O_COL + c, o);
+                            tc::st_32x32b_x32(to + c, o);
                         }
                     }
+                    if (set) m = top - kLift;
                 }
                 const float base = m == -INFINITY ? 0.f : m;
-                float sum[2] = {0.f, 0.f};
-                uint32_t p[32];
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t p[16];
                 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    const float e00 = exp2_approx(fmaf(__uint_as_float(x0[2 * j]), a.scale, -base));
-                    const float e01 = exp2_approx(fmaf(__uint_as_float(x0[2 * j + 1]), a.scale, -base));
-                    const float e10 = exp2_approx(fmaf(__uint_as_float(x1[2 * j]), a.scale, -base));
-                    const float e11 = exp2_approx(fmaf(__uint_as_float(x1[2 * j + 1]), a.scale, -base));
-                    sum[0] += e00 + e01;
-                    sum[1] += e10 + e11;
-                    const __half2 h0 = __floats2half2_rn(e00, e01), h1 = __floats2half2_rn(e10, e11);
-                    p[j] = *reinterpret_cast<const uint32_t*>(&h0);
-                    p[16 + j] = *reinterpret_cast<const uint32_t*>(&h1);
+                    const float e0 = exp2_approx(fmaf(__uint_as_float(x[2 * j]), a.scale, -base));
+                    const float e1 = exp2_approx(fmaf(__uint_as_float(x[2 * j + 1]), a.scale, -base));
+                    sum[j & 3] += e0 + e1;
+                    const __half2 h2 = __floats2half2_rn(e0, e1);
+                    p[j] = *reinterpret_cast<const uint32_t*>(&h2);
                 }
-                l += sum[0] + sum[1];
-                tc::st_32x32b_x32(ts, p);
-                if (u == 0 && tid == 0) *(volatile int*)&s_acc = 0;
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tc::st_32x32b_x16(ts + half * 16, p);
+                if (u == 0 && tid == 0) *(volatile int*)&sm.acc = 0;
                 if (edge) {
                     // Values that no row sees become zeros; values that only some rows see and that are not
                     // finite (0 x NaN is not 0) are added row by row here and then cleared.
                     const long long ev = e0 + (u + 1 < w.nu ? (long long)C::KE * (u + 2) + u : (long long)C::KE * w.nu + u);
                     const int s = (int)(ev % C::NST);
                     wait(full(s), (uint32_t)(ev / C::NST) & 1u);
-                    if (tid == 0) s_odd = 0;
-                    named_bar_sync(1, 128);
-                    uint4* vt = reinterpret_cast<uint4*>(ring_p + s * C::ENTRY);    // [DV / 64][64 keys][8 x 16 bytes]
-                    for (int i = tid; i < C::ENTRY / 16; i += 128) {
-                        const int k = key + (i >> 3) % kUnit;
-                        if (k < any_lo || k >= any_hi) {
-                            vt[i] = make_uint4(0, 0, 0, 0);
-                        } else if (k < all_lo || k >= all_hi) {
-                            const uint4 v = vt[i];
-                            auto odd = [](uint32_t y) {
-                                return (y & 0x7c00u) == 0x7c00u || (y & 0x7c000000u) == 0x7c000000u;
-                            };
-                            if (odd(v.x) || odd(v.y) || odd(v.z) || odd(v.w))
-                                atomicOr(&s_odd, 1ull << ((i >> 3) % kUnit));
+                    // this thread's share: 16 bytes (tid % 8) of keys tid / 8 + 32 r in each 64-column chunk
+                    const uint32_t vt = ring + s * C::ENTRY + tid * 16;
+                    uint32_t bad = 0;
+                    bool some[2];                            // key r is seen by some rows only
+                    #pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const int k = key + (tid >> 3) + 32 * r;
+                        const bool none = k < any_lo || k >= any_hi;
+                        some[r] = !none && (k < all_lo || k >= all_hi);
+                        #pragma unroll
+                        for (int c = 0; c < C::DV / 64; c++) {
+                            const uint32_t at = vt + c * (kUnit * 128) + r * (32 * 128);
+                            if (none) {
+                                st_shared(at, make_uint4(0, 0, 0, 0));
+                            } else if (some[r]) {
+                                const uint4 v = ld_shared(at);
+                                bad |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
+                            }
                         }
                     }
-                    named_bar_sync(1, 128);
-                    unsigned long long odd = s_odd;
+                    unsigned long long odd = 0;
+                    if (any_soft((bad & 0x80008000u) != 0)) {
+                        if (tid == 0) sm.odd = 0;
+                        named_bar_sync(1, kSoft);
+                        for (int r = 0; r < 2; r++)
+                            for (int c = 0; c < C::DV / 64 && some[r]; c++) {
+                                const uint4 v = ld_shared(vt + c * (kUnit * 128) + r * (32 * 128));
+                                if ((not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w)) & 0x80008000u)
+                                    atomicOr(&sm.odd, 1ull << ((tid >> 3) + 32 * r));
+                            }
+                        named_bar_sync(1, kSoft);
+                        odd = *(volatile unsigned long long*)&sm.odd;
+                    }
                     if (odd) {
-                        tc::wait_st();                       // P, read back below
+                        tc::wait_st();                       // P, read back below, the other half's too
+                        tc::fence_before();
+                        named_bar_sync(1, kSoft);
+                        tc::fence_after();
                         if (u > 0) {
                             wait_pv(it - 1);
                         } else {
@@ -477,9 +571,9 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                             #pragma unroll
                             for (int j = 0; j < 32; j++) z[j] = 0;
                             #pragma unroll
-                            for (int c = 0; c < C::DV; c += 32) tc::st_32x32b_x32(tl + C::O_COL + c, z);
+                            for (int c = 0; c < DH; c += 32) tc::st_32x32b_x32(to + c, z);
                             tc::wait_st();
-                            if (tid == 0) *(volatile int*)&s_acc = 1;
+                            if (tid == 0) *(volatile int*)&sm.acc = 1;
                         }
                         while (odd) {
                             const int j = __ffsll((long long)odd) - 1;
@@ -487,20 +581,20 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                             const uint32_t pj = ld_tmem_x1(ts + j / 2);
                             tc::wait_ld();
                             const float pf = j & 1 ? h_hi(pj) : h_lo(pj);
-                            const bool sees = key + j >= vlo && key + j < vhi && ((there >> (j >> lbox)) & 1u);
+                            const bool sees = key + j >= vlo && key + j < vhi && ((there >> (j / box)) & 1u);
                             #pragma unroll 1
-                            for (int c = 0; c < C::DV; c += 32) {
+                            for (int c = half * DH; c < (half + 1) * DH; c += 32) {
                                 uint32_t o[32];
                                 tc::ld_32x32b_x32(tl + C::O_COL + c, o);
                                 tc::wait_ld();
-                                const uint8_t* vr = ring_p + s * C::ENTRY + (c / 64) * (kUnit * 128) + j * 128;
+                                const uint32_t vr = ring + s * C::ENTRY + (c / 64) * (kUnit * 128) + j * 128;
                                 #pragma unroll
                                 for (int q = 0; q < 4; q++) {
                                     const int un = (c % 64) / 8 + q;
-                                    const uint4 v = *reinterpret_cast<const uint4*>(vr + ((un ^ (j & 7)) << 4));
+                                    const uint4 v = ld_shared(vr + ((un ^ (j & 7)) << 4));
                                     const uint32_t y[4] = {v.x, v.y, v.z, v.w};
                                     #pragma unroll
-                                    for (int r = 0; r < 4; r++) {
+                                    for (int r = 0; r < 2; r++) {
                                         float lo = __uint_as_float(o[8 * q + 2 * r]), hi = __uint_as_float(o[8 * q + 2 * r + 1]);
                                         if (sees) {
                                             lo += pf * h_lo(y[r]);
@@ -514,10 +608,13 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                                 tc::wait_st();
                             }
                         }
-                        named_bar_sync(1, 128);              // every row has read the values
-                        odd = s_odd;
-                        for (int i = tid; i < C::ENTRY / 16; i += 128)
-                            if ((odd >> ((i >> 3) % kUnit)) & 1ull) vt[i] = make_uint4(0, 0, 0, 0);
+                        named_bar_sync(1, kSoft);              // every row has read the values
+                        odd = *(volatile unsigned long long*)&sm.odd;
+                        for (int r = 0; r < 2; r++)
+                            for (int c = 0; c < C::DV / 64; c++)
+                                if ((odd >> ((tid >> 3) + 32 * r)) & 1ull)
+                                    st_shared(vt + c * (kUnit * 128) + r * (32 * 128), make_uint4(0, 0, 0, 0));
+                        named_bar_sync(1, kSoft);              // sm.odd has been read
                     }
                     tc::fence_proxy_async_smem();
                 }
@@ -526,42 +623,67 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 mbar_arrive(b_p + 8u * (it & 1u));
             }
             wait_pv(it - 1);
+            sm.top[it & 1][half][r0] = l;
+            pair_sync();
+            l += sm.top[it & 1][half ^ 1][r0];
+            pair_sync();
             // the row's result: finished, or this stretch's part of it
             const bool whole = w.nu == w.t.n, direct = whole && w.t.solo;
             const float inv = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;
             const size_t slot = whole ? ((size_t)(w.t.seq < 0 ? 0 : 1) * d.T + tok) * d.nH + hq
-                                      : ((size_t)blockIdx.x * 2 + (w.unit == 0 ? 1 : 0)) * kRowsP + tid;
-            float* dst = whole ? a.w.row + slot * HD + part * C::DV : a.w.edge[1] + slot * C::DV;
-            const long long at0 = (long long)tok * a.out_stride + (long long)hq * HD + part * C::DV;
-            if (live && ok && !direct) {
+                                      : ((size_t)blockIdx.x * 2 + (w.unit == 0 ? 1 : 0)) * kRowsP + r0;
+            if (live && ok && !direct && half == 0) {
                 if (whole) a.w.row_ml[slot * 2 + part] = make_float2(m, l);
                 else a.w.edge_ml[1][slot] = make_float2(m, l);
             }
-            #pragma unroll 2
-            for (int c = 0; c < C::DV; c += 32) {
-                uint32_t o[32];
-                tc::ld_32x32b_x32(tl + C::O_COL + c, o);
-                tc::wait_ld();
-                if (!live || !ok) continue;
-                if (direct && !a.out_f32) {
-                    uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<__half*>(a.out) + at0 + c);
+            char* dst = reinterpret_cast<char*>(!direct ? whole ? a.w.row : a.w.edge[1] : a.out);
+            const size_t elem = direct && !a.out_f32 ? 2 : 4;
+            const size_t mine = elem * (!direct ? whole ? slot * HD + part * C::DV : slot * C::DV
+                                                : (size_t)tok * a.out_stride + (size_t)hq * HD + part * C::DV);
+            // 128 bytes of every row of the warp, from a row per lane to eight lanes per row
+            auto flush = [&](const uint32_t (&v)[32], size_t off) {
+                #pragma unroll
+                for (int j = 0; j < 8; j++)
+                    st_shared(stage + lane * 128 + ((j ^ (lane & 7)) << 4),
+                              make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                __syncwarp();
+                #pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int r = 4 * i + (lane >> 3);
+                    const uint4 x = ld_shared(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                    const size_t o = __shfl_sync(0xffffffffu, mine, r) + off;
+                    if (ok && wq * 32 + r < w.t.nrows) *reinterpret_cast<uint4*>(dst + o + (lane & 7) * 16) = x;
+                }
+                __syncwarp();
+            };
+            if (elem == 4) {
+                #pragma unroll 1
+                for (int c = half * DH; c < (half + 1) * DH; c += 32) {
+                    uint32_t o[32];
+                    tc::ld_32x32b_x32(tl + C::O_COL + c, o);
+                    tc::wait_ld();
                     #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        uint32_t y[4];
+                    for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * inv);
+                    flush(o, (size_t)c * 4);
+                }
+            } else {
+                #pragma unroll 1
+                for (int c = half * DH; c < (half + 1) * DH; c += 64) {
+                    uint32_t y[32];
+                    #pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        uint32_t o[32];
+                        tc::ld_32x32b_x32(tl + C::O_COL + c + 32 * k, o);
+                        tc::wait_ld();
                         #pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            y[r] = pack_half2(__float2half_rn(__uint_as_float(o[8 * j + 2 * r]) * inv),
-                                              __float2half_rn(__uint_as_float(o[8 * j + 2 * r + 1]) * inv));
-                        out[j] = make_uint4(y[0], y[1], y[2], y[3]);
+                        for (int j = 0; j < 16; j++)
+                            y[16 * k + j] = pack_half2(__float2half_rn(__uint_as_float(o[2 * j]) * inv),
+                                                       __float2half_rn(__uint_as_float(o[2 * j + 1]) * inv));
                     }
-                } else {
-                    float4* out = reinterpret_cast<float4*>(direct ? reinterpret_cast<float*>(a.out) + at0 + c : dst + c);
-                    #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        out[j] = make_float4(__uint_as_float(o[4 * j]) * inv, __uint_as_float(o[4 * j + 1]) * inv,
-                                             __uint_as_float(o[4 * j + 2]) * inv, __uint_as_float(o[4 * j + 3]) * inv);
+                    flush(y, (size_t)c * 2);
                 }
             }
+            if constexpr (HD > C::QT) named_bar_sync(1, kSoft);   // the stages: the next piece's Q goes there
             tc::fence_before();
             e0 += (long long)(C::KE + 1) * w.nu;
             w.step();
@@ -570,7 +692,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    if (warp == 5) tc::tmem_dealloc(tmem, 512);
+    if (warp == 9) tc::tmem_dealloc(tmem, 512);
 }
 
 bool many_rows(int hd) { return hd == 128 || hd == 256 || hd == 512; }
