@@ -75,6 +75,13 @@ __device__ __forceinline__ uint32_t ld_tmem_x1(uint32_t taddr) {
     return v;
 }
 
+// One lane of a converged warp.  The MMA warp runs as a whole and lets one lane issue: an MMA of 128 x 64 x 16 then
+// takes 32 clocks to issue, against 46 where lane 0 alone runs the role (descriptors stay in uniform registers).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 // or of all softmax threads' flags
 __device__ __forceinline__ bool any_soft(bool v) {
     int r;
@@ -265,35 +272,37 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 mbar_wait_drain(full(s), s < slot ? turn : turn ^ 1u, status);
     } else if (warp == 9) {
         // ---------------------------------------------------------------- MMA
-        if (lane == 0) {
-            constexpr uint32_t id_s = tc::idesc(1, 0, 0, 0, 0, kUnit, kRowsP);
-            constexpr uint32_t id_o = tc::idesc(1, 0, 0, 0, 1, C::DV, kRowsP);
-            int slot = 0;                          // the next entry's
-            uint32_t turn = 0;                     // parity of the ring's round
-            uint32_t it = 0, piece = 0;            // units and pieces so far
-            bool ok = true;
-            auto entry = [&](int& s) {             // the next entry, once it has landed
-                s = slot;
-                ok = ok && wait_short(full(s), turn, abort, status);
-                if (++slot == C::NST) {
-                    slot = 0;
-                    turn ^= 1u;
-                }
-                return ok;
-            };
-            // A descriptor's address field counts 16 bytes and has room for all of shared memory: the descriptors of an
-            // entry's tiles are its first one's plus a constant, one addition each.  (This thread's instructions
-            // between two MMAs of 32 clocks are what bounds the rate.)
-            const uint64_t k_desc = tc::sdesc_sw128(ring, 16, 1024), v_desc = tc::sdesc_sw128(ring, kUnit * 128, 1024);
-            const uint64_t q_desc = tc::sdesc_sw128(qs, 16, 1024);
-            auto scores = [&](uint32_t i) {
-                const uint32_t ds = tmem + C::S_COL + (i & 1u) * kUnit;
-                #pragma unroll
-                for (int pe = 0; pe < C::KE; pe++) {
-                    int s;
-                    if (!entry(s)) return;
-                    tc::fence_after();
-                    const uint64_t kd = k_desc + (uint64_t)(s * (C::ENTRY / 16));
+        constexpr uint32_t id_s = tc::idesc(1, 0, 0, 0, 0, kUnit, kRowsP);
+        constexpr uint32_t id_o = tc::idesc(1, 0, 0, 0, 1, C::DV, kRowsP);
+        int slot = 0;                              // the next entry's
+        uint32_t turn = 0;                         // parity of the ring's round
+        uint32_t it = 0, piece = 0;                // units and pieces so far
+        bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            ok = __all_sync(0xffffffffu, ok && wait_short(bar, parity, abort, status));
+            tc::fence_after();
+        };
+        auto entry = [&]() {                       // the next entry, once it has landed
+            const int s = slot;
+            wait(full(s), turn);
+            if (++slot == C::NST) {
+                slot = 0;
+                turn ^= 1u;
+            }
+            return s;
+        };
+        // A descriptor's address field counts 16 bytes and has room for all of shared memory: the descriptors of an
+        // entry's tiles are its first one's plus a constant.
+        const uint64_t k_desc = tc::sdesc_sw128(ring, 16, 1024), v_desc = tc::sdesc_sw128(ring, kUnit * 128, 1024);
+        const uint64_t q_desc = tc::sdesc_sw128(qs, 16, 1024);
+        auto scores = [&](uint32_t i) {
+            const uint32_t ds = tmem + C::S_COL + (i & 1u) * kUnit;
+            #pragma unroll
+            for (int pe = 0; pe < C::KE; pe++) {
+                const int s = entry();
+                if (!ok) return;
+                const uint64_t kd = k_desc + (uint64_t)(s * (C::ENTRY / 16));
+                if (elect_one()) {
                     #pragma unroll
                     for (int k = 0; k < C::QT / 16; k++) {
                         const uint64_t bd = kd + (uint64_t)((k / 4) * (kUnit * 128 / 16) + (k % 4) * 2);
@@ -303,36 +312,39 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                             tc::mma_f16_ss(ds, q_desc + (uint64_t)((k / 4) * (kRowsP * 128 / 16) + (k % 4) * 2), bd, id_s, 1);
                     }
                     tc::commit(empty(s));
+                    if (pe == C::KE - 1) tc::commit(b_s + 8u * (i & 1u));
                 }
-                tc::commit(b_s + 8u * (i & 1u));
-            };
-            while (ok && w.next()) {
-                ok = wait_short(b_q, piece & 1u, abort, status);
-                piece++;
-                tc::fence_after();
-                if (ok) scores(it);
-                for (int u = 0; ok && u < w.nu; u++) {
-                    if (u + 1 < w.nu) scores(it + 1);
-                    ok = ok && wait_short(b_p + 8u * (it & 1u), (it >> 1) & 1u, abort, status);
-                    int s;
-                    if (!ok || !entry(s)) break;
-                    tc::fence_after();
-                    const int acc = u > 0 || *(volatile int*)&sm.acc;
-                    const uint64_t vd = v_desc + (uint64_t)(s * (C::ENTRY / 16));
+                __syncwarp();
+            }
+        };
+        while (ok && w.next()) {
+            wait(b_q, piece & 1u);
+            piece++;
+            if (ok) scores(it);
+            for (int u = 0; ok && u < w.nu; u++) {
+                if (u + 1 < w.nu) scores(it + 1);
+                wait(b_p + 8u * (it & 1u), (it >> 1) & 1u);
+                const int s = entry();
+                if (!ok) break;
+                const int acc = u > 0 || *(volatile int*)&sm.acc;
+                const uint64_t vd = v_desc + (uint64_t)(s * (C::ENTRY / 16));
+                if (elect_one()) {
                     #pragma unroll
                     for (int k = 0; k < kUnit / 16; k++)      // 16 keys: two groups of 8 rows of 128 bytes
                         tc::mma_f16_ts(tmem + C::O_COL, tmem + C::S_COL + (it & 1u) * kUnit + 8 * k,
                                        vd + (uint64_t)(k * (2048 / 16)), id_o, acc || k > 0);
                     tc::commit(empty(s));
                     tc::commit(b_pv + 8u * (it & 1u));
-                    it++;
                 }
-                w.step();
+                __syncwarp();
+                it++;
             }
-            if (*abort) {
-                tc::commit(b_drain);
-                mbar_wait_drain(b_drain, 0, status);
-            }
+            w.step();
+        }
+        if (*abort) {
+            if (elect_one()) tc::commit(b_drain);
+            __syncwarp();
+            mbar_wait_drain(b_drain, 0, status);
         }
         __syncwarp();
     } else {
@@ -359,15 +371,13 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             wait(b_pv + 8u * (unit & 1u), (unit >> 1) & 1u);
             tc::fence_after();
         };
-        while (w.next()) {
-            const int head = w.head / C::CS, part = w.head % C::CS;
-            const bool live = r0 < w.t.nrows;
+        // Q of the piece that w stands at
+        auto load_q = [&]() {
             const int row = w.t.row0 + min(r0, w.t.nrows - 1);
-            const int tok = row / G, hq = head * G + row % G;
             // Q's rows into tensor memory (two elements per column) and, past QT, shared memory.  Eight lanes read 128
             // bytes of a row; the stage turns rows over lanes into a row per lane.
             {
-                const long long mine = ((long long)tok * a.q_stride + (long long)hq * HD) * 2;
+                const long long mine = ((long long)(row / G) * a.q_stride + (long long)((w.head / C::CS) * G + row % G) * HD) * 2;
                 const char* qb = reinterpret_cast<const char*>(a.q) + (lane & 7) * 16;
                 auto fetch = [&](int c, uint4 (&x)[8]) {       // chunk c: 64 elements of rows 4 i + lane / 8
                     #pragma unroll
@@ -420,6 +430,13 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 tc::fence_before();
                 mbar_arrive(b_q);
             }
+        };
+        bool more = w.next();
+        if (more) load_q();
+        while (more) {
+            const int head = w.head / C::CS, part = w.head % C::CS;
+            const int nrows = w.t.nrows, row = w.t.row0 + min(r0, nrows - 1);
+            const int tok = row / G, hq = head * G + row % G;
             const int kbase = w.t.seq < 0 ? 0 : pl;
             const int* table = w.t.seq < 0 ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
             const int table_n = w.t.seq < 0 ? d.pre_pages : d.own_pages;
@@ -575,9 +592,8 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                             tc::wait_st();
                             if (tid == 0) *(volatile int*)&sm.acc = 1;
                         }
-                        while (odd) {
-                            const int j = __ffsll((long long)odd) - 1;
-                            odd &= odd - 1;
+                        for (unsigned long long rest = odd; rest; rest &= rest - 1) {
+                            const int j = __ffsll((long long)rest) - 1;
                             const uint32_t pj = ld_tmem_x1(ts + j / 2);
                             tc::wait_ld();
                             const float pf = j & 1 ? h_hi(pj) : h_lo(pj);
@@ -609,37 +625,39 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                             }
                         }
                         named_bar_sync(1, kSoft);              // every row has read the values
-                        odd = *(volatile unsigned long long*)&sm.odd;
                         for (int r = 0; r < 2; r++)
                             for (int c = 0; c < C::DV / 64; c++)
                                 if ((odd >> ((tid >> 3) + 32 * r)) & 1ull)
                                     st_shared(vt + c * (kUnit * 128) + r * (32 * 128), make_uint4(0, 0, 0, 0));
-                        named_bar_sync(1, kSoft);              // sm.odd has been read
                     }
-                    tc::fence_proxy_async_smem();
+                    if (odd || key < any_lo || key + kUnit > any_hi) tc::fence_proxy_async_smem();   // V was written
                 }
                 tc::wait_st();
                 tc::fence_before();
                 mbar_arrive(b_p + 8u * (it & 1u));
             }
+            // where the row's result goes: finished, or this stretch's part of it
+            const bool whole = w.nu == w.t.n, direct = whole && w.t.solo;
+            const size_t slot = whole ? ((size_t)(w.t.seq < 0 ? 0 : 1) * d.T + tok) * d.nH + hq
+                                      : ((size_t)blockIdx.x * 2 + (w.unit == 0 ? 1 : 0)) * kRowsP + r0;
+            char* dst = reinterpret_cast<char*>(!direct ? whole ? a.w.row : a.w.edge[1] : a.out);
+            const size_t elem = direct && !a.out_f32 ? 2 : 4;
+            const size_t mine = elem * (!direct ? whole ? slot * HD + part * C::DV : slot * C::DV
+                                                : (size_t)tok * a.out_stride + (size_t)hq * HD + part * C::DV);
+            e0 += (long long)(C::KE + 1) * w.nu;
+            w.step();
+            more = w.next();
+            // The scores of this piece are all made: the next one's Q may come, so that its first scores are made while
+            // this one's result is written.  (At hd 512 the stages lie in Q's place: after that.)
+            if (HD == C::QT && more) load_q();
             wait_pv(it - 1);
             sm.top[it & 1][half][r0] = l;
             pair_sync();
             l += sm.top[it & 1][half ^ 1][r0];
             pair_sync();
-            // the row's result: finished, or this stretch's part of it
-            const bool whole = w.nu == w.t.n, direct = whole && w.t.solo;
             const float inv = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            const size_t slot = whole ? ((size_t)(w.t.seq < 0 ? 0 : 1) * d.T + tok) * d.nH + hq
-                                      : ((size_t)blockIdx.x * 2 + (w.unit == 0 ? 1 : 0)) * kRowsP + r0;
-            if (live && ok && !direct && half == 0) {
-                if (whole) a.w.row_ml[slot * 2 + part] = make_float2(m, l);
-                else a.w.edge_ml[1][slot] = make_float2(m, l);
-            }
-            char* dst = reinterpret_cast<char*>(!direct ? whole ? a.w.row : a.w.edge[1] : a.out);
-            const size_t elem = direct && !a.out_f32 ? 2 : 4;
-            const size_t mine = elem * (!direct ? whole ? slot * HD + part * C::DV : slot * C::DV
-                                                : (size_t)tok * a.out_stride + (size_t)hq * HD + part * C::DV);
+            if (r0 < nrows && ok && !direct && half == 0)
+                *(whole ? a.w.row_ml + slot * 2 + part : a.w.edge_ml[1] + slot) = make_float2(m, l);
             // 128 bytes of every row of the warp, from a row per lane to eight lanes per row
             auto flush = [&](const uint32_t (&v)[32], size_t off) {
                 #pragma unroll
@@ -652,7 +670,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     const int r = 4 * i + (lane >> 3);
                     const uint4 x = ld_shared(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
                     const size_t o = __shfl_sync(0xffffffffu, mine, r) + off;
-                    if (ok && wq * 32 + r < w.t.nrows) *reinterpret_cast<uint4*>(dst + o + (lane & 7) * 16) = x;
+                    if (ok && wq * 32 + r < nrows) *reinterpret_cast<uint4*>(dst + o + (lane & 7) * 16) = x;
                 }
                 __syncwarp();
             };
@@ -683,10 +701,11 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     flush(y, (size_t)c * 2);
                 }
             }
-            if constexpr (HD > C::QT) named_bar_sync(1, kSoft);   // the stages: the next piece's Q goes there
             tc::fence_before();
-            e0 += (long long)(C::KE + 1) * w.nu;
-            w.step();
+            if constexpr (HD > C::QT) {
+                named_bar_sync(1, kSoft);   // every stage has been emptied
+                if (more) load_q();
+            }
         }
     }
     tc::fence_before();
