@@ -33,7 +33,7 @@ static int make_dims(const char* op, int T, int B, int nH, int nkv, int hd, int 
                      int window, Dims& d) {
     G4B_REQUIRE(T >= 1 && B >= 1 && B <= kMaxSeqs, G4B_E_SHAPE, "%s: T=%d tokens, B=%d sequences (1 to %d)", op, T, B,
                 kMaxSeqs);
-    G4B_REQUIRE(nkv >= 1 && nkv <= 65535 && nH >= nkv && nH % nkv == 0 && (hd == 128 || hd == 256 || hd == 512),
+    G4B_REQUIRE(nkv >= 1 && nkv <= 65535 && nH <= 262144 && nH >= nkv && nH % nkv == 0 && (hd == 128 || hd == 256 || hd == 512),
                 G4B_E_SHAPE, "%s: nH=%d nkv=%d hd=%d (nH a multiple of nkv, hd 128, 256 or 512)", op, nH, nkv, hd);
     G4B_REQUIRE(ps >= 16 && ps <= 1024 && (ps & (ps - 1)) == 0, G4B_E_SHAPE,
                 "%s: page_size=%d (a power of two from 16 to 1024)", op, ps);
@@ -398,79 +398,260 @@ __device__ __forceinline__ void load_n(const void* base, long long e, float (&v)
             v[4 * j] = x.x; v[4 * j + 1] = x.y; v[4 * j + 2] = x.z; v[4 * j + 3] = x.w;
         }
     } else {
-        const uint2* p = reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(base) + e);
+        const __half* p = reinterpret_cast<const __half*>(base) + e;
         #pragma unroll
-        for (int j = 0; j < N / 4; j++) {
-            const uint2 u = __ldg(p + j);
-            v[4 * j] = h_lo(u.x); v[4 * j + 1] = h_hi(u.x); v[4 * j + 2] = h_lo(u.y); v[4 * j + 3] = h_hi(u.y);
+        for (int j = 0; j < N; j += 8) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if constexpr (N >= 8) u = __ldg(reinterpret_cast<const uint4*>(p + j));
+            else *reinterpret_cast<uint2*>(&u) = __ldg(reinterpret_cast<const uint2*>(p));
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            #pragma unroll
+            for (int i = 0; i < (N < 8 ? N : 8); i++) v[j + i] = i & 1 ? h_hi(w[i / 2]) : h_lo(w[i / 2]);
         }
     }
 }
 
 template <int N>
 __device__ __forceinline__ void store_half(uint16_t* p, const float (&v)[N]) {
+    uint32_t w[N / 2];
     #pragma unroll
-    for (int j = 0; j < N / 4; j++) {
-        uint2 u;
-        u.x = pack_half2(__float2half_rn(v[4 * j]), __float2half_rn(v[4 * j + 1]));
-        u.y = pack_half2(__float2half_rn(v[4 * j + 2]), __float2half_rn(v[4 * j + 3]));
-        reinterpret_cast<uint2*>(p)[j] = u;
+    for (int j = 0; j < N / 2; j++) w[j] = pack_half2(__float2half_rn(v[2 * j]), __float2half_rn(v[2 * j + 1]));
+    if constexpr (N == 4) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+        #pragma unroll
+        for (int j = 0; j < N / 8; j++)
+            reinterpret_cast<uint4*>(p)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
     }
 }
 
-// One warp per head, the heads of a token spread over the warps of its CTAs (blockIdx.y).  Lane l holds
-// elements l * PER ..; element i's rotation partner i +- hd/2 is in lane l ^ 16.
+// Few tokens: one warp per head, a token's heads over several CTAs (blockIdx.y); latency is what counts.  Lane l holds
+// elements l * PER .. of the head; element i's rotation partner i +- hd/2 is in lane l ^ 16.
 template <int HD, bool XF32>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
     constexpr int PER = HD / 32;
     const Dims& d = a.d;
     const Hdr* h = hdr_of(a.plan);
-    if (h->sig != d.sig) {
+    const int t = blockIdx.x, lane = threadIdx.x & 31;
+    const int j = blockIdx.y * (kAppendThreads / 32) + (threadIdx.x >> 5);
+    const bool is_q = j < d.nH, is_v = j >= d.nH + d.nkv;
+    const int kv = is_v ? j - d.nH - d.nkv : j - d.nH;
+    if (j >= d.nH + 2 * d.nkv) return;
+    // the head, before it is known where it goes: that is a chain of three loads
+    float v[PER];
+    load_n<PER, XF32>(a.qkv, (long long)t * a.row_stride + lane * PER +
+                      (is_q ? (long long)j * HD : (is_v ? a.voff : a.koff) + (long long)kv * HD), v);
+    const unsigned sig = h->sig;
+    const int prefix_len = h->prefix_len;
+    const int b = __ldg(at<int>(a.plan, d.tok_seq) + t), pos = __ldg(at<int>(a.plan, d.tok_pos) + t);
+    if (sig != d.sig) {
         if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(&g_status_paged, kStatusPlan);
         return;
     }
-    const int t = blockIdx.x, lane = threadIdx.x & 31;
-    const int warps = gridDim.y * (kAppendThreads / 32), w0 = blockIdx.y * (kAppendThreads / 32) + (threadIdx.x >> 5);
-    const int b = __ldg(at<int>(a.plan, d.tok_seq) + t), pos = __ldg(at<int>(a.plan, d.tok_pos) + t);
     if (b < 0 || pos < 0) return;    // behind the last sequence; or more new tokens than its length says
-    const int own = pos - h->prefix_len;
     int slot = -1;                   // the token's row of the cache for KV head 0
-    if (own >= 0)
+    if (pos >= prefix_len) {
+        const int own = pos - prefix_len;
         slot = cache_row(__ldg(a.table + (size_t)b * d.own_pages + own / d.ps), a.num_pages, d.nkv, d.ps, 0, own);
-    float cs[PER], sn[PER];
-    load_n<PER, true>(a.cos_t, (long long)pos * HD + lane * PER, cs);
-    load_n<PER, true>(a.sin_t, (long long)pos * HD + lane * PER, sn);
-    const int heads = d.nH + 2 * d.nkv;
-    for (int j = w0; j < heads; j += warps) {
-        const bool is_q = j < d.nH, is_v = j >= d.nH + d.nkv;
-        const int kv = is_v ? j - d.nH - d.nkv : j - d.nH;
-        if (!is_q && slot < 0) continue;
-        const long long e = (long long)t * a.row_stride + lane * PER +
-                            (is_q ? (long long)j * HD : (is_v ? a.voff : a.koff) + (long long)kv * HD);
-        float v[PER];
-        load_n<PER, XF32>(a.qkv, e, v);
-        float ss = 0.f;
+    }
+    if (!is_q && slot < 0) return;
+    float ss = 0.f;
+    #pragma unroll
+    for (int i = 0; i < PER; i++) ss = fmaf(v[i], v[i], ss);
+    #pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+    const float r = rsqrtf(ss / (float)HD + kEps);
+    if (is_v) {
         #pragma unroll
-        for (int i = 0; i < PER; i++) ss = fmaf(v[i], v[i], ss);
+        for (int i = 0; i < PER; i++) v[i] *= r;
+    } else {
+        float cs[PER], sn[PER], g[PER];
+        load_n<PER, true>(a.cos_t, (long long)pos * HD + lane * PER, cs);
+        load_n<PER, true>(a.sin_t, (long long)pos * HD + lane * PER, sn);
+        load_n<PER, true>(is_q ? a.qnw : a.knw, lane * PER, g);
         #pragma unroll
-        for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-        const float r = rsqrtf(ss / (float)HD + kEps);
-        if (is_v) {
-            #pragma unroll
-            for (int i = 0; i < PER; i++) v[i] *= r;
-        } else {
-            float g[PER];
-            load_n<PER, true>(is_q ? a.qnw : a.knw, lane * PER, g);
-            #pragma unroll
-            for (int i = 0; i < PER; i++) {
-                const float n = v[i] * r * g[i];
-                const float o = __shfl_xor_sync(0xffffffffu, n, 16);
-                v[i] = n * cs[i] + (lane < 16 ? -o : o) * sn[i];
+        for (int i = 0; i < PER; i++) {
+            const float n = v[i] * r * g[i];
+            const float o = __shfl_xor_sync(0xffffffffu, n, 16);
+            v[i] = n * cs[i] + (lane < 16 ? -o : o) * sn[i];
+        }
+    }
+    uint16_t* dst = is_q ? a.q_out + (long long)t * a.q_stride + (long long)j * HD
+                         : (is_v ? a.vc : a.kc) + ((long long)slot + kv * d.ps) * HD;
+    store_half<PER>(dst + lane * PER, v);
+}
+
+// Many tokens: HBM-bound on q|k|v in and out, so the rows stream through shared memory.  A warp of each persistent
+// CTA copies a token's q, k, v and rotation rows into a ring of stages (bulk copies, 32 tokens' places looked up
+// at once), the others take the heads from there.  Lane l holds elements l * PER/2 .. of both halves of a head, so that
+// both ends of a rotation are its own.
+// head warps of a CTA, by what their registers leave room for twice per SM
+constexpr int stream_warps(int hd) { return hd == 512 ? 8 : 16; }
+
+template <int N, bool F32>
+__device__ __forceinline__ void lds_n(uint32_t at, float* v) {   // N = 2, 4, 8 elements
+    if constexpr (F32) {
+        #pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            if constexpr (N >= 4)
+                asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[j]), "=f"(v[j + 1]), "=f"(v[j + 2]),
+                             "=f"(v[j + 3]) : "r"(at + 4 * j) : "memory");
+            else
+                asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(at) : "memory");
+        }
+    } else {
+        uint32_t w[N / 2];
+        if constexpr (N == 8)
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+        else if constexpr (N == 4)
+            asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+        else
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
+        #pragma unroll
+        for (int i = 0; i < N; i++) v[i] = i & 1 ? h_hi(w[i / 2]) : h_lo(w[i / 2]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_half_n(uint16_t* p, const float* v) {
+    uint32_t w[N / 2];
+    #pragma unroll
+    for (int j = 0; j < N / 2; j++) w[j] = pack_half2(__float2half_rn(v[2 * j]), __float2half_rn(v[2 * j + 1]));
+    if constexpr (N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (N == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
+}
+
+// bytes of a stage: the heads, then the two rotation rows
+__host__ __device__ inline int stage_bytes(const Dims& d, int esz) { return (d.nH + 2 * d.nkv) * d.hd * esz + 2 * d.hd * 4; }
+
+template <int HD, bool XF32>
+__global__ void __launch_bounds__(32 * (stream_warps(HD) + 1), 2) append_stream_kernel(const AppendArgs a, int stages) {
+    constexpr int kStreamWarps = stream_warps(HD);
+    constexpr int PER = HD / 32, HP = PER / 2, ESZ = XF32 ? 4 : 2;
+    extern __shared__ __align__(128) uint8_t ring_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * 8];
+    __shared__ int s_slot[8], s_abort;
+    const Dims& d = a.d;
+    const Hdr* h = hdr_of(a.plan);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (h->sig != d.sig) {
+        if (blockIdx.x == 0 && tid == 0) atomicOr(&g_status_paged, kStatusPlan);
+        return;
+    }
+    const uint32_t ring = smem_u32(ring_raw), bar0 = smem_u32(bars);
+    const int bytes = stage_bytes(d, ESZ);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (8 + s); };
+    if (tid == 0) {
+        for (int s = 0; s < 8; s++) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), kStreamWarps);
+        }
+        fence_mbar_init();
+        s_abort = 0;
+    }
+    __syncthreads();
+    volatile int* abort = &s_abort;
+    const int lo = h->tok_lo, hi = h->tok_hi, prefix_len = h->prefix_len;   // the rows that belong to a sequence
+    const int first = lo + blockIdx.x, step = gridDim.x;
+    const int nq = d.nH * HD, nk = d.nkv * HD;
+    if (warp == kStreamWarps) {
+        int slot = -1, pos = -1, s = 0, used = 0;
+        uint32_t turn = 0;
+        bool ok = true;
+        for (int t = first, n = 0; t < hi; t += step, n++) {
+            if ((n & 31) == 0) {     // the places of this CTA's next 32 tokens
+                const long long mine = t + (long long)lane * step;
+                pos = slot = -1;
+                if (mine < hi) {
+                    const int b = __ldg(at<int>(a.plan, d.tok_seq) + mine);
+                    pos = __ldg(at<int>(a.plan, d.tok_pos) + mine);
+                    const int own = pos - prefix_len;
+                    if (b >= 0 && pos >= 0 && own >= 0)
+                        slot = cache_row(__ldg(a.table + (size_t)b * d.own_pages + own / d.ps), a.num_pages, d.nkv, d.ps, 0, own);
+                }
+            }
+            const int p = __shfl_sync(0xffffffffu, pos, n & 31), c = __shfl_sync(0xffffffffu, slot, n & 31);
+            if (used == stages) ok = __all_sync(0xffffffffu, wait_short(empty(s), turn ^ 1u, abort, &g_status_paged));
+            if (!ok) break;
+            if (lane == 0) {
+                s_slot[s] = p < 0 ? -2 : c;            // -2: no position, nothing to do; -1: its q only
+                const uint32_t dst = ring + s * bytes;
+                const char* src = reinterpret_cast<const char*>(a.qkv) + (long long)t * a.row_stride * ESZ;
+                // every stage is filled whole, so its count is always the same
+                const long long rot = (long long)max(p, 0) * HD;
+                mbar_arrive_expect_tx(full(s), bytes);
+                bulk_g2s_nohint(dst, src, nq * ESZ, full(s));
+                bulk_g2s_nohint(dst + nq * ESZ, src + (long long)a.koff * ESZ, nk * ESZ, full(s));
+                bulk_g2s_nohint(dst + (nq + nk) * ESZ, src + (long long)a.voff * ESZ, nk * ESZ, full(s));
+                bulk_g2s_nohint(dst + (nq + 2 * nk) * ESZ, a.cos_t + rot, HD * 4, full(s));
+                bulk_g2s_nohint(dst + (nq + 2 * nk) * ESZ + HD * 4, a.sin_t + rot, HD * 4, full(s));
+            }
+            __syncwarp();
+            used = max(used, s + 1);
+            if (++s == stages) {
+                s = 0;
+                turn ^= 1u;
             }
         }
-        uint16_t* dst = is_q ? a.q_out + (long long)t * a.q_stride + (long long)j * HD
-                             : (is_v ? a.vc : a.kc) + ((long long)slot + kv * d.ps) * HD;
-        store_half<PER>(dst + lane * PER, v);
+        if (*abort)                  // what is in flight lands before the CTA gives up its shared memory
+            for (int k = 0; k < used; k++) mbar_wait_drain(full(k), k < s ? turn : turn ^ 1u, &g_status_paged);
+        return;
+    }
+    const int heads = d.nH + 2 * d.nkv;
+    float gq[PER], gk[PER];          // the norm weights of this lane's elements
+    #pragma unroll
+    for (int e = 0; e < 2; e++)
+        #pragma unroll
+        for (int i = 0; i < HP; i++) {
+            gq[e * HP + i] = __ldg(a.qnw + e * (HD / 2) + lane * HP + i);
+            gk[e * HP + i] = __ldg(a.knw + e * (HD / 2) + lane * HP + i);
+        }
+    int s = 0;
+    uint32_t turn = 0;
+    for (int t = first; t < hi; t += step) {
+        if (!__all_sync(0xffffffffu, wait_short(full(s), turn, abort, &g_status_paged))) break;
+        const int slot = *(volatile int*)&s_slot[s];
+        const uint32_t base = ring + s * bytes, rot = base + (nq + 2 * nk) * ESZ;
+        float cs[PER], sn[PER];
+        #pragma unroll
+        for (int e = 0; e < 2; e++) {
+            lds_n<HP, true>(rot + (e * (HD / 2) + lane * HP) * 4, cs + e * HP);
+            lds_n<HP, true>(rot + HD * 4 + (e * (HD / 2) + lane * HP) * 4, sn + e * HP);
+        }
+        for (int j = warp; j < heads && slot > -2; j += kStreamWarps) {
+            const bool is_q = j < d.nH, is_v = j >= d.nH + d.nkv;
+            const int kv = is_v ? j - d.nH - d.nkv : j - d.nH;
+            if (!is_q && slot < 0) break;
+            float v[PER], ss = 0.f;
+            #pragma unroll
+            for (int e = 0; e < 2; e++) lds_n<HP, XF32>(base + (j * HD + e * (HD / 2) + lane * HP) * ESZ, v + e * HP);
+            #pragma unroll
+            for (int i = 0; i < PER; i++) ss = fmaf(v[i], v[i], ss);
+            #pragma unroll
+            for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+            const float r = rsqrtf(ss / (float)HD + kEps);
+            #pragma unroll
+            for (int i = 0; i < PER; i++) v[i] *= is_v ? r : r * (is_q ? gq[i] : gk[i]);
+            if (!is_v) {
+                #pragma unroll
+                for (int i = 0; i < HP; i++) {
+                    const float x = v[i], y = v[HP + i];
+                    v[i] = x * cs[i] - y * sn[i];
+                    v[HP + i] = y * cs[HP + i] + x * sn[HP + i];
+                }
+            }
+            uint16_t* dst = is_q ? a.q_out + (long long)t * a.q_stride + (long long)j * HD
+                                 : (is_v ? a.vc : a.kc) + ((long long)slot + kv * d.ps) * HD;
+            #pragma unroll
+            for (int e = 0; e < 2; e++) store_half_n<HP>(dst + e * (HD / 2) + lane * HP, v + e * HP);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(s));
+        if (++s == stages) {
+            s = 0;
+            turn ^= 1u;
+        }
     }
 }
 
@@ -1006,11 +1187,29 @@ static cudaError_t launch_few(const Args& a, const CUtensorMap& km, const CUtens
     return launch_pdl(join_kernel<HD>, dim3((unsigned)((rows + per - 1) / per)), kJoinThreads, 0, s, a);
 }
 
+template <int HD, bool XF32>
+static cudaError_t launch_append_hd(const AppendArgs& a, int sms, cudaStream_t s) {
+    const int heads = a.d.nH + 2 * a.d.nkv, per = kAppendThreads / 32;
+    const int bytes = stage_bytes(a.d, XF32 ? 4 : 2);
+    // two CTAs per SM, as many stages as their half of the shared memory holds; a token too wide for two stages takes
+    // the other kernel, as a batch of few tokens does
+    const int stages = std::min(8, 110 * 1024 / bytes);
+    if (a.d.T >= 2 * sms && stages >= 2) {
+        cudaError_t e = cudaFuncSetAttribute(append_stream_kernel<HD, XF32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             stages * bytes);
+        if (e != cudaSuccess) return e;
+        append_stream_kernel<HD, XF32><<<2 * sms, 32 * (stream_warps(HD) + 1), stages * bytes, s>>>(a, stages);
+    } else {
+        append_kernel<HD, XF32><<<dim3(a.d.T, (heads + per - 1) / per), kAppendThreads, 0, s>>>(a);
+    }
+    return cudaGetLastError();
+}
+
 template <bool XF32>
-static void launch_append(const AppendArgs& a, dim3 grid, cudaStream_t s) {
-    if (a.d.hd == 128) append_kernel<128, XF32><<<grid, kAppendThreads, 0, s>>>(a);
-    else if (a.d.hd == 256) append_kernel<256, XF32><<<grid, kAppendThreads, 0, s>>>(a);
-    else append_kernel<512, XF32><<<grid, kAppendThreads, 0, s>>>(a);
+static cudaError_t launch_append(const AppendArgs& a, int sms, cudaStream_t s) {
+    return a.d.hd == 128 ? launch_append_hd<128, XF32>(a, sms, s)
+         : a.d.hd == 256 ? launch_append_hd<256, XF32>(a, sms, s)
+                         : launch_append_hd<512, XF32>(a, sms, s);
 }
 
 }  // namespace pg
@@ -1123,14 +1322,12 @@ int g4b_paged_append(const void* qkv, int dtype, long long row_stride, const flo
     a.koff = koff;
     a.voff = voff;
     a.num_pages = num_pages;
-    st = check_device(nullptr);
+    int sms = 148;
+    st = check_device(&sms);
     if (st != G4B_OK) return st;
-    // few tokens: one head per warp; many: a token per CTA, whose warps keep the rotation for their heads
-    const int heads = nH + 2 * nkv, per = kAppendThreads / 32;
-    const int y = T >= 256 ? 1 : std::min(65535, (heads + per - 1) / per);
-    const dim3 grid(T, y);
-    if (dtype == G4B_DT_F32) launch_append<true>(a, grid, reinterpret_cast<cudaStream_t>(stream));
-    else launch_append<false>(a, grid, reinterpret_cast<cudaStream_t>(stream));
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const cudaError_t e = dtype == G4B_DT_F32 ? launch_append<true>(a, sms, s) : launch_append<false>(a, sms, s);
+    if (e != cudaSuccess) return fail(G4B_E_CUDA, "paged_append: launch: %s", cudaGetErrorString(e));
     count_launch();
     return launch_status("paged_append");
 }

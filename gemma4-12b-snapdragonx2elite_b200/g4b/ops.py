@@ -42,29 +42,32 @@ class _on:
     call allocates and launches: what it allocates is then ordered with the stream that uses it."""
     __slots__ = ("dev", "stream")
 
-    def __init__(self, device: torch.device, stream: Optional[torch.cuda.Stream]):
-        index = torch.cuda.current_device() if device.index is None else device.index
-        self.dev = torch.cuda.device(index) if index != torch.cuda.current_device() else None
+    def __init__(self, index: int, stream: Optional[torch.cuda.Stream]):
+        self.dev = torch.cuda.device(index)
         self.stream = None if stream is None else torch.cuda.stream(stream)
 
     def __enter__(self):
-        if self.dev is not None:
-            self.dev.__enter__()
+        self.dev.__enter__()
         if self.stream is not None:
             self.stream.__enter__()
 
     def __exit__(self, *exc):
         if self.stream is not None:
             self.stream.__exit__(*exc)
-        if self.dev is not None:
-            self.dev.__exit__(*exc)
+        self.dev.__exit__(*exc)
 
 
-def _rows_shape(op: str, t: torch.Tensor, name: str):
-    _need(t, name)
-    if t.dim() != 2 or t.dtype != torch.float32:
-        raise ValueError(f"{op}: {name} must be [rows, D] f32, got {tuple(t.shape)} {t.dtype}")
-    return t.shape
+def _raw_stream(index: int) -> int:
+    """The current stream of device `index` as a handle (torch.cuda.current_stream() builds an object around it)."""
+    return _RAW(index) if _RAW is not None else int(torch.cuda.current_stream(index).cuda_stream)
+
+
+_RAW = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _is(t, dtype, shape, index: int) -> bool:
+    """t is a contiguous CUDA tensor of this dtype and shape on device `index`."""
+    return t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous()
 
 
 @dataclass
@@ -632,25 +635,29 @@ def rows_normadd_i8(x: Optional[torch.Tensor], h: torch.Tensor, w: torch.Tensor,
     (A8, sa) = cast_i8(rmsnorm(h') * w), gemm_w8a8's operand.  Returns (A8 [M, D] int8, sa [M] f32).
 
     h' is written to h_out, or to h where none is given."""
-    M, D = _rows_shape("rows_normadd_i8", h, "h")
-    for t, n, shape in ((x, "x", (M, D)), (w, "w", (D,)), (w_post, "w_post", (D,)), (h_out, "h_out", (M, D)),
-                        (A8, "A8", (M, D)), (sa, "sa", (M,))):
-        if t is None:
-            continue
-        _need(t, n)
-        if t.device != h.device or tuple(t.shape) != shape:
-            raise ValueError(f"rows_normadd_i8: {n} is {tuple(t.shape)} on {t.device}, want {shape} on {h.device}")
-        want = {"x": (torch.float32, torch.float16), "A8": (torch.int8,)}.get(n, (torch.float32,))
-        if t.dtype not in want:
-            raise TypeError(f"rows_normadd_i8: {n} is {t.dtype}")
-    with _on(h.device, stream):
-        if A8 is None:
-            A8 = torch.empty((M, D), dtype=torch.int8, device=h.device)
-        if sa is None:
-            sa = torch.empty((M,), dtype=torch.float32, device=h.device)
-        if h_out is None and (x is not None or scl != 1.0):
-            h_out = h
-        L.check("g4b_rows_normadd_i8", L.load().g4b_rows_normadd_i8(
-            _ptr(x), L.DT_F32 if x is None else _DT[x.dtype], _ptr(w_post), _ptr(h), _ptr(h_out), float(scl), _ptr(w),
-            _ptr(A8), _ptr(sa), M, D, _stream_handle(stream, h.device)))
+    if h.dim() != 2:
+        raise ValueError(f"rows_normadd_i8: h must be [rows, D], got {tuple(h.shape)}")
+    M, D = shape = h.shape
+    index, f32 = h.get_device(), torch.float32
+    if not (index >= 0 and _is(h, f32, shape, index) and _is(w, f32, (D,), index)
+            and (x is None or _is(x, f32, shape, index) or _is(x, torch.float16, shape, index))
+            and (w_post is None or _is(w_post, f32, (D,), index)) and (h_out is None or _is(h_out, f32, shape, index))
+            and (A8 is None or _is(A8, torch.int8, shape, index)) and (sa is None or _is(sa, f32, (M,), index))):
+        for t, n in ((x, "x"), (h, "h"), (w, "w"), (w_post, "w_post"), (h_out, "h_out"), (A8, "A8"), (sa, "sa")):
+            if t is not None:
+                _need(t, n)
+        raise ValueError("rows_normadd_i8: x [M, D] f32 or f16, h and h_out [M, D], w and w_post [D], sa [M] f32, A8 "
+                         f"[M, D] int8, all on one device (h is {tuple(shape)} {h.dtype} on {h.device})")
+    if stream is not None or torch.cuda.current_device() != index:
+        with _on(index, stream):
+            return rows_normadd_i8(x, h, w, w_post, scl, h_out, A8, sa)
+    if A8 is None:
+        A8 = torch.empty_like(h, dtype=torch.int8)
+    if sa is None:
+        sa = h.new_empty(M)
+    if h_out is None and (x is not None or scl != 1.0):
+        h_out = h
+    L.check("g4b_rows_normadd_i8", L.load().g4b_rows_normadd_i8(
+        None if x is None else x.data_ptr(), L.DT_F32 if x is None else _DT[x.dtype], _ptr(w_post), h.data_ptr(),
+        _ptr(h_out), scl, w.data_ptr(), A8.data_ptr(), sa.data_ptr(), M, D, _raw_stream(index)))
     return A8, sa

@@ -602,7 +602,7 @@ G4B_API int g4b_gelumul(const void* gate, const void* up, int dtype, void* out, 
  *   y  = h' * rsqrt(mean(h'^2) + 1e-6) * w
  *   sa[m] = max(max_k |y[m,k]| / 127, 1e-12),  A8[m,k] = clamp(round_half_even(y[m,k] / sa[m]), -127, 127)
  * x f32 or f16; h, w_post, w f32.  h' goes to h_out, which may be h itself (in place) but not overlap it
- * otherwise; NULL: it is not stored.  The codes are formed without rounding y first, so one may differ by a
+ * otherwise; NULL: it is not stored.  x, w_post, h, h_out and w are 32-byte aligned.  The codes are formed without rounding y first, so one may differ by a
  * step from the three calls' where y / sa is next to a half.  D is a multiple of 16. */
 G4B_API int g4b_rows_normadd_i8(const void* x, int x_dtype, const float* w_post, const float* h, float* h_out, float scl,
                                 const float* w, int8_t* A8, float* sa, int M, int D, g4b_stream_t stream);

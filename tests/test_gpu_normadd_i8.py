@@ -116,7 +116,7 @@ def test_python_refusals():
         ops.rows_normadd_i8(x[:3], h, w)
     with pytest.raises(ValueError):
         ops.rows_normadd_i8(x, h[:, ::2], w)
-    with pytest.raises(TypeError):
+    with pytest.raises(ValueError):
         ops.rows_normadd_i8(x.to(torch.bfloat16), h, w)
     with pytest.raises(ValueError):
         ops.rows_normadd_i8(x, h.half(), w)

@@ -317,7 +317,7 @@ def test_python_refusals():
     plan, q = bt.plan(), bt.queries()
     with pytest.raises(ValueError):
         plan.attend(q, bt.kc, bt.vc, bt.table, prefix_table=bt.table[0])
-    with pytest.raises(TypeError):
+    with pytest.raises(ValueError):
         plan.attend(q.float(), bt.kc, bt.vc, bt.table)
     with pytest.raises(ValueError):
         plan.attend(q[:1], bt.kc, bt.vc, bt.table)

@@ -105,7 +105,13 @@ def test_normadd_i8_refusals(buf):
     assert f(p, 1, p, p, p + 64, 1.0, p, p, p, 4, 256, None) == L.G4B_E_ARG         # h_out overlaps h
     for m, d in ((0, 256), (4, 8), (4, 24), (-1, 16)):
         assert f(p, 1, p, p, p, 1.0, p, p, p, m, d, None) == L.G4B_E_SHAPE
-    assert f(p + 8, 1, p, p, p, 1.0, p, p, p, 4, 256, None) == L.G4B_E_ALIGN
+    q = (p + 31) & ~31
+    for i in (0, 2, 3, 4, 6, 7, 8):             # x, w_post, h, h_out, w, A8, sa
+        args = [q, 1, q, q, q, 1.0, q, q, q, 4, 256, None]
+        args[i] += 2 if i == 8 else 8 if i == 7 else 16
+        if i in (3, 4):
+            args[3] = args[4] = q + 16
+        assert f(*args) == L.G4B_E_ALIGN
 
 
 @pytest.fixture(scope="module")
