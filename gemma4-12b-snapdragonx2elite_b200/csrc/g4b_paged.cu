@@ -72,11 +72,11 @@ static int make_dims(const char* op, int T, int B, int nH, int nkv, int hd, int 
     };
     d.tok_seq = take((size_t)T * 4);
     d.tok_pos = take((size_t)T * 4);
-    d.row_own = take((size_t)rows * 4);
     d.row_pre = take((size_t)rows * 4);
     for (int k = 0; k < 2; k++) {
         d.start[k] = take((size_t)d.ctas[k] * sizeof(Start));
         d.tiles[k] = take((size_t)d.max_tiles[k] * sizeof(Tile));
+        d.joins[k] = take((size_t)d.max_tiles[k] * nkv * sizeof(int2));
     }
     d.bytes = o;
     d.sig = sig_of(d);
@@ -159,7 +159,7 @@ __device__ X block_scan(X v, X init, X* warp_buf, X* total, F op) {   // exclusi
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     extern __shared__ int sm[];
     __shared__ long long wbuf[kPlanThreads / 32];
-    __shared__ int ibuf[kPlanThreads / 32];
+    __shared__ int ibuf[kPlanThreads / 32], s_joins;
     const Dims& d = a.d;
     const int B = d.B, G = d.G, tid = threadIdx.x;
     int* st = sm;                    // [B + 1] first row of each sequence
@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     const bool pre_many = a.many && r_hi - r_lo > kRowsS;
     const int pre_rows = pre_many ? kRowsP : kRowsS;
     const int pre_tiles = pl > 0 ? (r_hi - r_lo + pre_rows - 1) / pre_rows : 0;
+    auto alone = [&](int b) { return (st[b + 1] - st[b]) * G > kRowsAlone; };
     auto many_of = [&](int b) { return a.many && (st[b + 1] - st[b]) * G > kRowsS; };
     // first tile of each sequence: the prefix's come first
     int nt[2] = {pre_many ? 0 : pre_tiles, pre_many ? pre_tiles : 0};
@@ -215,15 +216,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         at<int>(a.plan, d.tok_pos)[t] = pos;
     }
     for (int r = gtid; r < d.T * G; r += gn) {
-        int own = -1, pre = -1;
-        if (r >= r_lo && r < r_hi) {
-            const int b = seq_of(st, B, r / G);
-            const unsigned kind = (unsigned)base[b] & 0x80000000u;
-            own = (int)(kind | (((unsigned)base[b] & 0x7fffffffu) +
-                                (unsigned)((r - st[b] * G) / (kind ? kRowsP : kRowsS))));
-            if (pre_tiles) pre = (int)((pre_many ? 0x80000000u : 0u) | (unsigned)((r - r_lo) / pre_rows));
-        }
-        at<int>(a.plan, d.row_own)[r] = own;
+        int pre = -1;                // the row's prefix tile: kind in bit 31
+        if (pre_tiles && r >= r_lo && r < r_hi && !(a.many && alone(seq_of(st, B, r / G))))
+            pre = (int)((pre_many ? 0x80000000u : 0u) | (unsigned)((r - r_lo) / pre_rows));
         at<int>(a.plan, d.row_pre)[r] = pre;
     }
     if (blockIdx.x != 0) return;
@@ -235,18 +230,18 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         t.row0 = r_lo + i * pre_rows;
         t.nrows = min(pre_rows, r_hi - t.row0);
         t.seq = -1;
-        // the positions of its rows: within a sequence they rise
+        // the positions of the rows that have no tile of both segments: within a sequence they rise
         const int t0 = t.row0 / G, t1 = (t.row0 + t.nrows - 1) / G;
         int lo = 0x7fffffff, hi = 0;
         for (int b = seq_of(st, B, t0); b < B && st[b] <= t1; b++) {
             const int f = max(t0, st[b]), l = min(t1, st[b + 1] - 1);
-            if (l < f) continue;
+            if (l < f || (a.many && alone(b))) continue;
             lo = min(lo, first_key(len[b] - st[b + 1] + f));
             hi = max(hi, len[b] - st[b + 1] + l + 1);
         }
-        t.lo = lo / kUnit * kUnit;
-        t.hi = min(pl, hi);
-        t.n = max(0, (t.hi - t.lo + kUnit - 1) / kUnit);
+        t.lo1 = lo / kUnit * kUnit;
+        t.hi1 = min(pl, hi);
+        t.n = t.n1 = max(0, (t.hi1 - t.lo1 + kUnit - 1) / kUnit);
         at<Tile>(a.plan, d.tiles[pre_many ? 1 : 0])[i] = t;
     }
     // each sequence names its tiles (a warp per sequence: a long prompt has many)
@@ -279,11 +274,17 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
                     t.nrows = min(br, (st[b0 + 1] - st[b0]) * G - lr);
                     const int p0 = len[b0] - st[b0 + 1] + t.row0 / G;
                     const int p1 = len[b0] - st[b0 + 1] + (t.row0 + t.nrows - 1) / G;
-                    t.lo = max(0, first_key(p0) - pl) / kUnit * kUnit;
-                    t.hi = p1 + 1 - pl;
-                    t.n = max(0, (t.hi - t.lo + kUnit - 1) / kUnit);
+                    t.lo2 = max(0, first_key(p0) - pl) / kUnit * kUnit;
+                    t.hi2 = p1 + 1 - pl;
+                    t.n = max(0, (t.hi2 - t.lo2 + kUnit - 1) / kUnit);
+                    if (kind == 1 && alone(b0)) {
+                        t.lo1 = first_key(p0) / kUnit * kUnit;
+                        t.hi1 = min(pl, p1 + 1);
+                        t.n1 = max(0, (t.hi1 - t.lo1 + kUnit - 1) / kUnit);
+                        t.n += t.n1;
+                    }
                     t.solo = 1;
-                    if (pre_tiles) {
+                    if (pre_tiles && !(kind && alone(b0))) {
                         const Tile* pt = at<Tile>(a.plan, d.tiles[pre_many ? 1 : 0]);
                         for (int j = (t.row0 - r_lo) / pre_rows; j <= (t.row0 + t.nrows - 1 - r_lo) / pre_rows; j++)
                             if (pt[j].n > 0) t.solo = 0;
@@ -341,6 +342,22 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
             h->wt[kind] = run;
             h->u[kind] = u;
         }
+        // what is left to the join kernel
+        if (tid == 0) s_joins = 0;
+        __syncthreads();
+        for (int i = tid; i < nt[kind] * d.nkv; i += kPlanThreads) {
+            const Tile& t = tiles[i / d.nkv];
+            if (t.seq < 0) continue;
+            const int walks = kind ? d.cs : 1, head = i % d.nkv;
+            bool left = !(t.solo && t.n > 0);
+            for (int k = 0; k < walks && !left; k++) {
+                const Span sp = span_of((long long)(head * walks + k) * run + t.off, t.n, u);
+                left = sp.c0 != sp.c1;
+            }
+            if (left) at<int2>(a.plan, d.joins[kind])[atomicAdd(&s_joins, 1)] = make_int2(i / d.nkv, head);
+        }
+        __syncthreads();
+        if (tid == 0) h->nj[kind] = s_joins;
         for (int c = tid; c < d.ctas[kind]; c += kPlanThreads) {
             Start s{};
             s.head = -1;
@@ -525,7 +542,7 @@ __device__ __forceinline__ void store_half_n(uint16_t* p, const float* v) {
 __host__ __device__ inline int stage_bytes(const Dims& d, int esz) { return (d.nH + 2 * d.nkv) * d.hd * esz + 2 * d.hd * 4; }
 
 template <int HD, bool XF32>
-__global__ void __launch_bounds__(32 * (stream_warps(HD) + 1), 2) append_stream_kernel(const AppendArgs a, int stages) {
+__global__ void __launch_bounds__(32 * (stream_warps(HD) + 1), HD == 512 ? 1 : 2) append_stream_kernel(const AppendArgs a, int stages) {
     constexpr int kStreamWarps = stream_warps(HD);
     constexpr int PER = HD / 32, HP = PER / 2, ESZ = XF32 ? 4 : 2;
     extern __shared__ __align__(128) uint8_t ring_raw[];
@@ -760,7 +777,8 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
             continue;
         }
         const int nu = (int)min((long long)(t.n - unit), left);
-        const int key0 = t.lo + unit * kUnit, key1 = min(t.hi, key0 + nu * kUnit);
+        const Unit un0 = unit_of(t, unit);                           // a few-rows tile has one segment
+        const int key0 = un0.key, key1 = min(un0.hi, key0 + nu * kUnit);
         const int kbase = t.seq < 0 ? 0 : pl;                        // position of the segment's key 0
         const int* table = t.seq < 0 ? a.pre_table : a.table + (size_t)t.seq * d.own_pages;
         const int table_n = t.seq < 0 ? d.pre_pages : d.own_pages;
@@ -1041,88 +1059,100 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
 }
 
 // ------------------------------------------------------------------ join
-// One warp per (token, query head): out = sum_p V_p 2^(m_p - M) / sum_p l_p 2^(m_p - M) over the partials
-// of its prefix tile and its own tile.  A row whose own whole tile wrote it is left; a row with no key at
-// all becomes zeros.
-constexpr int kJoinThreads = 128;
+// out = sum_p V_p 2^(m_p - M) / sum_p l_p 2^(m_p - M) over the partials of a row's prefix tile and of its own tile, for
+// the rows that no whole tile wrote; a row with no key at all becomes zeros.  The plan lists the (tile, KV head) pairs;
+// a CTA takes eight rows of one at a time.  Where there are fewer rows than warps, several warps share a row's partials:
+// a decode token over a long prefix has twenty or so, and their loads are what takes time here.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinSubs = kRowsP / kJoinWarps;       // groups of eight rows in a many-rows tile
 
 template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
     constexpr int PER = HD / 32;
+    __shared__ float s_v[kJoinWarps][HD], s_m[kJoinWarps][32], s_l[kJoinWarps][32];
     const Dims& d = a.d;
     const Hdr* h = hdr_of(a.plan);
-    const int lane = threadIdx.x & 31;
-    const long long w = (long long)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
-    const bool mine = h->sig == d.sig && w < (long long)d.T * d.nH && w >= (long long)h->tok_lo * d.nH &&
-                      w < (long long)h->tok_hi * d.nH;
-    if (!mine) {          // not a row of any sequence: left as it was
-        pdl_wait();       // (a grid that ends is taken for the end of the one it depends on, too)
-        return;
-    }
-    const int tok = (int)(w / d.nH), hq = (int)(w % d.nH), head = hq / d.G, row = tok * d.G + hq % d.G;
-    // where the partials are: from the plan, which no kernel before this one writes
-    const float* part[2] = {nullptr, nullptr};         // of segment 0 (prefix) and 1 (own): first partial,
-    const float2* ml[2] = {nullptr, nullptr};
-    int n[2] = {0, 0}, next[2] = {0, 0}, part_width[2] = {HD, HD};   // how many; slots between the later ones; floats of a slot
-    bool done = false;
-    #pragma unroll
-    for (int seg = 0; seg < 2; seg++) {
-        const int ref = __ldg(at<int>(a.plan, seg ? d.row_own : d.row_pre) + row);
-        if (ref == -1 && seg == 0) continue;
-        const int kind = (unsigned)ref >> 31;
-        const Tile& t = at<Tile>(a.plan, d.tiles[kind])[ref & 0x7fffffff];
-        if (t.n == 0) continue;
-        // a many-rows tile of a wide head is walked once per part of the columns: this lane's is `walk`
-        const int width = kind ? HD / d.cs : HD, walk = lane * PER / width, col = lane * PER % width;
-        const Span sp = span_of(h, kind, t.off, t.n, kind ? head * d.cs + walk : head);
-        n[seg] = sp.c1 - sp.c0 + 1;
-        if (sp.c0 == sp.c1) {
-            done = t.solo;                             // written by its tile
-            const size_t slot = ((size_t)seg * d.T + tok) * d.nH + hq;
-            part[seg] = a.w.row + slot * HD + lane * PER;
-            ml[seg] = a.w.row_ml + 2 * slot + walk;
-        } else {
-            // edge slots: 1 in the tile's first CTA, 0 in the ones behind it
-            const int br = kind ? kRowsP : kRowsS;
-            const size_t slot = ((size_t)sp.c0 * 2 + 1) * br + (row - t.row0);
-            part[seg] = a.w.edge[kind] + slot * width + col;
-            ml[seg] = a.w.edge_ml[kind] + slot;
-            next[seg] = 2 * br;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n0 = h->sig == d.sig ? h->nj[0] : 0, items = n0 + (h->sig == d.sig ? h->nj[1] * kJoinSubs : 0);
+    bool waited = false;
+    for (int it = blockIdx.x; it < items; it += gridDim.x) {
+        // the plan's part first: no kernel before this one writes it
+        const int kind = it >= n0, e = kind ? (it - n0) / kJoinSubs : it, sub = kind ? (it - n0) % kJoinSubs : 0;
+        const int2 pair = at<int2>(a.plan, d.joins[kind])[e];
+        const Tile t = at<Tile>(a.plan, d.tiles[kind])[pair.x];
+        const int head = pair.y, rows = min(kJoinWarps, t.nrows - sub * kJoinWarps);
+        if (rows <= 0) continue;
+        const int share = rows > 4 ? 1 : rows > 2 ? 2 : rows > 1 ? 4 : 8;       // warps per row
+        const int r = sub * kJoinWarps + warp / share;
+        const bool busy = r < t.nrows && warp / share < rows;
+        const int row = t.row0 + min(r, t.nrows - 1), tok = row / d.G, hq = head * d.G + row % d.G;
+        // A many-rows tile of a wide head is walked once per part of the columns; this lane's part may have been cut
+        // elsewhere than another lane's.
+        const float* part[2] = {nullptr, nullptr};      // of the prefix (0) and this tile (1): the first partial's sums,
+        const float2* ml[2] = {nullptr, nullptr};       // its (maximum, sum),
+        int n[2] = {0, 0}, next[2] = {0, 0}, width[2] = {HD, HD};   // how many; slots between later ones; floats of a slot
+        bool done = false;
+        #pragma unroll
+        for (int seg = 0; seg < 2; seg++) {
+            const int ref = seg ? 0 : __ldg(at<int>(a.plan, d.row_pre) + row);
+            if (ref == -1) continue;
+            const int k = seg ? kind : (unsigned)ref >> 31;
+            const Tile& x = seg ? t : at<Tile>(a.plan, d.tiles[k])[ref & 0x7fffffff];
+            if (x.n == 0) continue;
+            width[seg] = k ? HD / d.cs : HD;
+            const int walk = lane * PER / width[seg];
+            const Span sp = span_of(h, k, x.off, x.n, k ? head * d.cs + walk : head);
+            n[seg] = sp.c1 - sp.c0 + 1;
+            if (sp.c0 == sp.c1) {
+                done = x.solo;                          // these columns are written
+                const size_t slot = ((size_t)seg * d.T + tok) * d.nH + hq;
+                part[seg] = a.w.row + slot * HD + lane * PER;
+                ml[seg] = a.w.row_ml + 2 * slot + walk;
+            } else {
+                // edge slots: 1 in the tile's first CTA, 0 in the ones behind it
+                const int br = k ? kRowsP : kRowsS;
+                const size_t slot = ((size_t)sp.c0 * 2 + 1) * br + (row - x.row0);
+                part[seg] = a.w.edge[k] + slot * width[seg] + lane * PER % width[seg];
+                ml[seg] = a.w.edge_ml[k] + slot;
+                next[seg] = 2 * br;
+            }
         }
-        part_width[seg] = width;
-    }
-    pdl_wait();
-    if (done) return;
-    float M = -INFINITY, L = 0.f, v[PER];
-    #pragma unroll
-    for (int i = 0; i < PER; i++) v[i] = 0.f;
-    #pragma unroll
-    for (int seg = 0; seg < 2; seg++) {
-        // up to four partials at once: their loads are independent, their sums are not
-        for (int k0 = 0; k0 < n[seg]; k0 += 4) {
-            float2 w2[4];
-            float x[4][PER];
+        if (!waited) pdl_wait();
+        waited = true;
+        float M = -INFINITY, L = 0.f, v[PER];
+        #pragma unroll
+        for (int i = 0; i < PER; i++) v[i] = 0.f;
+        const int total = busy && !done ? n[0] + n[1] : 0;
+        constexpr int NB = HD == 512 ? 2 : 4;           // partials at once: their loads are independent, their sums are not
+        for (int k0 = warp % share; k0 < total; k0 += NB * share) {
+            float2 w2[NB];
+            float x[NB][PER];
             #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                // slot of partial k0 + k from the first one's: -br + k 2 br behind the first
-                const long long s = k0 + k == 0 ? 0 : (long long)(k0 + k) * next[seg] - next[seg] / 2;
+            for (int k = 0; k < NB; k++) {
+                const int p = k0 + k * share;
                 w2[k] = make_float2(-INFINITY, 0.f);
-                if (k0 + k < n[seg]) {
-                    w2[k] = __ldcg(ml[seg] + s);
+                #pragma unroll
+                for (int i = 0; i < PER; i++) x[k][i] = 0.f;
+                if (p < total) {
+                    const bool own = p >= n[0];
+                    const int q = own ? p - n[0] : p;
+                    // slots from the first partial: partial q > 0 is q pairs of slots on, less one
+                    const long long s = q == 0 ? 0 : (long long)q * (own ? next[1] : next[0]) - (own ? next[1] : next[0]) / 2;
+                    w2[k] = __ldcg((own ? ml[1] : ml[0]) + s);
+                    const float* src = (own ? part[1] : part[0]) + s * (own ? width[1] : width[0]);
                     #pragma unroll
                     for (int i = 0; i < PER; i += 4) {
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(part[seg] + s * part_width[seg] + i));
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(src + i));
                         x[k][i] = y.x;
                         x[k][i + 1] = y.y;
                         x[k][i + 2] = y.z;
                         x[k][i + 3] = y.w;
                     }
-                } else {
-                    #pragma unroll
-                    for (int i = 0; i < PER; i++) x[k][i] = 0.f;
                 }
             }
-            const float mn = fmaxf(fmaxf(fmaxf(M, w2[0].x), fmaxf(w2[1].x, w2[2].x)), w2[3].x);
+            float mn = M;
+            #pragma unroll
+            for (int k = 0; k < NB; k++) mn = fmaxf(mn, w2[k].x);
             const float mu = mn == -INFINITY ? 0.f : mn;
             const float f = exp2_approx(M - mu);
             M = mn;
@@ -1130,26 +1160,47 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
             #pragma unroll
             for (int i = 0; i < PER; i++) v[i] *= f;
             #pragma unroll
-            for (int k = 0; k < 4; k++) {
+            for (int k = 0; k < NB; k++) {
                 const float g = exp2_approx(w2[k].x - mu);
                 L = fmaf(w2[k].y, g, L);
                 #pragma unroll
                 for (int i = 0; i < PER; i++) v[i] = fmaf(x[k][i], g, v[i]);
             }
         }
-    }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    const long long o = (long long)tok * a.out_stride + (long long)hq * HD + lane * PER;
-    #pragma unroll
-    for (int i = 0; i < PER; i++) v[i] *= inv;
-    if (a.out_f32) {
+        if (share > 1) {
+            // the row's warps add up; the first of them goes on
+            #pragma unroll
+            for (int i = 0; i < PER; i++) s_v[warp][lane + 32 * i] = v[i];
+            s_m[warp][lane] = M;
+            s_l[warp][lane] = L;
+            __syncthreads();
+            if (warp % share == 0) {
+                for (int k = 1; k < share; k++) {
+                    const float m2 = s_m[warp + k][lane], mn = fmaxf(M, m2), mu = mn == -INFINITY ? 0.f : mn;
+                    const float f = exp2_approx(M - mu), g = exp2_approx(m2 - mu);
+                    M = mn;
+                    L = L * f + s_l[warp + k][lane] * g;
+                    #pragma unroll
+                    for (int i = 0; i < PER; i++) v[i] = v[i] * f + s_v[warp + k][lane + 32 * i] * g;
+                }
+            }
+            __syncthreads();
+        }
+        if (!busy || done || warp % share != 0) continue;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const long long o = (long long)tok * a.out_stride + (long long)hq * HD + lane * PER;
         #pragma unroll
-        for (int i = 0; i < PER; i += 4)
-            *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o + i) =
-                make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    } else {
-        store_half<PER>(reinterpret_cast<uint16_t*>(a.out) + o, v);
+        for (int i = 0; i < PER; i++) v[i] *= inv;
+        if (a.out_f32) {
+            #pragma unroll
+            for (int i = 0; i < PER; i += 4)
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o + i) =
+                    make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        } else {
+            store_half<PER>(reinterpret_cast<uint16_t*>(a.out) + o, v);
+        }
     }
+    if (!waited) pdl_wait();    // a grid that ends is taken for the end of the one it depends on, too
 }
 
 // a launch that may begin while the kernel before it in the stream finishes
@@ -1183,8 +1234,8 @@ static cudaError_t launch_few(const Args& a, const CUtensorMap& km, const CUtens
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) return e;
-    const long long rows = (long long)a.d.T * a.d.nH, per = kJoinThreads / 32;
-    return launch_pdl(join_kernel<HD>, dim3((unsigned)((rows + per - 1) / per)), kJoinThreads, 0, s, a);
+    const long long most = ((long long)a.d.max_tiles[0] + (long long)a.d.max_tiles[1] * kJoinSubs) * a.d.nkv;
+    return launch_pdl(join_kernel<HD>, dim3((unsigned)std::min(most, 2LL * a.d.ctas[0])), kJoinThreads, 0, s, a);
 }
 
 template <int HD, bool XF32>

@@ -6,9 +6,11 @@
 // position kv_len[b] - n_b + i.  Positions below prefix_len live in the pages of one prefix table that all
 // sequences share, the others in the sequence's own table row.
 //
-// The attention of a KV head reads "segments": the prefix's keys for the rows of all sequences, and every
-// sequence's own keys for its own rows (row = token * G + query head of the group).  A segment is cut
-// into tiles of kRowsS or kRowsP rows; a tile is n units of 64 keys.  The units of all tiles and KV heads
+// The attention of a KV head is cut into tiles: rows (row = token * G + query head of the group) against keys, in
+// units of 64 keys.  A sequence with up to kRowsS rows (a decode step, a few proposed tokens) has a tile of its own keys
+// for the few-rows kernel, one with more has tiles of kRowsP rows.  Up to kRowsAlone, its rows also join those of
+// the other such sequences in tiles against the prefix; with more (a prompt's chunk) it fills tiles by itself,
+// which read the prefix and then its own keys.  The units of all tiles and KV heads
 // form one line that is cut into equal lengths, one per CTA, whatever the lengths of the sequences: a CTA
 // walks its stretch piece by piece.  Where that costs no more (few tiles, many CTAs) every tile starts at a border.  A tile that lies in one CTA's stretch is finished there; one that
 // crosses a border leaves a partial (running maximum, sum, weighted values) in the edge slots of each CTA,
@@ -24,19 +26,35 @@ namespace pg {
 constexpr int kUnit = 64;        // keys per unit of work
 constexpr int kRowsS = 8;        // rows of a tile of the few-rows kernel (the n of m16n8k16)
 constexpr int kRowsP = 128;      // rows of a tile of the many-rows kernel (tensor memory lanes)
+// A sequence of more rows than this reads the prefix in its own tiles; one of fewer shares tiles of the prefix with
+// others and has its partial results joined.  Half a tile: by itself it would use less of a tile's products than that.
+constexpr int kRowsAlone = 64;
 constexpr int kMaxSeqs = 4096;   // the plan kernel keeps the sequences in shared memory
 constexpr unsigned kStatusPlan = 2u;   // a plan made for other sizes (or never made) was passed
 
-struct Tile {
+struct __align__(16) Tile {
     int row0;        // first row: token * G + g
     int nrows;       // rows of the tile
-    int seq;         // sequence whose own keys it reads; -1: the shared prefix
-    int lo, hi;      // keys [lo, hi) of the segment; lo is a multiple of kUnit
-    int n;           // units
-    int solo;        // its rows have keys in no other segment: a whole tile writes the output itself
+    int seq;         // sequence whose own keys it reads; -1: the shared prefix alone
+    int n;           // units: first n1 of the prefix, then the sequence's own
+    int n1, lo1, hi1;   // prefix keys [lo1, hi1); lo1 is a multiple of kUnit
+    int lo2, hi2;       // own keys [lo2, hi2), counted from the prefix's end; lo2 is a multiple of kUnit
+    int solo;        // its rows have keys in no other tile: a whole tile writes the output itself
     int idle;        // units behind it that are nobody's work: they align the next tile with a stretch's start
+    int pad;
     long long off;   // units of the tiles before it, their idle ones included
+    long long pad2;
 };
+
+// unit u of a tile: its first key (in the prefix's or the sequence's own count), its segment, the segment's end
+struct Unit {
+    bool pre;
+    int key, hi;
+};
+__host__ __device__ __forceinline__ Unit unit_of(const Tile& t, int u) {
+    const bool pre = u < t.n1;
+    return {pre, pre ? t.lo1 + u * kUnit : t.lo2 + (u - t.n1) * kUnit, pre ? t.hi1 : t.hi2};
+}
 
 struct Start {       // where a CTA's stretch begins
     int head, tile, unit, pad;   // head: KV head * walks per tile + walk; -1: nothing to do
@@ -48,7 +66,7 @@ struct Hdr {
     int prefix_len;
     int tok_lo, tok_hi;              // rows of the token buffers that belong to a sequence
     int nt[2];                       // tiles: [0] few rows, [1] many rows
-    int pad[2];
+    int nj[2];                       // (tile, KV head) pairs whose rows the join kernel finishes
     long long wt[2];                 // units of one KV head
     long long u[2];                  // units per CTA
 };
@@ -59,7 +77,7 @@ struct Dims {
     int cs;                          // walks per many-rows tile: parts of hd's output columns
     int ctas[2];                     // stretches per kind
     int max_tiles[2];
-    size_t tok_seq, tok_pos, row_own, row_pre, start[2], tiles[2], bytes;
+    size_t tok_seq, tok_pos, row_pre, start[2], tiles[2], joins[2], bytes;
     unsigned sig;
 };
 

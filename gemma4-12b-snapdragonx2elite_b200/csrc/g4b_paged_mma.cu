@@ -108,7 +108,7 @@ struct Walk {
     int ntiles, head, ti, unit;   // head: KV head * CS + column part
     bool first;
     Tile t;
-    int nu, key0, key1;
+    int nu;                       // units of the piece: unit .. unit + nu - 1 of t
 
     __device__ __forceinline__ bool init(const Args& a) {
         const Hdr* h = hdr_of(a.plan);
@@ -138,8 +138,6 @@ struct Walk {
         }
         if (left <= 0) return false;
         nu = (int)min((long long)(t.n - unit), left);
-        key0 = t.lo + unit * kUnit;
-        key1 = min(t.hi, key0 + nu * kUnit);
         return true;
     }
     __device__ __forceinline__ void step() {
@@ -218,8 +216,6 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         bool ok = true;
         while (ok && w.next()) {
             const int head = w.head / C::CS, part = w.head % C::CS;
-            const int* table = w.t.seq < 0 ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
-            const int table_n = w.t.seq < 0 ? d.pre_pages : d.own_pages;
             // An entry is DV / 64 column chunks of `boxes` boxes of `box` rows.  Each lane has one box of it: one
             // instruction of the warp issues them all (one thread's loop over them took longer than the units' MMAs).
             const int box = min(d.ps, kUnit), boxes = kUnit / box, lboxes = __ffs(boxes) - 1;
@@ -227,14 +223,17 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             const bool issues = my_c < C::DV / 64;
             const uint32_t my_dst = ring + my_c * (kUnit * 128) + my_p * box * 128;
             int ids = -1, ids_at = -64;
+            bool ids_pre = false;
             // unit u of the piece: K (all of hd) or V (this walk's columns)
             auto load = [&](int u, bool is_v) {
-                const int key = w.key0 + u * kUnit;
-                const int last = (key + kUnit - 1) / d.ps;
-                if (key / d.ps < ids_at || last >= ids_at + 32) {
+                const Unit un = unit_of(w.t, w.unit + u);
+                const int key = un.key, last = (key + kUnit - 1) / d.ps;
+                if (un.pre != ids_pre || key / d.ps < ids_at || last >= ids_at + 32) {
                     // 32 page ids ahead; from the unit before on, whose V may still be to come
-                    ids_at = max(w.key0, key - kUnit) / d.ps;
-                    ids = ids_at + lane < table_n ? __ldg(table + ids_at + lane) : -1;
+                    const int* table = un.pre ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
+                    ids_pre = un.pre;
+                    ids_at = max(0, key - kUnit) / d.ps;
+                    ids = ids_at + lane < (un.pre ? d.pre_pages : d.own_pages) ? __ldg(table + ids_at + lane) : -1;
                 }
                 const int k = key + my_p * box;
                 const int id = __shfl_sync(0xffffffffu, ids, k / d.ps - ids_at);
@@ -372,8 +371,11 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             tc::fence_after();
         };
         // Q of the piece that w stands at
+        unsigned alive = 0;      // this warp's rows that the piece is for: a prefix tile may span rows that are not
         auto load_q = [&]() {
             const int row = w.t.row0 + min(r0, w.t.nrows - 1);
+            alive = __ballot_sync(0xffffffffu, r0 < w.t.nrows &&
+                                                   (w.t.seq >= 0 || __ldg(at<int>(a.plan, d.row_pre) + row) != -1));
             // Q's rows into tensor memory (two elements per column) and, past QT, shared memory.  Eight lanes read 128
             // bytes of a row; the stage turns rows over lanes into a row per lane.
             {
@@ -384,7 +386,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     for (int i = 0; i < 8; i++) {
                         const int r = 4 * i + (lane >> 3);
                         const long long o = __shfl_sync(0xffffffffu, mine, r);
-                        x[i] = wq * 32 + r < w.t.nrows ? __ldg(reinterpret_cast<const uint4*>(qb + o + c * 128))
+                        x[i] = (alive >> r) & 1u ? __ldg(reinterpret_cast<const uint4*>(qb + o + c * 128))
                                                          : make_uint4(0, 0, 0, 0);
                     }
                 };
@@ -437,14 +439,14 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             const int head = w.head / C::CS, part = w.head % C::CS;
             const int nrows = w.t.nrows, row = w.t.row0 + min(r0, nrows - 1);
             const int tok = row / G, hq = head * G + row % G;
-            const int kbase = w.t.seq < 0 ? 0 : pl;
-            const int* table = w.t.seq < 0 ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
-            const int table_n = w.t.seq < 0 ? d.pre_pages : d.own_pages;
+            const unsigned mask = alive;
+            const bool live = (mask >> lane) & 1u;
+            // the positions that this row sees, [vlo, vhi)
             const int pos = __ldg(at<int>(a.plan, d.tok_pos) + tok);
-            const int vhi = min(w.key1, pos + 1 - kbase), vlo = d.window > 0 ? max(0, pos + 1 - d.window - kbase) : 0;
-            // keys that all rows see, keys that any row sees
-            int all_lo = __reduce_max_sync(0xffffffffu, vlo), all_hi = __reduce_min_sync(0xffffffffu, vhi);
-            int any_lo = __reduce_min_sync(0xffffffffu, vlo), any_hi = __reduce_max_sync(0xffffffffu, vhi);
+            const int vhi = live ? pos + 1 : 0, vlo = live && d.window > 0 ? max(0, pos + 1 - d.window) : 0;
+            // what all rows see, what any row sees
+            int all_lo = __reduce_max_sync(0xffffffffu, vlo), all_hi = __reduce_min_sync(0xffffffffu, live ? vhi : 0x7fffffff);
+            int any_lo = __reduce_min_sync(0xffffffffu, live ? vlo : 0x7fffffff), any_hi = __reduce_max_sync(0xffffffffu, vhi);
             named_bar_sync(1, kSoft);             // the piece before has been read out of sm.red
             if (lane == 0 && half == 0) {
                 sm.red[wq][0] = all_lo;
@@ -463,16 +465,20 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             // page ids of a unit, one per box, in the first lanes; fetched a unit ahead
             const int box = min(d.ps, kUnit), boxes = kUnit / box;
             auto page_of = [&](int u) {
-                const int k = w.key0 + u * kUnit + (lane & 3) * box, idx = k / d.ps;
-                return lane < boxes && u < w.nu && idx < table_n ? __ldg(table + idx) : -1;
+                if (u >= w.nu) return -1;
+                const Unit un = unit_of(w.t, w.unit + u);
+                const int idx = (un.key + (lane & 3) * box) / d.ps;
+                const int* table = un.pre ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
+                return lane < boxes && idx < (un.pre ? d.pre_pages : d.own_pages) ? __ldg(table + idx) : -1;
             };
             int page = page_of(0);
             float m = -INFINITY, l = 0.f;
             for (int u = 0; u < w.nu; u++, it++) {
-                const int key = w.key0 + u * kUnit;
+                const Unit un = unit_of(w.t, w.unit + u);
+                const int key = un.pre ? un.key : un.key + pl, end = un.pre ? un.hi : un.hi + pl;   // as positions
                 const unsigned there = __ballot_sync(0xffffffffu, lane < boxes && page >= 0 && page < a.num_pages);
                 page = page_of(u + 1);
-                const bool edge = there != (1u << boxes) - 1 || key < all_lo || key + kUnit > all_hi;
+                const bool edge = there != (1u << boxes) - 1 || key < all_lo || key + kUnit > min(all_hi, end);
                 wait(b_s + 8u * (it & 1u), (it >> 1) & 1u);
                 if (it >= 2) wait_pv(it - 2);
                 tc::fence_after();
@@ -483,7 +489,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 if (edge) {
                     // the keys that this row sees, one bit each
                     auto below = [&](int k) { return k >= kUnit ? ~0ull : k <= 0 ? 0ull : (1ull << k) - 1; };
-                    unsigned long long bits = below(vhi - key) & ~below(vlo - key);
+                    unsigned long long bits = below(min(vhi, end) - key) & ~below(vlo - key);
                     if (there != (1u << boxes) - 1)
                         for (int b = 0; b < boxes; b++)
                             if (!((there >> b) & 1u)) bits &= ~(below((b + 1) * box) & ~below(b * box));
@@ -550,7 +556,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     #pragma unroll
                     for (int r = 0; r < 2; r++) {
                         const int k = key + (tid >> 3) + 32 * r;
-                        const bool none = k < any_lo || k >= any_hi;
+                        const bool none = k < any_lo || k >= min(any_hi, end);
                         some[r] = !none && (k < all_lo || k >= all_hi);
                         #pragma unroll
                         for (int c = 0; c < C::DV / 64; c++) {
@@ -597,7 +603,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                             const uint32_t pj = ld_tmem_x1(ts + j / 2);
                             tc::wait_ld();
                             const float pf = j & 1 ? h_hi(pj) : h_lo(pj);
-                            const bool sees = key + j >= vlo && key + j < vhi && ((there >> (j / box)) & 1u);
+                            const bool sees = key + j >= vlo && key + j < min(vhi, end) && ((there >> (j / box)) & 1u);
                             #pragma unroll 1
                             for (int c = half * DH; c < (half + 1) * DH; c += 32) {
                                 uint32_t o[32];
@@ -630,7 +636,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                                 if ((odd >> ((tid >> 3) + 32 * r)) & 1ull)
                                     st_shared(vt + c * (kUnit * 128) + r * (32 * 128), make_uint4(0, 0, 0, 0));
                     }
-                    if (odd || key < any_lo || key + kUnit > any_hi) tc::fence_proxy_async_smem();   // V was written
+                    if (odd || key < any_lo || key + kUnit > min(any_hi, end)) tc::fence_proxy_async_smem();   // V was written
                 }
                 tc::wait_st();
                 tc::fence_before();
@@ -656,7 +662,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             l += sm.top[it & 1][half ^ 1][r0];
             pair_sync();
             const float inv = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            if (r0 < nrows && ok && !direct && half == 0)
+            if (live && ok && !direct && half == 0)
                 *(whole ? a.w.row_ml + slot * 2 + part : a.w.edge_ml[1] + slot) = make_float2(m, l);
             // 128 bytes of every row of the warp, from a row per lane to eight lanes per row
             auto flush = [&](const uint32_t (&v)[32], size_t off) {
@@ -670,7 +676,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     const int r = 4 * i + (lane >> 3);
                     const uint4 x = ld_shared(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
                     const size_t o = __shfl_sync(0xffffffffu, mine, r) + off;
-                    if (ok && wq * 32 + r < nrows) *reinterpret_cast<uint4*>(dst + o + (lane & 7) * 16) = x;
+                    if (ok && (mask >> r) & 1u) *reinterpret_cast<uint4*>(dst + o + (lane & 7) * 16) = x;
                 }
                 __syncwarp();
             };
