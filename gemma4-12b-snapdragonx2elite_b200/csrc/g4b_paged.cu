@@ -56,6 +56,7 @@ static int make_dims(const char* op, int T, int B, int nH, int nkv, int hd, int 
     d.own_pages = own_pages;
     d.pre_pages = pre_pages;
     d.window = window;
+    while ((1 << d.lps) < ps) d.lps++;
     d.cs = hd == 512 ? 2 : 1;
     d.ctas[0] = sms * few_per_sm(hd);
     d.ctas[1] = sms;
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     int slot = -1;                   // the token's row of the cache for KV head 0
     if (pos >= prefix_len) {
         const int own = pos - prefix_len;
-        slot = cache_row(__ldg(a.table + (size_t)b * d.own_pages + own / d.ps), a.num_pages, d.nkv, d.ps, 0, own);
+        slot = cache_row(__ldg(a.table + (size_t)b * d.own_pages + (own >> d.lps)), a.num_pages, d.nkv, d.lps, 0, own);
     }
     if (!is_q && slot < 0) return;
     float ss = 0.f;
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(32 * (stream_warps(HD) + 1), HD == 512 ? 1 : 2
                     pos = __ldg(at<int>(a.plan, d.tok_pos) + mine);
                     const int own = pos - prefix_len;
                     if (b >= 0 && pos >= 0 && own >= 0)
-                        slot = cache_row(__ldg(a.table + (size_t)b * d.own_pages + own / d.ps), a.num_pages, d.nkv, d.ps, 0, own);
+                        slot = cache_row(__ldg(a.table + (size_t)b * d.own_pages + (own >> d.lps)), a.num_pages, d.nkv, d.lps, 0, own);
                 }
             }
             const int p = __shfl_sync(0xffffffffu, pos, n & 31), c = __shfl_sync(0xffffffffu, slot, n & 31);
@@ -827,12 +828,12 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
             if (n >= ids_at + 32) {
                 ids_at = n;
                 const int key = key0 + kBlk * (warp + kFewWarps * (n + lane));
-                const int page = key / d.ps;
+                const int page = key >> d.lps;
                 ids = key < key1 && page < table_n ? __ldg(table + page) : -1;
             }
             const int key = key0 + kBlk * (warp + kFewWarps * n);
             const int page = __shfl_sync(0xffffffffu, ids, n - ids_at);
-            const int at_row = cache_row(page, a.num_pages, d.nkv, d.ps, head, key);
+            const int at_row = cache_row(page, a.num_pages, d.nkv, d.lps, head, key);
             const bool ok = at_row >= 0;
             if (!(e & 1)) valid = (valid & ~(1u << (n & 31))) | ((ok ? 1u : 0u) << (n & 31));
             // a page that is not there: past the map's last row, which TMA fills with zeros

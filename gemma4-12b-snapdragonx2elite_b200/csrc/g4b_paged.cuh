@@ -74,6 +74,7 @@ struct Hdr {
 // sizes fixed on the host, and the offsets of the arrays in the plan buffer that follow from them
 struct Dims {
     int T, B, nH, nkv, G, hd, ps, own_pages, pre_pages, window;
+    int lps;                         // log2 of the page size
     int cs;                          // walks per many-rows tile: parts of hd's output columns
     int ctas[2];                     // stretches per kind
     int max_tiles[2];

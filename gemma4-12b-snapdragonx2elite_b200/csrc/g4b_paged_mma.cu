@@ -6,15 +6,17 @@
 //   S [128 x 64] = Q K^T      (tcgen05, Q in tensor memory, K from shared memory)
 //   P = 2^(S scale - m)       (two threads per row: a row's maximum takes one exchange through shared memory)
 //   O [128 x hd] += P V       (tcgen05, P in tensor memory over S's columns, V from shared memory)
-// S is double buffered, so the tensor core makes unit i + 1's scores while the softmax warps work on unit i.
+// S is double buffered and P has columns of its own, so the tensor core makes the scores two units ahead: a buffer is
+// free as soon as its scores have been read, and the softmax warps find the next ones ready.  (With P over S, the scores of
+// unit i + 1 waited for the product of unit i - 1: 1.2 us a unit at hd 256 where the MMAs take 0.55.)
 // m is a base, 2^4 under the maximum seen when it was set: O is rescaled only where a row's weights would pass
 // 2^15, the last power of two of f16 (a larger weight's relative rounding is the same; the 2^4 keep weights down
 // to 2^-18 of the maximum out of f16's subnormals).
 // K and V units come by TMA through one ring of 64-key buffers, issued ahead across pieces.
 //
 // Warps: 0-7 softmax, the mask, the rows' Q and the result; 8 TMA; 9 MMA issue.
-// At hd 512 the 512 output columns of O would fill tensor memory, so a tile is walked once for each half of
-// them (the scores are made twice), and half of Q stays in shared memory.
+// Tensor memory's 512 columns: O 256, S 128, P 32 and the first 192 elements of Q; its others are in shared memory.  At hd
+// 512 O alone would fill them, so a tile is walked once for each half of the output columns (the scores are made twice).
 //
 // The weights P are rounded to f16, the type of V, as the tensor core needs one type for both: 2^-11 of each
 // weight, unbiased; sums and maxima are f32.
@@ -35,21 +37,25 @@ template <int HD>
 struct ManyCfg {
     static constexpr int DV = HD < 256 ? HD : 256;      // output columns of a walk
     static constexpr int CS = HD / DV;                  // walks per tile
-    static constexpr int QT = DV;                       // elements of Q in tensor memory; the rest in shared memory
-    static constexpr int KE = HD / QT;                  // ring entries per unit of K
+    static constexpr int QT = HD == 128 ? 128 : 192;    // elements of Q in tensor memory; the rest in shared memory
+    static constexpr int KE = HD / DV;                  // ring entries per unit of K
     static constexpr int ENTRY = kUnit * DV * 2;        // bytes of a ring entry: 64 keys x DV elements
     static constexpr int QS_BYTES = kRowsP * (HD - QT) * 2;
     // a warp's 32 rows x 128 bytes on their way between rows in memory and rows in lanes; at hd 512 they lie in
-    // the shared half of Q, which is idle then
+    // the shared part of Q, which is idle then
     static constexpr int STAGE = 32 * 128;
-    static constexpr int NST = HD == 128 ? 12 : HD == 256 ? 6 : 5;
-    static constexpr int BUF = NST * ENTRY + (QS_BYTES ? QS_BYTES : 8 * STAGE);
-    static constexpr int O_COL = 0, S_COL = DV, Q_COL = DV + 2 * kUnit;
+    static constexpr bool STAGE_IN_Q = HD == 512;
+    static constexpr int NST = HD == 128 ? 10 : HD == 256 ? 5 : 4;
+    static constexpr int BUF = NST * ENTRY + QS_BYTES + (STAGE_IN_Q ? 0 : 8 * STAGE);
+    static constexpr int O_COL = 0, S_COL = DV, P_COL = S_COL + 2 * kUnit, Q_COL = P_COL + kUnit / 2;
     static_assert(Q_COL + QT / 2 <= 512, "tensor memory columns");
+    // (the stages are the last two 64-element chunks of Q's shared part, which are written last)
+    static_assert(!STAGE_IN_Q || (QS_BYTES >= 8 * STAGE && 8 * STAGE == 2 * kRowsP * 128), "the stages fit");
+    static_assert(KE * 2 <= NST, "the scores of two units need nothing but K");
     // Everything else that is shared, behind the buffers: no static shared memory, so that the buffers begin where the
     // CTA's window does, at a multiple of 1024 (the kernel checks).
     struct Small {
-        uint64_t bars[2 * NST + 8];
+        uint64_t bars[2 * NST + 10];
         unsigned long long odd;            // keys of the unit with a value that is not finite
         float top[2][2][kRowsP];           // [unit % 2][half][row]
         int red[4][4];
@@ -58,7 +64,6 @@ struct ManyCfg {
     };
     static constexpr int SMEM = BUF + (int)sizeof(Small);
     static_assert(SMEM <= 227 * 1024, "shared memory");
-    static_assert(KE * 2 + 1 <= NST, "the units issued before the first release");
 };
 
 namespace {
@@ -175,24 +180,26 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         if (tid == 0) atomicOr(&g_status_paged_mma, kStatusTimeout);
         return;
     }
-    const uint32_t qs = ring + C::NST * C::ENTRY;                    // hd 512: the second half of Q; else the stages
+    const uint32_t qs = ring + C::NST * C::ENTRY;                    // the part of Q that is not in tensor memory
+    const uint32_t stages = qs + (C::STAGE_IN_Q ? C::QS_BYTES - 8 * C::STAGE : C::QS_BYTES);
     const uint32_t bar0 = smem_u32(sm.bars);
     auto full = [&](int s) { return bar0 + 8u * s; };
     auto empty = [&](int s) { return bar0 + 8u * (C::NST + s); };
     const uint32_t b_s = bar0 + 8u * (2 * C::NST);                   // [2] scores of a unit are there
-    const uint32_t b_p = b_s + 16;                                   // [2] its weights are there
-    const uint32_t b_pv = b_s + 32;                                  // [2] its product is added
+    const uint32_t b_read = b_s + 16;                                // [2] and have been read
+    const uint32_t b_p = b_s + 32;                                   // its weights are there
+    const uint32_t b_pv = b_s + 40;                                  // its product is added
     const uint32_t b_q = b_s + 48;                                   // the piece's Q is there
     const uint32_t b_drain = b_s + 56;
     if (tid == 0) {
         for (int i = 0; i < 2 * C::NST; i++) mbar_init(bar0 + 8u * i, 1);
         mbar_init(b_s, 1);
         mbar_init(b_s + 8, 1);
-        mbar_init(b_p, kSoft);
-        mbar_init(b_p + 8, kSoft);
+        mbar_init(b_read, kSoft / 32);
+        mbar_init(b_read + 8, kSoft / 32);
+        mbar_init(b_p, kSoft / 32);
         mbar_init(b_pv, 1);
-        mbar_init(b_pv + 8, 1);
-        mbar_init(b_q, kSoft);
+        mbar_init(b_q, kSoft / 32);
         mbar_init(b_drain, 1);
         fence_mbar_init();
         sm.abort = 0;
@@ -227,17 +234,17 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             // unit u of the piece: K (all of hd) or V (this walk's columns)
             auto load = [&](int u, bool is_v) {
                 const Unit un = unit_of(w.t, w.unit + u);
-                const int key = un.key, last = (key + kUnit - 1) / d.ps;
-                if (un.pre != ids_pre || key / d.ps < ids_at || last >= ids_at + 32) {
-                    // 32 page ids ahead; from the unit before on, whose V may still be to come
+                const int key = un.key, last = (key + kUnit - 1) >> d.lps;
+                if (un.pre != ids_pre || (key >> d.lps) < ids_at || last >= ids_at + 32) {
+                    // 32 page ids ahead; from two units before on, whose V may still be to come
                     const int* table = un.pre ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
                     ids_pre = un.pre;
-                    ids_at = max(0, key - kUnit) / d.ps;
+                    ids_at = max(0, key - 2 * kUnit) >> d.lps;
                     ids = ids_at + lane < (un.pre ? d.pre_pages : d.own_pages) ? __ldg(table + ids_at + lane) : -1;
                 }
                 const int k = key + my_p * box;
-                const int id = __shfl_sync(0xffffffffu, ids, k / d.ps - ids_at);
-                const int at_row = cache_row(id, a.num_pages, d.nkv, d.ps, head, k);
+                const int id = __shfl_sync(0xffffffffu, ids, (k >> d.lps) - ids_at);
+                const int at_row = cache_row(id, a.num_pages, d.nkv, d.lps, head, k);
                 const int row = at_row < 0 ? a.num_pages * d.nkv * d.ps : at_row;   // past the map: zeros
                 for (int part_e = 0; part_e < (is_v ? 1 : C::KE); part_e++) {
                     const int s = slot;
@@ -257,10 +264,12 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     }
                 }
             };
-            load(0, false);
-            for (int u = 0; u < w.nu && ok; u++) {
-                if (u + 1 < w.nu) load(u + 1, false);
-                if (ok) load(u, true);
+            // in the order of the MMAs: K runs two units ahead of V
+            #pragma unroll 1
+            for (int i = 0; i < 2 * (w.nu + 2) && ok; i++) {
+                const bool is_v = i & 1;
+                const int u = (i >> 1) - (is_v ? 2 : 0);
+                if (u >= 0 && u < w.nu) load(u, is_v);
             }
             w.step();
         }
@@ -294,7 +303,8 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         // entry's tiles are its first one's plus a constant.
         const uint64_t k_desc = tc::sdesc_sw128(ring, 16, 1024), v_desc = tc::sdesc_sw128(ring, kUnit * 128, 1024);
         const uint64_t q_desc = tc::sdesc_sw128(qs, 16, 1024);
-        auto scores = [&](uint32_t i) {
+        auto scores = [&](uint32_t i) {            // i: units before this one, all pieces'
+            if (i >= 2) wait(b_read + 8u * (i & 1u), ((i >> 1) - 1) & 1u);     // its buffer's last scores have been read
             const uint32_t ds = tmem + C::S_COL + (i & 1u) * kUnit;
             #pragma unroll
             for (int pe = 0; pe < C::KE; pe++) {
@@ -303,12 +313,14 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 const uint64_t kd = k_desc + (uint64_t)(s * (C::ENTRY / 16));
                 if (elect_one()) {
                     #pragma unroll
-                    for (int k = 0; k < C::QT / 16; k++) {
+                    for (int k = 0; k < C::DV / 16; k++) {
+                        const int e = pe * C::DV + 16 * k;                     // element of the head
                         const uint64_t bd = kd + (uint64_t)((k / 4) * (kUnit * 128 / 16) + (k % 4) * 2);
-                        if (pe == 0)
-                            tc::mma_f16_ts(ds, tmem + C::Q_COL + 8 * k, bd, id_s, k > 0);
+                        if (e < C::QT)
+                            tc::mma_f16_ts(ds, tmem + C::Q_COL + e / 2, bd, id_s, e > 0);
                         else
-                            tc::mma_f16_ss(ds, q_desc + (uint64_t)((k / 4) * (kRowsP * 128 / 16) + (k % 4) * 2), bd, id_s, 1);
+                            tc::mma_f16_ss(ds, q_desc + (uint64_t)(((e - C::QT) / 64) * (kRowsP * 128 / 16) + (k % 4) * 2), bd,
+                                           id_s, 1);
                     }
                     tc::commit(empty(s));
                     if (pe == C::KE - 1) tc::commit(b_s + 8u * (i & 1u));
@@ -319,10 +331,13 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         while (ok && w.next()) {
             wait(b_q, piece & 1u);
             piece++;
-            if (ok) scores(it);
-            for (int u = 0; ok && u < w.nu; u++) {
-                if (u + 1 < w.nu) scores(it + 1);
-                wait(b_p + 8u * (it & 1u), (it >> 1) & 1u);
+            // two units of scores ahead of the products: their buffers are free as soon as they have been read
+            #pragma unroll 1
+            for (int j = 0; ok && j < w.nu + 2; j++) {
+                if (j < w.nu) scores(it + j);
+                if (j < 2) continue;
+                const int u = j - 2;
+                wait(b_p, (it + u) & 1u);
                 const int s = entry();
                 if (!ok) break;
                 const int acc = u > 0 || *(volatile int*)&sm.acc;
@@ -330,14 +345,14 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 if (elect_one()) {
                     #pragma unroll
                     for (int k = 0; k < kUnit / 16; k++)      // 16 keys: two groups of 8 rows of 128 bytes
-                        tc::mma_f16_ts(tmem + C::O_COL, tmem + C::S_COL + (it & 1u) * kUnit + 8 * k,
-                                       vd + (uint64_t)(k * (2048 / 16)), id_o, acc || k > 0);
+                        tc::mma_f16_ts(tmem + C::O_COL, tmem + C::P_COL + 8 * k, vd + (uint64_t)(k * (2048 / 16)), id_o,
+                                       acc || k > 0);
                     tc::commit(empty(s));
-                    tc::commit(b_pv + 8u * (it & 1u));
+                    tc::commit(b_pv);
                 }
                 __syncwarp();
-                it++;
             }
+            it += w.nu;
             w.step();
         }
         if (*abort) {
@@ -355,7 +370,12 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         constexpr int DH = C::DV / 2;                                // this half's columns of O
         const uint32_t to = tl + C::O_COL + half * DH;
         auto pair_sync = [&]() { named_bar_sync(2 + wq, 64); };
-        const uint32_t stage = qs + warp * C::STAGE;
+        // one arrival per warp: 32 lanes' on one barrier would come one after the other
+        auto arrive = [&](uint32_t bar) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        const uint32_t stage = stages + warp * C::STAGE;
         uint32_t it = 0;                          // units so far
         long long e0 = 0;                         // ring entries of the pieces before
         // A wait that ran out clears ok.  The warp then walks on without waiting, so that the warps meet at
@@ -364,10 +384,10 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         auto wait = [&](uint32_t bar, uint32_t parity) {
             ok = __all_sync(0xffffffffu, ok && wait_short(bar, parity, abort, status));
         };
-        // The product of a unit is added.  A parity tells a barrier's last two phases apart only: units alternate
-        // between two barriers, and every unit u waits for unit u - 2's, so neither runs ahead unseen.
+        // The product of a unit is added.  A parity tells a barrier's last two phases apart only: every unit waits for
+        // the one before it, once.
         auto wait_pv = [&](uint32_t unit) {
-            wait(b_pv + 8u * (unit & 1u), (unit >> 1) & 1u);
+            wait(b_pv, unit & 1u);
             tc::fence_after();
         };
         // Q of the piece that w stands at
@@ -381,65 +401,114 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             {
                 const long long mine = ((long long)(row / G) * a.q_stride + (long long)((w.head / C::CS) * G + row % G) * HD) * 2;
                 const char* qb = reinterpret_cast<const char*>(a.q) + (lane & 7) * 16;
-                auto fetch = [&](int c, uint4 (&x)[8]) {       // chunk c: 64 elements of rows 4 i + lane / 8
+                // chunk c: 64 elements.  A loop that stays one: code that runs once comes from memory as slowly as data
+                // does, and two chunks' loads at once cost more in instructions than they hid.
+                constexpr int NC = HD / 128;                   // chunks of this half
+                #pragma unroll 1
+                for (int n = 0; n < NC; n++) {
+                    const int c = C::STAGE_IN_Q ? half + 2 * n : half * NC + n;
+                    // (at hd 512 the chunks from the third on may go where the stages are: those are done with then)
+                    if (C::STAGE_IN_Q && n == 2) named_bar_sync(1, kSoft);
+                    uint4 x[8];
                     #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const int r = 4 * i + (lane >> 3);
+                        const int r = 4 * i + (lane >> 3);     // of the warp's rows
                         const long long o = __shfl_sync(0xffffffffu, mine, r);
                         x[i] = (alive >> r) & 1u ? __ldg(reinterpret_cast<const uint4*>(qb + o + c * 128))
-                                                         : make_uint4(0, 0, 0, 0);
+                                                 : make_uint4(0, 0, 0, 0);
                     }
-                };
-                constexpr int CH = C::QT / 128;                // chunks of this half
-                uint4 x[CH][8];
-                #pragma unroll
-                for (int c = 0; c < CH; c++) fetch(half * CH + c, x[c]);
-                #pragma unroll
-                for (int c = 0; c < CH; c++) {
+                    const bool in_tmem = c < C::QT / 64;
+                    const uint32_t to_row = in_tmem ? stage : qs + (c - C::QT / 64) * (kRowsP * 128) + wq * (32 * 128);
                     #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int r = 4 * i + (lane >> 3);
-                        st_shared(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4), x[c][i]);
+                        st_shared(to_row + r * 128 + (((lane & 7) ^ (r & 7)) << 4), x[i]);
                     }
                     __syncwarp();
-                    uint32_t v[32];
-                    #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const uint4 y = ld_shared(stage + lane * 128 + ((j ^ (lane & 7)) << 4));
-                        v[4 * j] = y.x;
-                        v[4 * j + 1] = y.y;
-                        v[4 * j + 2] = y.z;
-                        v[4 * j + 3] = y.w;
-                    }
-                    tc::st_32x32b_x32(tl + C::Q_COL + 32 * (half * CH + c), v);
-                    __syncwarp();
-                }
-                if constexpr (HD > C::QT) {
-                    constexpr int CR = (HD - C::QT) / 128;
-                    #pragma unroll
-                    for (int c = 0; c < CR; c++) fetch(C::QT / 64 + half * CR + c, x[c]);
-                    named_bar_sync(1, kSoft);   // the stages lie where the rest of Q goes
-                    #pragma unroll
-                    for (int c = 0; c < CR; c++)
+                    if (in_tmem) {
+                        uint32_t v[32];
                         #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const int r = wq * 32 + 4 * i + (lane >> 3);
-                            st_shared(qs + (half * CR + c) * (kRowsP * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4), x[c][i]);
+                        for (int j = 0; j < 8; j++) {
+                            const uint4 y = ld_shared(stage + lane * 128 + ((j ^ (lane & 7)) << 4));
+                            v[4 * j] = y.x;
+                            v[4 * j + 1] = y.y;
+                            v[4 * j + 2] = y.z;
+                            v[4 * j + 3] = y.w;
                         }
-                    tc::fence_proxy_async_smem();
+                        tc::st_32x32b_x32(tl + C::Q_COL + 32 * c, v);
+                        __syncwarp();
+                    }
                 }
+                if constexpr (HD > C::QT) tc::fence_proxy_async_smem();
                 tc::wait_st();
                 tc::fence_before();
-                mbar_arrive(b_q);
+                arrive(b_q);
             }
         };
-        bool more = w.next();
-        if (more) load_q();
-        while (more) {
-            const int head = w.head / C::CS, part = w.head % C::CS;
-            const int nrows = w.t.nrows, row = w.t.row0 + min(r0, nrows - 1);
-            const int tok = row / G, hq = head * G + row % G;
-            const unsigned mask = alive;
+        // A piece's result is written after the next piece's Q has been loaded (its scores are made meanwhile), except
+        // at hd 512, where the stages lie in Q's place.
+        bool more = w.next(), pending = false;
+        float m = -INFINITY, l = 0.f;
+        unsigned mask = 0;                        // the pending result's rows,
+        char* dst = nullptr;                      // where they go,
+        size_t mine = 0;                          // this row's offset there,
+        float2* ml = nullptr;                     // its (base, sum), null where the result is finished here,
+        int esize = 4;                            // the bytes of an element
+        for (;;) {
+            if (!C::STAGE_IN_Q && more) load_q();
+            if (pending) {
+                wait_pv(it - 1);
+                sm.top[it & 1][half][r0] = l;
+                pair_sync();
+                l += sm.top[it & 1][half ^ 1][r0];
+                pair_sync();
+                const float inv = ml ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                if (((mask >> lane) & 1u) && ok && ml && half == 0) *ml = make_float2(m, l);
+                // 128 bytes of every row of the warp, from a row per lane to eight lanes per row
+                const int per = 128 / esize;      // columns
+                #pragma unroll 1
+                for (int c = half * DH; c < (half + 1) * DH; c += per) {
+                    uint32_t v[32];
+                    tc::ld_32x32b_x32(tl + C::O_COL + c, v);
+                    tc::wait_ld();
+                    #pragma unroll
+                    for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * inv);
+                    if (esize == 2) {
+                        uint32_t y[32];
+                        tc::ld_32x32b_x32(tl + C::O_COL + c + 32, y);
+                        tc::wait_ld();
+                        #pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            v[j] = pack_half2(__float2half_rn(__uint_as_float(v[2 * j])),
+                                              __float2half_rn(__uint_as_float(v[2 * j + 1])));
+                            y[j] = pack_half2(__float2half_rn(__uint_as_float(y[2 * j]) * inv),
+                                              __float2half_rn(__uint_as_float(y[2 * j + 1]) * inv));
+                        }
+                        #pragma unroll
+                        for (int j = 0; j < 16; j++) v[16 + j] = y[j];
+                    }
+                    #pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        st_shared(stage + lane * 128 + ((j ^ (lane & 7)) << 4),
+                                  make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                    __syncwarp();
+                    #pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int r = 4 * i + (lane >> 3);
+                        const uint4 x = ld_shared(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                        const size_t o = __shfl_sync(0xffffffffu, mine, r) + (size_t)c * esize;
+                        if (ok && (mask >> r) & 1u) *reinterpret_cast<uint4*>(dst + o + (lane & 7) * 16) = x;
+                    }
+                    __syncwarp();
+                }
+                tc::fence_before();
+                if (C::STAGE_IN_Q) named_bar_sync(1, kSoft);   // every stage has been emptied
+            }
+            if (C::STAGE_IN_Q && more) load_q();
+            if (!more) break;
+            const int part = w.head % C::CS, nrows = w.t.nrows, row = w.t.row0 + min(r0, nrows - 1);
+            const int tok = row / G, hq = (w.head / C::CS) * G + row % G;
+            mask = alive;
             const bool live = (mask >> lane) & 1u;
             // the positions that this row sees, [vlo, vhi)
             const int pos = __ldg(at<int>(a.plan, d.tok_pos) + tok);
@@ -467,12 +536,13 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             auto page_of = [&](int u) {
                 if (u >= w.nu) return -1;
                 const Unit un = unit_of(w.t, w.unit + u);
-                const int idx = (un.key + (lane & 3) * box) / d.ps;
+                const int idx = (un.key + (lane & 3) * box) >> d.lps;
                 const int* table = un.pre ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
                 return lane < boxes && idx < (un.pre ? d.pre_pages : d.own_pages) ? __ldg(table + idx) : -1;
             };
             int page = page_of(0);
-            float m = -INFINITY, l = 0.f;
+            m = -INFINITY;
+            l = 0.f;
             for (int u = 0; u < w.nu; u++, it++) {
                 const Unit un = unit_of(w.t, w.unit + u);
                 const int key = un.pre ? un.key : un.key + pl, end = un.pre ? un.hi : un.hi + pl;   // as positions
@@ -480,12 +550,13 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 page = page_of(u + 1);
                 const bool edge = there != (1u << boxes) - 1 || key < all_lo || key + kUnit > min(all_hi, end);
                 wait(b_s + 8u * (it & 1u), (it >> 1) & 1u);
-                if (it >= 2) wait_pv(it - 2);
                 tc::fence_after();
                 const uint32_t ts = tl + C::S_COL + (it & 1u) * kUnit;
                 uint32_t x[32];
                 tc::ld_32x32b_x32(ts + half * 32, x);
                 tc::wait_ld();
+                tc::fence_before();
+                arrive(b_read + 8u * (it & 1u));
                 if (edge) {
                     // the keys that this row sees, one bit each
                     auto below = [&](int k) { return k >= kUnit ? ~0ull : k <= 0 ? 0ull : (1ull << k) - 1; };
@@ -503,12 +574,11 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(x[j]));
                 float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 sm.top[it & 1][half][r0] = top;
-                tc::fence_before();
-                pair_sync();          // both have read their scores, too: P goes over them
-                tc::fence_after();
+                pair_sync();
                 top = fmaxf(top, sm.top[it & 1][half ^ 1][r0]) * a.scale;
                 // Units so far of this piece are in O: rescale it where a row's maximum has left its base behind.
                 // A row that saw nothing yet has zeros there and in l.
+                bool added = u == 0;  // the unit before is in O, and its P may be written over
                 if (u == 0) {
                     m = top - kLift;
                 } else {
@@ -516,7 +586,8 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     if (__any_sync(0xffffffffu, scale)) {
                         const float f = scale ? exp2_approx(m - (top - kLift)) : 1.f;
                         l *= f;
-                        wait_pv(it - 1);
+                        if (!added) wait_pv(it - 1);
+                        added = true;
                         #pragma unroll
                         for (int c = 0; c < DH; c += 32) {
                             uint32_t o[32];
@@ -541,12 +612,13 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     p[j] = *reinterpret_cast<const uint32_t*>(&h2);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tc::st_32x32b_x16(ts + half * 16, p);
+                if (!added) wait_pv(it - 1);
+                tc::st_32x32b_x16(tl + C::P_COL + half * 16, p);
                 if (u == 0 && tid == 0) *(volatile int*)&sm.acc = 0;
                 if (edge) {
                     // Values that no row sees become zeros; values that only some rows see and that are not
                     // finite (0 x NaN is not 0) are added row by row here and then cleared.
-                    const long long ev = e0 + (u + 1 < w.nu ? (long long)C::KE * (u + 2) + u : (long long)C::KE * w.nu + u);
+                    const long long ev = e0 + (long long)C::KE * min(u + 3, w.nu) + u;
                     const int s = (int)(ev % C::NST);
                     wait(full(s), (uint32_t)(ev / C::NST) & 1u);
                     // this thread's share: 16 bytes (tid % 8) of keys tid / 8 + 32 r in each 64-column chunk
@@ -587,9 +659,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         tc::fence_before();
                         named_bar_sync(1, kSoft);
                         tc::fence_after();
-                        if (u > 0) {
-                            wait_pv(it - 1);
-                        } else {
+                        if (u == 0) {
                             uint32_t z[32];
                             #pragma unroll
                             for (int j = 0; j < 32; j++) z[j] = 0;
@@ -600,7 +670,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         }
                         for (unsigned long long rest = odd; rest; rest &= rest - 1) {
                             const int j = __ffsll((long long)rest) - 1;
-                            const uint32_t pj = ld_tmem_x1(ts + j / 2);
+                            const uint32_t pj = ld_tmem_x1(tl + C::P_COL + j / 2);
                             tc::wait_ld();
                             const float pf = j & 1 ? h_hi(pj) : h_lo(pj);
                             const bool sees = key + j >= vlo && key + j < min(vhi, end) && ((there >> (j / box)) & 1u);
@@ -640,78 +710,21 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 }
                 tc::wait_st();
                 tc::fence_before();
-                mbar_arrive(b_p + 8u * (it & 1u));
+                arrive(b_p);
             }
             // where the row's result goes: finished, or this stretch's part of it
             const bool whole = w.nu == w.t.n, direct = whole && w.t.solo;
-            const size_t slot = whole ? ((size_t)(w.t.seq < 0 ? 0 : 1) * d.T + tok) * d.nH + hq
-                                      : ((size_t)blockIdx.x * 2 + (w.unit == 0 ? 1 : 0)) * kRowsP + r0;
-            char* dst = reinterpret_cast<char*>(!direct ? whole ? a.w.row : a.w.edge[1] : a.out);
-            const size_t elem = direct && !a.out_f32 ? 2 : 4;
-            const size_t mine = elem * (!direct ? whole ? slot * HD + part * C::DV : slot * C::DV
-                                                : (size_t)tok * a.out_stride + (size_t)hq * HD + part * C::DV);
+            const size_t at_slot = whole ? ((size_t)(w.t.seq < 0 ? 0 : 1) * d.T + tok) * d.nH + hq
+                                         : ((size_t)blockIdx.x * 2 + (w.unit == 0 ? 1 : 0)) * kRowsP + r0;
+            dst = reinterpret_cast<char*>(!direct ? whole ? a.w.row : a.w.edge[1] : a.out);
+            ml = direct ? nullptr : whole ? a.w.row_ml + at_slot * 2 + part : a.w.edge_ml[1] + at_slot;
+            esize = direct && !a.out_f32 ? 2 : 4;
+            mine = (size_t)esize * (!direct ? whole ? at_slot * HD + part * C::DV : at_slot * C::DV
+                                            : (size_t)tok * a.out_stride + (size_t)hq * HD + part * C::DV);
+            pending = true;
             e0 += (long long)(C::KE + 1) * w.nu;
             w.step();
             more = w.next();
-            // The scores of this piece are all made: the next one's Q may come, so that its first scores are made while
-            // this one's result is written.  (At hd 512 the stages lie in Q's place: after that.)
-            if (HD == C::QT && more) load_q();
-            wait_pv(it - 1);
-            sm.top[it & 1][half][r0] = l;
-            pair_sync();
-            l += sm.top[it & 1][half ^ 1][r0];
-            pair_sync();
-            const float inv = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            if (live && ok && !direct && half == 0)
-                *(whole ? a.w.row_ml + slot * 2 + part : a.w.edge_ml[1] + slot) = make_float2(m, l);
-            // 128 bytes of every row of the warp, from a row per lane to eight lanes per row
-            auto flush = [&](const uint32_t (&v)[32], size_t off) {
-                #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    st_shared(stage + lane * 128 + ((j ^ (lane & 7)) << 4),
-                              make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
-                __syncwarp();
-                #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int r = 4 * i + (lane >> 3);
-                    const uint4 x = ld_shared(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-                    const size_t o = __shfl_sync(0xffffffffu, mine, r) + off;
-                    if (ok && (mask >> r) & 1u) *reinterpret_cast<uint4*>(dst + o + (lane & 7) * 16) = x;
-                }
-                __syncwarp();
-            };
-            if (elem == 4) {
-                #pragma unroll 1
-                for (int c = half * DH; c < (half + 1) * DH; c += 32) {
-                    uint32_t o[32];
-                    tc::ld_32x32b_x32(tl + C::O_COL + c, o);
-                    tc::wait_ld();
-                    #pragma unroll
-                    for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * inv);
-                    flush(o, (size_t)c * 4);
-                }
-            } else {
-                #pragma unroll 1
-                for (int c = half * DH; c < (half + 1) * DH; c += 64) {
-                    uint32_t y[32];
-                    #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        uint32_t o[32];
-                        tc::ld_32x32b_x32(tl + C::O_COL + c + 32 * k, o);
-                        tc::wait_ld();
-                        #pragma unroll
-                        for (int j = 0; j < 16; j++)
-                            y[16 * k + j] = pack_half2(__float2half_rn(__uint_as_float(o[2 * j]) * inv),
-                                                       __float2half_rn(__uint_as_float(o[2 * j + 1]) * inv));
-                    }
-                    flush(y, (size_t)c * 2);
-                }
-            }
-            tc::fence_before();
-            if constexpr (HD > C::QT) {
-                named_bar_sync(1, kSoft);   // every stage has been emptied
-                if (more) load_q();
-            }
         }
     }
     tc::fence_before();

@@ -11,10 +11,11 @@ namespace g4b {
 namespace pg {
 
 // Row of the cache, seen as [num_pages * nkv * page_size] rows of hd, that holds key `key` of a segment for KV
-// head `head`, given the page's id; -1 where the id names no page.  num_pages * nkv * page_size < 2^31.
-G4B_HD int cache_row(int page, int num_pages, int nkv, int page_size, int head, int key) {
+// head `head`, given the page's id and the log2 of the page size; -1 where the id names no page.
+// num_pages * nkv * page_size < 2^31.
+G4B_HD int cache_row(int page, int num_pages, int nkv, int log2_page_size, int head, int key) {
     if (page < 0 || page >= num_pages) return -1;
-    return (page * nkv + head) * page_size + key % page_size;
+    return ((page * nkv + head) << log2_page_size) + (key & ((1 << log2_page_size) - 1));
 }
 
 // The CTAs whose stretches of `u` units hold the units [g, g + n) of the line of all work (n >= 1).

@@ -120,7 +120,8 @@ def host(tmp_path_factory):
     d = tmp_path_factory.mktemp("pages")
     src, so = d / "pages.cpp", d / "pages.so"
     src.write_text('#include "g4b_pages.h"\nextern "C" {\n'
-                   "int row(int p, int n, int k, int s, int h, int key) { return g4b::pg::cache_row(p, n, k, s, h, key); }\n"
+                   "int row(int p, int n, int k, int s, int h, int key) "
+                   "{ return g4b::pg::cache_row(p, n, k, __builtin_ctz(s), h, key); }\n"
                    "void span(long long g, int n, long long u, int* o) "
                    "{ auto s = g4b::pg::span_of(g, n, u); o[0] = s.c0; o[1] = s.c1; }\n}\n")
     subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-I", CSRC, str(src), "-o", str(so)], check=True)
