@@ -57,13 +57,14 @@ static int make_dims(const char* op, int T, int B, int nH, int nkv, int hd, int 
     d.pre_pages = pre_pages;
     d.window = window;
     while ((1 << d.lps) < ps) d.lps++;
+    d.few = few_most(hd);
     d.cs = hd == 512 ? 2 : 1;
     d.ctas[0] = sms * few_per_sm(hd);
     d.ctas[1] = sms;
     const int rows = T * d.G;
     const bool many = many_rows(hd);
     // tiles of sequences (one more each for the last, partial one) and of the prefix
-    d.max_tiles[0] = (many ? 0 : 2 * (rows / kRowsS)) + B + 1;
+    d.max_tiles[0] = many ? (B + 1) * (d.few / kRowsS) : 2 * (rows / kRowsS) + B + 1;
     d.max_tiles[1] = many ? 2 * (rows / kRowsP) + B + 1 : 0;
     size_t o = up256(sizeof(Hdr));
     auto take = [&](size_t bytes) {
@@ -183,11 +184,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     }
     __syncthreads();
     const int r_lo = st[0] * G, r_hi = st[B] * G;
-    const bool pre_many = a.many && r_hi - r_lo > kRowsS;
+    const bool pre_many = a.many && r_hi - r_lo > d.few;
     const int pre_rows = pre_many ? kRowsP : kRowsS;
     const int pre_tiles = pl > 0 ? (r_hi - r_lo + pre_rows - 1) / pre_rows : 0;
     auto alone = [&](int b) { return (st[b + 1] - st[b]) * G > kRowsAlone; };
-    auto many_of = [&](int b) { return a.many && (st[b + 1] - st[b]) * G > kRowsS; };
+    auto many_of = [&](int b) { return a.many && (st[b + 1] - st[b]) * G > d.few; };
     // first tile of each sequence: the prefix's come first
     int nt[2] = {pre_many ? 0 : pre_tiles, pre_many ? pre_tiles : 0};
     for (int i0 = 0; i0 < B; i0 += kPlanThreads) {
@@ -1434,7 +1435,7 @@ int g4b_paged_attn(const uint16_t* q, long long q_stride, const uint16_t* kc, co
     }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     // no tile of many rows: neither a sequence nor the prefix has more rows than the batch
-    const bool many = many_rows(hd) && T * a.d.G > kRowsS;
+    const bool many = many_rows(hd) && T * a.d.G > a.d.few;
     if (many) {
         st = launch_many(a, s);
         if (st != G4B_OK) return st;

@@ -7,8 +7,8 @@
 // sequences share, the others in the sequence's own table row.
 //
 // The attention of a KV head is cut into tiles: rows (row = token * G + query head of the group) against keys, in
-// units of 64 keys.  A sequence with up to kRowsS rows (a decode step, a few proposed tokens) has a tile of its own keys
-// for the few-rows kernel, one with more has tiles of kRowsP rows.  Up to kRowsAlone, its rows also join those of
+// units of 64 keys.  A sequence with up to few_most rows (a decode step, a few proposed tokens) has a tile of its own keys
+// for the few-rows kernel (or two, of kRowsS rows each), one with more has tiles of kRowsP rows.  Up to kRowsAlone, its rows also join those of
 // the other such sequences in tiles against the prefix; with more (a prompt's chunk) it fills tiles by itself,
 // which read the prefix and then its own keys.  The units of all tiles and KV heads
 // form one line that is cut into equal lengths, one per CTA, whatever the lengths of the sequences: a CTA
@@ -25,6 +25,11 @@ namespace pg {
 
 constexpr int kUnit = 64;        // keys per unit of work
 constexpr int kRowsS = 8;        // rows of a tile of the few-rows kernel (the n of m16n8k16)
+// A sequence of up to this many rows goes to the few-rows kernel, in one tile or two.  Two tiles read the keys twice,
+// mostly from L2: at hd 128 that is faster than a 128-row tile with 16 rows in it (64 sequences of 16 rows over 2,000
+// keys: 31 us against 40; over 200: 12 against 17), from hd 256 on only for short sequences (32 of 16 rows over
+// 2,000 keys: 174 us against 122).
+constexpr int few_most(int hd) { return hd == 128 ? 16 : 8; }
 constexpr int kRowsP = 128;      // rows of a tile of the many-rows kernel (tensor memory lanes)
 // A sequence of more rows than this reads the prefix in its own tiles; one of fewer shares tiles of the prefix with
 // others and has its partial results joined.  Half a tile: by itself it would use less of a tile's products than that.
@@ -75,6 +80,7 @@ struct Hdr {
 struct Dims {
     int T, B, nH, nkv, G, hd, ps, own_pages, pre_pages, window;
     int lps;                         // log2 of the page size
+    int few;                         // few_most(hd)
     int cs;                          // walks per many-rows tile: parts of hd's output columns
     int ctas[2];                     // stretches per kind
     int max_tiles[2];

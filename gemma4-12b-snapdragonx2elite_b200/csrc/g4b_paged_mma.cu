@@ -620,6 +620,9 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     // finite (0 x NaN is not 0) are added row by row here and then cleared.
                     const long long ev = e0 + (long long)C::KE * min(u + 3, w.nu) + u;
                     const int s = (int)(ev % C::NST);
+                    // A barrier's parity tells a phase from the one before only, so the slot's last tenant has to have landed:
+                    // it is at the latest a K entry of the next unit, and that one's scores say so.
+                    if (u + 1 < w.nu) wait(b_s + 8u * ((it + 1) & 1u), ((it + 1) >> 1) & 1u);
                     wait(full(s), (uint32_t)(ev / C::NST) & 1u);
                     // this thread's share: 16 bytes (tid % 8) of keys tid / 8 + 32 r in each 64-column chunk
                     const uint32_t vt = ring + s * C::ENTRY + tid * 16;
