@@ -4,7 +4,7 @@
 // A tile is 128 rows (token, query head of the group) of one KV head, a row per tensor memory lane; units of 64
 // keys stream past it.  Per unit
 //   S [128 x 64] = Q K^T      (tcgen05, Q in tensor memory, K from shared memory)
-//   P = 2^(S scale - m)       (two threads per row: a row's maximum takes one exchange through shared memory)
+//   P = 2^(S scale - m)       (a thread per row: no reduction leaves it; two groups of four warps take units in turn)
 //   O [128 x hd] += P V       (tcgen05, P in tensor memory over S's columns, V from shared memory)
 // S is double buffered and P has columns of its own, so the tensor core makes the scores two units ahead: a buffer is
 // free as soon as its scores have been read, and the softmax warps find the next ones ready.  (With P over S, the scores of
@@ -28,7 +28,8 @@ namespace pg {
 
 __device__ unsigned g_status_paged_mma;
 
-constexpr int kSoft = 256;              // softmax threads: two per row
+constexpr int kGroup = 128;             // softmax threads of a group: one per row
+constexpr int kSoft = 2 * kGroup;       // two groups
 constexpr int kManyThreads = kSoft + 64;
 constexpr float kLift = 4.f;            // log2 of the weight that a row's maximum gets when its base is set
 constexpr float kMost = 15.f;           // log2 of the largest weight before the base is set anew (f16: below 2^16)
@@ -55,9 +56,10 @@ struct ManyCfg {
     // Everything else that is shared, behind the buffers: no static shared memory, so that the buffers begin where the
     // CTA's window does, at a multiple of 1024 (the kernel checks).
     struct Small {
-        uint64_t bars[2 * NST + 10];
-        unsigned long long odd;            // keys of the unit with a value that is not finite
-        float top[2][2][kRowsP];           // [unit % 2][half][row]
+        uint64_t bars[2 * NST + 14];
+        unsigned long long odd[2];         // [group]: keys of its unit with a value that is not finite
+        float base[2][kRowsP];             // [unit % 2][row]: the base after that unit
+        float sum[2][kRowsP];              // [group][row]: the groups' sums at a piece's end
         int red[4][4];
         uint32_t tmem;
         int abort, acc;
@@ -87,12 +89,12 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
     return r != 0;
 }
-// or of all softmax threads' flags
-__device__ __forceinline__ bool any_soft(bool v) {
+// or of a softmax group's flags, at its barrier
+__device__ __forceinline__ bool any_of_group(bool v, int barrier) {
     int r;
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
-        : "=r"(r) : "r"((int)v) : "memory");
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+        : "=r"(r) : "r"((int)v), "r"(barrier) : "memory");
     return r != 0;
 }
 __device__ __forceinline__ void st_shared(uint32_t at, uint4 v) {
@@ -187,19 +189,23 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
     auto empty = [&](int s) { return bar0 + 8u * (C::NST + s); };
     const uint32_t b_s = bar0 + 8u * (2 * C::NST);                   // [2] scores of a unit are there
     const uint32_t b_read = b_s + 16;                                // [2] and have been read
-    const uint32_t b_p = b_s + 32;                                   // its weights are there
-    const uint32_t b_pv = b_s + 40;                                  // its product is added
-    const uint32_t b_q = b_s + 48;                                   // the piece's Q is there
-    const uint32_t b_drain = b_s + 56;
+    const uint32_t b_base = b_s + 32;                                // [2] the rows' bases are set
+    const uint32_t b_pv = b_s + 48;                                  // [2] the unit's product is added
+    const uint32_t b_p = b_s + 64;                                   // its weights are there
+    const uint32_t b_q = b_s + 72;                                   // the piece's Q is there
+    const uint32_t b_o = b_s + 80;                                   // the piece's products are all added
+    const uint32_t b_drain = b_s + 88;
     if (tid == 0) {
         for (int i = 0; i < 2 * C::NST; i++) mbar_init(bar0 + 8u * i, 1);
-        mbar_init(b_s, 1);
-        mbar_init(b_s + 8, 1);
-        mbar_init(b_read, kSoft / 32);
-        mbar_init(b_read + 8, kSoft / 32);
-        mbar_init(b_p, kSoft / 32);
-        mbar_init(b_pv, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(b_s + 8 * i, 1);
+            mbar_init(b_read + 8 * i, kGroup / 32);
+            mbar_init(b_base + 8 * i, kGroup / 32);
+            mbar_init(b_pv + 8 * i, 1);
+        }
+        mbar_init(b_p, kGroup / 32);
         mbar_init(b_q, kSoft / 32);
+        mbar_init(b_o, 1);
         mbar_init(b_drain, 1);
         fence_mbar_init();
         sm.abort = 0;
@@ -348,7 +354,8 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         tc::mma_f16_ts(tmem + C::O_COL, tmem + C::P_COL + 8 * k, vd + (uint64_t)(k * (2048 / 16)), id_o,
                                        acc || k > 0);
                     tc::commit(empty(s));
-                    tc::commit(b_pv);
+                    tc::commit(b_pv + 8u * ((it + u) & 1u));
+                    if (u == w.nu - 1) tc::commit(b_o);
                 }
                 __syncwarp();
             }
@@ -362,21 +369,22 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         }
         __syncwarp();
     } else {
-        // ---------------------------------------------------------------- softmax: two threads per row
-        // Thread `half` of row `r` takes 32 of a unit's 64 keys, half of Q's and of O's columns; the two rows of warps
-        // that share tensor memory lanes meet at a barrier of their own once per unit, for the row's maximum.
+        // ---------------------------------------------------------------- softmax: two groups
+        // A unit is one group's, a thread per row; the groups take units in turn, so that one's loads, exchanges and
+        // stores run beside the other's exponentials.  A row's base passes from group to group with each unit.  (Q and the
+        // result are halved by columns instead.)
         const int half = warp >> 2, wq = warp & 3, r0 = wq * 32 + lane;
         const uint32_t tl = tmem + ((uint32_t)(wq * 32) << 16);      // this warp's lanes
-        constexpr int DH = C::DV / 2;                                // this half's columns of O
-        const uint32_t to = tl + C::O_COL + half * DH;
-        auto pair_sync = [&]() { named_bar_sync(2 + wq, 64); };
+        constexpr int DH = C::DV / 2;                                // columns of the result that this warp writes
+        const int group_bar = 2 + half;                              // the group's named barrier; 1 is both's
+        auto group_sync = [&]() { named_bar_sync(2 + half, kGroup); };
         // one arrival per warp: 32 lanes' on one barrier would come one after the other
         auto arrive = [&](uint32_t bar) {
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
         const uint32_t stage = stages + warp * C::STAGE;
-        uint32_t it = 0;                          // units so far
+        uint32_t it = 0, pieces = 0;              // units and pieces so far
         long long e0 = 0;                         // ring entries of the pieces before
         // A wait that ran out clears ok.  The warp then walks on without waiting, so that the warps meet at
         // the same named barriers to the end; it writes no result.
@@ -384,10 +392,10 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         auto wait = [&](uint32_t bar, uint32_t parity) {
             ok = __all_sync(0xffffffffu, ok && wait_short(bar, parity, abort, status));
         };
-        // The product of a unit is added.  A parity tells a barrier's last two phases apart only: every unit waits for
-        // the one before it, once.
+        // The product of a unit is added, waited for by the next unit's group.  (A parity tells a barrier's phase from the
+        // one before only: with a barrier for each group's units, none is skipped.)
         auto wait_pv = [&](uint32_t unit) {
-            wait(b_pv, unit & 1u);
+            wait(b_pv + 8u * (unit & 1u), (unit >> 1) & 1u);
             tc::fence_after();
         };
         // Q of the piece that w stands at
@@ -455,13 +463,20 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         float2* ml = nullptr;                     // its (base, sum), null where the result is finished here,
         int esize = 4;                            // the bytes of an element
         for (;;) {
+            // the last unit's scores, which may be the other group's, are made: Q may be written over
+            if (pending) wait(b_s + 8u * ((it - 1) & 1u), ((it - 1) >> 1) & 1u);
             if (!C::STAGE_IN_Q && more) load_q();
             if (pending) {
-                wait_pv(it - 1);
-                sm.top[it & 1][half][r0] = l;
-                pair_sync();
-                l += sm.top[it & 1][half ^ 1][r0];
-                pair_sync();
+                // both groups' sums, on the last unit's base
+                wait(b_base + 8u * ((it - 1) & 1u), ((it - 1) >> 1) & 1u);
+                const float last = sm.base[(it - 1) & 1][r0];
+                if (m != last && l != 0.f) l *= exp2_approx(m - last);
+                m = last;
+                sm.sum[half][r0] = l;
+                named_bar_sync(1, kSoft);
+                l = sm.sum[0][r0] + sm.sum[1][r0];
+                wait(b_o, (pieces - 1) & 1u);
+                tc::fence_after();
                 const float inv = ml ? 1.f : l == 0.f ? 0.f : 1.f / l;
                 if (((mask >> lane) & 1u) && ok && ml && half == 0) *ml = make_float2(m, l);
                 // 128 bytes of every row of the warp, from a row per lane to eight lanes per row
@@ -540,23 +555,28 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 const int* table = un.pre ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
                 return lane < boxes && idx < (un.pre ? d.pre_pages : d.own_pages) ? __ldg(table + idx) : -1;
             };
-            int page = page_of(0);
             m = -INFINITY;
             l = 0.f;
-            for (int u = 0; u < w.nu; u++, it++) {
+            const uint32_t it0 = it;
+            const int u0 = (int)((it0 ^ (uint32_t)half) & 1u);       // this group's first unit
+            int page = page_of(u0);
+            #pragma unroll 1
+            for (int u = u0; u < w.nu; u += 2) {
+                it = it0 + u;
                 const Unit un = unit_of(w.t, w.unit + u);
                 const int key = un.pre ? un.key : un.key + pl, end = un.pre ? un.hi : un.hi + pl;   // as positions
                 const unsigned there = __ballot_sync(0xffffffffu, lane < boxes && page >= 0 && page < a.num_pages);
-                page = page_of(u + 1);
+                page = page_of(u + 2);
                 const bool edge = there != (1u << boxes) - 1 || key < all_lo || key + kUnit > min(all_hi, end);
-                wait(b_s + 8u * (it & 1u), (it >> 1) & 1u);
+                wait(b_s + 8u * half, (it >> 1) & 1u);
                 tc::fence_after();
-                const uint32_t ts = tl + C::S_COL + (it & 1u) * kUnit;
-                uint32_t x[32];
-                tc::ld_32x32b_x32(ts + half * 32, x);
+                const uint32_t ts = tl + C::S_COL + half * kUnit;
+                uint32_t x[2][32];
+                tc::ld_32x32b_x32(ts, x[0]);
+                tc::ld_32x32b_x32(ts + 32, x[1]);
                 tc::wait_ld();
                 tc::fence_before();
-                arrive(b_read + 8u * (it & 1u));
+                arrive(b_read + 8u * half);
                 if (edge) {
                     // the keys that this row sees, one bit each
                     auto below = [&](int k) { return k >= kUnit ? ~0ull : k <= 0 ? 0ull : (1ull << k) - 1; };
@@ -564,57 +584,61 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     if (there != (1u << boxes) - 1)
                         for (int b = 0; b < boxes; b++)
                             if (!((there >> b) & 1u)) bits &= ~(below((b + 1) * box) & ~below(b * box));
-                    const uint32_t mine = (uint32_t)(bits >> (32 * half));
                     #pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (!((mine >> j) & 1u)) x[j] = 0xff800000u;
+                    for (int k = 0; k < 2; k++)
+                        #pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if (!(((uint32_t)(bits >> (32 * k)) >> j) & 1u)) x[k][j] = 0xff800000u;
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 #pragma unroll
-                for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(x[j]));
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                sm.top[it & 1][half][r0] = top;
-                pair_sync();
-                top = fmaxf(top, sm.top[it & 1][half ^ 1][r0]) * a.scale;
-                // Units so far of this piece are in O: rescale it where a row's maximum has left its base behind.
-                // A row that saw nothing yet has zeros there and in l.
+                for (int j = 0; j < 32; j++) {
+                    mx[j & 1] = fmaxf(mx[j & 1], __uint_as_float(x[0][j]));
+                    mx[2 + (j & 1)] = fmaxf(mx[2 + (j & 1)], __uint_as_float(x[1][j]));
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
+                // The base that the other group left, or a new one.  Units so far of this piece are in O: rescale it where
+                // a row's maximum has left its base behind.  A row that saw nothing yet has zeros there and in l.
+                if (it > 0) wait(b_base + 8u * (half ^ 1), ((it - 1) >> 1) & 1u);
+                const float from = u > 0 ? sm.base[half ^ 1][r0] : -INFINITY;
+                if (m != from && l != 0.f) l *= exp2_approx(m - from);
+                const bool set = u == 0 || top > from + kMost, scale = set && from != -INFINITY;
+                m = set ? top - kLift : from;
+                sm.base[half][r0] = m;
+                arrive(b_base + 8u * half);
                 bool added = u == 0;  // the unit before is in O, and its P may be written over
-                if (u == 0) {
-                    m = top - kLift;
-                } else {
-                    const bool set = top > m + kMost, scale = set && m != -INFINITY;
-                    if (__any_sync(0xffffffffu, scale)) {
-                        const float f = scale ? exp2_approx(m - (top - kLift)) : 1.f;
-                        l *= f;
-                        if (!added) wait_pv(it - 1);
-                        added = true;
+                if (__any_sync(0xffffffffu, scale)) {
+                    const float f = scale ? exp2_approx(from - m) : 1.f;
+                    l *= f;
+                    wait_pv(it - 1);
+                    added = true;
+                    #pragma unroll 1
+                    for (int c = 0; c < C::DV; c += 32) {
+                        uint32_t o[32];
+                        tc::ld_32x32b_x32(tl + C::O_COL + c, o);
+                        tc::wait_ld();
                         #pragma unroll
-                        for (int c = 0; c < DH; c += 32) {
-                            uint32_t o[32];
-                            tc::ld_32x32b_x32(to + c, o);
-                            tc::wait_ld();
-                            #pragma unroll
-                            for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                            tc::st_32x32b_x32(to + c, o);
-                        }
+                        for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        tc::st_32x32b_x32(tl + C::O_COL + c, o);
                     }
-                    if (set) m = top - kLift;
                 }
                 const float base = m == -INFINITY ? 0.f : m;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t p[16];
                 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const float e0 = exp2_approx(fmaf(__uint_as_float(x[2 * j]), a.scale, -base));
-                    const float e1 = exp2_approx(fmaf(__uint_as_float(x[2 * j + 1]), a.scale, -base));
-                    sum[j & 3] += e0 + e1;
-                    const __half2 h2 = __floats2half2_rn(e0, e1);
-                    p[j] = *reinterpret_cast<const uint32_t*>(&h2);
-                }
+                for (int k = 0; k < 2; k++)
+                    #pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const float e0x = exp2_approx(fmaf(__uint_as_float(x[k][2 * j]), a.scale, -base));
+                        const float e1x = exp2_approx(fmaf(__uint_as_float(x[k][2 * j + 1]), a.scale, -base));
+                        sum[j & 3] += e0x + e1x;
+                        const __half2 h2 = __floats2half2_rn(e0x, e1x);
+                        x[0][16 * k + j] = *reinterpret_cast<const uint32_t*>(&h2);   // P over the scores it is made of
+                    }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                if (!added) wait_pv(it - 1);
-                tc::st_32x32b_x16(tl + C::P_COL + half * 16, p);
-                if (u == 0 && tid == 0) *(volatile int*)&sm.acc = 0;
+                if (u == 0 && it > 0) wait_pv(it - 1);     // of the piece before: done, but its phase is counted
+                else if (!added) wait_pv(it - 1);
+                tc::st_32x32b_x32(tl + C::P_COL, x[0]);
+                if (u == 0 && r0 == 0) *(volatile int*)&sm.acc = 0;
                 if (edge) {
                     // Values that no row sees become zeros; values that only some rows see and that are not
                     // finite (0 x NaN is not 0) are added row by row here and then cleared.
@@ -622,20 +646,20 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     const int s = (int)(ev % C::NST);
                     // A barrier's parity tells a phase from the one before only, so the slot's last tenant has to have landed:
                     // it is at the latest a K entry of the next unit, and that one's scores say so.
-                    if (u + 1 < w.nu) wait(b_s + 8u * ((it + 1) & 1u), ((it + 1) >> 1) & 1u);
+                    if (u + 1 < w.nu) wait(b_s + 8u * (half ^ 1), ((it + 1) >> 1) & 1u);
                     wait(full(s), (uint32_t)(ev / C::NST) & 1u);
-                    // this thread's share: 16 bytes (tid % 8) of keys tid / 8 + 32 r in each 64-column chunk
-                    const uint32_t vt = ring + s * C::ENTRY + tid * 16;
+                    // this thread's share: 16 bytes (r0 % 8) of keys r0 / 8 + 16 r in each 64-column chunk
+                    const uint32_t vt = ring + s * C::ENTRY + r0 * 16;
                     uint32_t bad = 0;
-                    bool some[2];                            // key r is seen by some rows only
+                    bool some[4];                            // key r is seen by some rows only
                     #pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        const int k = key + (tid >> 3) + 32 * r;
+                    for (int r = 0; r < 4; r++) {
+                        const int k = key + (r0 >> 3) + 16 * r;
                         const bool none = k < any_lo || k >= min(any_hi, end);
                         some[r] = !none && (k < all_lo || k >= all_hi);
                         #pragma unroll
                         for (int c = 0; c < C::DV / 64; c++) {
-                            const uint32_t at = vt + c * (kUnit * 128) + r * (32 * 128);
+                            const uint32_t at = vt + c * (kUnit * 128) + r * (16 * 128);
                             if (none) {
                                 st_shared(at, make_uint4(0, 0, 0, 0));
                             } else if (some[r]) {
@@ -645,31 +669,28 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         }
                     }
                     unsigned long long odd = 0;
-                    if (any_soft((bad & 0x80008000u) != 0)) {
-                        if (tid == 0) sm.odd = 0;
-                        named_bar_sync(1, kSoft);
-                        for (int r = 0; r < 2; r++)
+                    if (any_of_group((bad & 0x80008000u) != 0, group_bar)) {
+                        if (r0 == 0) sm.odd[half] = 0;
+                        group_sync();
+                        for (int r = 0; r < 4; r++)
                             for (int c = 0; c < C::DV / 64 && some[r]; c++) {
-                                const uint4 v = ld_shared(vt + c * (kUnit * 128) + r * (32 * 128));
+                                const uint4 v = ld_shared(vt + c * (kUnit * 128) + r * (16 * 128));
                                 if ((not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w)) & 0x80008000u)
-                                    atomicOr(&sm.odd, 1ull << ((tid >> 3) + 32 * r));
+                                    atomicOr(&sm.odd[half], 1ull << ((r0 >> 3) + 16 * r));
                             }
-                        named_bar_sync(1, kSoft);
-                        odd = *(volatile unsigned long long*)&sm.odd;
+                        group_sync();
+                        odd = *(volatile unsigned long long*)&sm.odd[half];
                     }
                     if (odd) {
-                        tc::wait_st();                       // P, read back below, the other half's too
-                        tc::fence_before();
-                        named_bar_sync(1, kSoft);
-                        tc::fence_after();
+                        tc::wait_st();                       // P, read back below
                         if (u == 0) {
                             uint32_t z[32];
                             #pragma unroll
                             for (int j = 0; j < 32; j++) z[j] = 0;
-                            #pragma unroll
-                            for (int c = 0; c < DH; c += 32) tc::st_32x32b_x32(to + c, z);
+                            #pragma unroll 1
+                            for (int c = 0; c < C::DV; c += 32) tc::st_32x32b_x32(tl + C::O_COL + c, z);
                             tc::wait_st();
-                            if (tid == 0) *(volatile int*)&sm.acc = 1;
+                            if (r0 == 0) *(volatile int*)&sm.acc = 1;
                         }
                         for (unsigned long long rest = odd; rest; rest &= rest - 1) {
                             const int j = __ffsll((long long)rest) - 1;
@@ -678,7 +699,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                             const float pf = j & 1 ? h_hi(pj) : h_lo(pj);
                             const bool sees = key + j >= vlo && key + j < min(vhi, end) && ((there >> (j / box)) & 1u);
                             #pragma unroll 1
-                            for (int c = half * DH; c < (half + 1) * DH; c += 32) {
+                            for (int c = 0; c < C::DV; c += 32) {
                                 uint32_t o[32];
                                 tc::ld_32x32b_x32(tl + C::O_COL + c, o);
                                 tc::wait_ld();
@@ -689,7 +710,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                                     const uint4 v = ld_shared(vr + ((un ^ (j & 7)) << 4));
                                     const uint32_t y[4] = {v.x, v.y, v.z, v.w};
                                     #pragma unroll
-                                    for (int r = 0; r < 2; r++) {
+                                    for (int r = 0; r < 4; r++) {
                                         float lo = __uint_as_float(o[8 * q + 2 * r]), hi = __uint_as_float(o[8 * q + 2 * r + 1]);
                                         if (sees) {
                                             lo += pf * h_lo(y[r]);
@@ -703,11 +724,11 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                                 tc::wait_st();
                             }
                         }
-                        named_bar_sync(1, kSoft);              // every row has read the values
-                        for (int r = 0; r < 2; r++)
+                        group_sync();                        // every row has read the values
+                        for (int r = 0; r < 4; r++)
                             for (int c = 0; c < C::DV / 64; c++)
-                                if ((odd >> ((tid >> 3) + 32 * r)) & 1ull)
-                                    st_shared(vt + c * (kUnit * 128) + r * (32 * 128), make_uint4(0, 0, 0, 0));
+                                if ((odd >> ((r0 >> 3) + 16 * r)) & 1ull)
+                                    st_shared(vt + c * (kUnit * 128) + r * (16 * 128), make_uint4(0, 0, 0, 0));
                     }
                     if (odd || key < any_lo || key + kUnit > min(any_hi, end)) tc::fence_proxy_async_smem();   // V was written
                 }
@@ -715,6 +736,8 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 tc::fence_before();
                 arrive(b_p);
             }
+            it = it0 + w.nu;
+            pieces++;
             // where the row's result goes: finished, or this stretch's part of it
             const bool whole = w.nu == w.t.n, direct = whole && w.t.solo;
             const size_t at_slot = whole ? ((size_t)(w.t.seq < 0 ? 0 : 1) * d.T + tok) * d.nH + hq
