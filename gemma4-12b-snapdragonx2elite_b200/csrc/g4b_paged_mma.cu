@@ -14,7 +14,7 @@
 // to 2^-18 of the maximum out of f16's subnormals).
 // K and V units come by TMA through one ring of 64-key buffers, issued ahead across pieces.
 //
-// Warps: 0-7 softmax, the mask, the rows' Q and the result; 8 TMA; 9 MMA issue.
+// Warps: 0-7 softmax, the mask, the rows' Q and the result; 8 TMA; 9 and 10 MMA issue.
 // Tensor memory's 512 columns: O 256, S 128, P 32 and the first 192 elements of Q; its others are in shared memory.  At hd
 // 512 O alone would fill them, so a tile is walked once for each half of the output columns (the scores are made twice).
 //
@@ -30,7 +30,7 @@ __device__ unsigned g_status_paged_mma;
 
 constexpr int kGroup = 128;             // softmax threads of a group: one per row
 constexpr int kSoft = 2 * kGroup;       // two groups
-constexpr int kManyThreads = kSoft + 64;
+constexpr int kManyThreads = kSoft + 96;    // and a warp each for TMA, scores and products
 constexpr float kLift = 4.f;            // log2 of the weight that a row's maximum gets when its base is set
 constexpr float kMost = 15.f;           // log2 of the largest weight before the base is set anew (f16: below 2^16)
 
@@ -39,20 +39,23 @@ struct ManyCfg {
     static constexpr int DV = HD < 256 ? HD : 256;      // output columns of a walk
     static constexpr int CS = HD / DV;                  // walks per tile
     static constexpr int QT = HD == 128 ? 128 : 192;    // elements of Q in tensor memory; the rest in shared memory
-    static constexpr int KE = HD / DV;                  // ring entries per unit of K
-    static constexpr int ENTRY = kUnit * DV * 2;        // bytes of a ring entry: 64 keys x DV elements
+    // A ring entry is 64 keys of EC elements; a unit's K is KE of them and its V (a walk's columns) VE.  K and V have a
+    // ring each: then the one warp that consumes a ring sees every phase of its barriers.
+    static constexpr int EC = HD == 512 ? 128 : DV;
+    static constexpr int KE = HD / EC, VE = DV / EC;
+    static constexpr int ENTRY = kUnit * EC * 2;
+    static constexpr int NK = HD == 128 ? 5 : HD == 256 ? 3 : 6, NV = HD == 128 ? 5 : HD == 256 ? 2 : 3;
+    static constexpr int NST = NK + NV;
     static constexpr int QS_BYTES = kRowsP * (HD - QT) * 2;
     // a warp's 32 rows x 128 bytes on their way between rows in memory and rows in lanes; at hd 512 they lie in
     // the shared part of Q, which is idle then
     static constexpr int STAGE = 32 * 128;
     static constexpr bool STAGE_IN_Q = HD == 512;
-    static constexpr int NST = HD == 128 ? 10 : HD == 256 ? 5 : 4;
     static constexpr int BUF = NST * ENTRY + QS_BYTES + (STAGE_IN_Q ? 0 : 8 * STAGE);
     static constexpr int O_COL = 0, S_COL = DV, P_COL = S_COL + 2 * kUnit, Q_COL = P_COL + kUnit / 2;
     static_assert(Q_COL + QT / 2 <= 512, "tensor memory columns");
     // (the stages are the last two 64-element chunks of Q's shared part, which are written last)
     static_assert(!STAGE_IN_Q || (QS_BYTES >= 8 * STAGE && 8 * STAGE == 2 * kRowsP * 128), "the stages fit");
-    static_assert(KE * 2 <= NST, "the scores of two units need nothing but K");
     // Everything else that is shared, behind the buffers: no static shared memory, so that the buffers begin where the
     // CTA's window does, at a multiple of 1024 (the kernel checks).
     struct Small {
@@ -194,7 +197,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
     const uint32_t b_p = b_s + 64;                                   // its weights are there
     const uint32_t b_q = b_s + 72;                                   // the piece's Q is there
     const uint32_t b_o = b_s + 80;                                   // the piece's products are all added
-    const uint32_t b_drain = b_s + 88;
+    const uint32_t b_drain = b_s + 88;                               // [2] winding down
     if (tid == 0) {
         for (int i = 0; i < 2 * C::NST; i++) mbar_init(bar0 + 8u * i, 1);
         for (int i = 0; i < 2; i++) {
@@ -207,6 +210,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         mbar_init(b_q, kSoft / 32);
         mbar_init(b_o, 1);
         mbar_init(b_drain, 1);
+        mbar_init(b_drain + 8, 1);
         fence_mbar_init();
         sm.abort = 0;
     }
@@ -224,16 +228,16 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
 
     if (warp == 8) {
         // ---------------------------------------------------------------- TMA
-        int slot = 0, used = 0;                   // the next entry's slot; slots that were ever filled
-        uint32_t turn = 0;                        // parity of the ring's round
+        int slot[2] = {0, 0}, used[2] = {0, 0};   // of K's and V's ring: the next slot; slots that were ever filled
+        uint32_t turn[2] = {0, 0};                // parity of the ring's round
         bool ok = true;
         while (ok && w.next()) {
             const int head = w.head / C::CS, part = w.head % C::CS;
-            // An entry is DV / 64 column chunks of `boxes` boxes of `box` rows.  Each lane has one box of it: one
+            // An entry is EC / 64 column chunks of `boxes` boxes of `box` rows.  Each lane has one box of it: one
             // instruction of the warp issues them all (one thread's loop over them took longer than the units' MMAs).
             const int box = min(d.ps, kUnit), boxes = kUnit / box, lboxes = __ffs(boxes) - 1;
             const int my_p = lane & (boxes - 1), my_c = lane >> lboxes;
-            const bool issues = my_c < C::DV / 64;
+            const bool issues = my_c < C::EC / 64;
             const uint32_t my_dst = ring + my_c * (kUnit * 128) + my_p * box * 128;
             int ids = -1, ids_at = -64;
             bool ids_pre = false;
@@ -252,23 +256,29 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 const int id = __shfl_sync(0xffffffffu, ids, (k >> d.lps) - ids_at);
                 const int at_row = cache_row(id, a.num_pages, d.nkv, d.lps, head, k);
                 const int row = at_row < 0 ? a.num_pages * d.nkv * d.ps : at_row;   // past the map: zeros
-                for (int part_e = 0; part_e < (is_v ? 1 : C::KE); part_e++) {
-                    const int s = slot;
-                    // from the second round on: the slot's products of the round before are done
-                    if (used == C::NST && !wait_short(empty(s), turn ^ 1u, abort, status)) ok = false;
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) return;
-                    if (lane == 0) mbar_arrive_expect_tx(full(s), C::ENTRY);
+                const int first = is_v ? C::NK : 0, slots = is_v ? C::NV : C::NK, x0 = is_v ? part * C::DV : 0;
+                int s = slot[is_v], n = used[is_v];
+                uint32_t t = turn[is_v];
+                #pragma unroll 1
+                for (int e = 0; e < (is_v ? C::VE : C::KE); e++) {
+                    // from the second round on: the slot's MMAs of the round before are done
+                    if (n == slots)
+                        ok = __all_sync(0xffffffffu, wait_short(empty(first + s), t ^ 1u, abort, status));
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(full(first + s), C::ENTRY);
                     __syncwarp();
                     if (issues)
-                        tma_box(my_dst + s * C::ENTRY, is_v ? &vmap : &kmap, (is_v ? part : part_e) * C::DV + 64 * my_c, row,
-                                full(s));
-                    used = max(used, s + 1);
-                    if (++slot == C::NST) {
-                        slot = 0;
-                        turn ^= 1u;
+                        tma_box(my_dst + (first + s) * C::ENTRY, is_v ? &vmap : &kmap, x0 + e * C::EC + 64 * my_c, row,
+                                full(first + s));
+                    n = max(n, s + 1);
+                    if (++s == slots) {
+                        s = 0;
+                        t ^= 1u;
                     }
                 }
+                slot[is_v] = s;
+                used[is_v] = n;
+                turn[is_v] = t;
             };
             // in the order of the MMAs: K runs two units ahead of V
             #pragma unroll 1
@@ -282,12 +292,16 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         __syncwarp();
         // every copy lands before the CTA gives up its shared memory
         if (*abort)
-            for (int s = 0; s < used; s++)        // the slots before the next one were filled in this round
-                mbar_wait_drain(full(s), s < slot ? turn : turn ^ 1u, status);
-    } else if (warp == 9) {
-        // ---------------------------------------------------------------- MMA
+            for (int v = 0; v < 2; v++)
+                for (int s = 0; s < used[v]; s++)        // the slots before the next one were filled in this round
+                    mbar_wait_drain(full((v ? C::NK : 0) + s), s < slot[v] ? turn[v] : turn[v] ^ 1u, status);
+    } else if (warp >= 9) {
+        // ---------------------------------------------------------------- MMA: warp 9 the scores, warp 10 the products
+        // Two warps, because one's waits would leave the tensor core without work: a unit's 1,100 clocks of MMAs took
+        // 2,300 with one.
+        const bool products = warp == 10;
         constexpr uint32_t id_s = tc::idesc(1, 0, 0, 0, 0, kUnit, kRowsP);
-        constexpr uint32_t id_o = tc::idesc(1, 0, 0, 0, 1, C::DV, kRowsP);
+        constexpr uint32_t id_o = tc::idesc(1, 0, 0, 0, 1, C::EC, kRowsP);
         int slot = 0;                              // the next entry's
         uint32_t turn = 0;                         // parity of the ring's round
         uint32_t it = 0, piece = 0;                // units and pieces so far
@@ -296,10 +310,10 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             ok = __all_sync(0xffffffffu, ok && wait_short(bar, parity, abort, status));
             tc::fence_after();
         };
-        auto entry = [&]() {                       // the next entry, once it has landed
-            const int s = slot;
+        auto entry = [&]() {                       // the next entry of this warp's ring, once it has landed
+            const int s = (products ? C::NK : 0) + slot;
             wait(full(s), turn);
-            if (++slot == C::NST) {
+            if (++slot == (products ? C::NV : C::NK)) {
                 slot = 0;
                 turn ^= 1u;
             }
@@ -319,8 +333,8 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 const uint64_t kd = k_desc + (uint64_t)(s * (C::ENTRY / 16));
                 if (elect_one()) {
                     #pragma unroll
-                    for (int k = 0; k < C::DV / 16; k++) {
-                        const int e = pe * C::DV + 16 * k;                     // element of the head
+                    for (int k = 0; k < C::EC / 16; k++) {
+                        const int e = pe * C::EC + 16 * k;                     // element of the head
                         const uint64_t bd = kd + (uint64_t)((k / 4) * (kUnit * 128 / 16) + (k % 4) * 2);
                         if (e < C::QT)
                             tc::mma_f16_ts(ds, tmem + C::Q_COL + e / 2, bd, id_s, e > 0);
@@ -334,38 +348,41 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 __syncwarp();
             }
         };
-        while (ok && w.next()) {
-            wait(b_q, piece & 1u);
-            piece++;
-            // two units of scores ahead of the products: their buffers are free as soon as they have been read
-            #pragma unroll 1
-            for (int j = 0; ok && j < w.nu + 2; j++) {
-                if (j < w.nu) scores(it + j);
-                if (j < 2) continue;
-                const int u = j - 2;
-                wait(b_p, (it + u) & 1u);
+        auto product = [&](int u) {
+            wait(b_p, (it + u) & 1u);
+            const int acc = u > 0 || *(volatile int*)&sm.acc;
+            #pragma unroll
+            for (int ve = 0; ve < C::VE; ve++) {
                 const int s = entry();
-                if (!ok) break;
-                const int acc = u > 0 || *(volatile int*)&sm.acc;
+                if (!ok) return;
                 const uint64_t vd = v_desc + (uint64_t)(s * (C::ENTRY / 16));
                 if (elect_one()) {
                     #pragma unroll
-                    for (int k = 0; k < kUnit / 16; k++)      // 16 keys: two groups of 8 rows of 128 bytes
-                        tc::mma_f16_ts(tmem + C::O_COL, tmem + C::P_COL + 8 * k, vd + (uint64_t)(k * (2048 / 16)), id_o,
-                                       acc || k > 0);
+                    for (int k = 0; k < kUnit / 16; k++)  // 16 keys: two groups of 8 rows of 128 bytes
+                        tc::mma_f16_ts(tmem + C::O_COL + ve * C::EC, tmem + C::P_COL + 8 * k, vd + (uint64_t)(k * (2048 / 16)),
+                                       id_o, acc || k > 0);
+                    if (ve == C::VE - 1) tc::commit(b_pv + 8u * ((it + u) & 1u));
                     tc::commit(empty(s));
-                    tc::commit(b_pv + 8u * ((it + u) & 1u));
-                    if (u == w.nu - 1) tc::commit(b_o);
+                    if (ve == C::VE - 1 && u == w.nu - 1) tc::commit(b_o);
                 }
                 __syncwarp();
+            }
+        };
+        while (ok && w.next()) {
+            if (!products) wait(b_q, piece & 1u);
+            piece++;
+            #pragma unroll 1
+            for (int u = 0; ok && u < w.nu; u++) {
+                if (products) product(u);
+                else scores(it + u);               // up to two units ahead: a buffer is free as soon as it has been read
             }
             it += w.nu;
             w.step();
         }
         if (*abort) {
-            if (elect_one()) tc::commit(b_drain);
+            if (elect_one()) tc::commit(b_drain + 8u * products);
             __syncwarp();
-            mbar_wait_drain(b_drain, 0, status);
+            mbar_wait_drain(b_drain + 8u * products, 0, status);
         }
         __syncwarp();
     } else {
@@ -385,7 +402,6 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         };
         const uint32_t stage = stages + warp * C::STAGE;
         uint32_t it = 0, pieces = 0;              // units and pieces so far
-        long long e0 = 0;                         // ring entries of the pieces before
         // A wait that ran out clears ok.  The warp then walks on without waiting, so that the warps meet at
         // the same named barriers to the end; it writes no result.
         bool ok = true;
@@ -642,14 +658,18 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 if (edge) {
                     // Values that no row sees become zeros; values that only some rows see and that are not
                     // finite (0 x NaN is not 0) are added row by row here and then cleared.
-                    const long long ev = e0 + (long long)C::KE * min(u + 3, w.nu) + u;
-                    const int s = (int)(ev % C::NST);
-                    // A barrier's parity tells a phase from the one before only, so the slot's last tenant has to have landed:
-                    // it is at the latest a K entry of the next unit, and that one's scores say so.
-                    if (u + 1 < w.nu) wait(b_s + 8u * (half ^ 1), ((it + 1) >> 1) & 1u);
-                    wait(full(s), (uint32_t)(ev / C::NST) & 1u);
+                    // (V of the unit before has landed, or its product were not done: the parity is this phase's.)
+                    uint32_t v_at[C::VE];
+                    #pragma unroll
+                    for (int ve = 0; ve < C::VE; ve++) {
+                        const uint32_t n = it * C::VE + ve, s = C::NK + n % C::NV;
+                        wait(full(s), (n / C::NV) & 1u);
+                        v_at[ve] = ring + s * C::ENTRY;
+                    }
                     // this thread's share: 16 bytes (r0 % 8) of keys r0 / 8 + 16 r in each 64-column chunk
-                    const uint32_t vt = ring + s * C::ENTRY + r0 * 16;
+                    auto piece_at = [&](int c, int r) {
+                        return v_at[c / (C::EC / 64)] + c % (C::EC / 64) * (kUnit * 128) + r * (16 * 128) + r0 * 16;
+                    };
                     uint32_t bad = 0;
                     bool some[4];                            // key r is seen by some rows only
                     #pragma unroll
@@ -659,7 +679,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         some[r] = !none && (k < all_lo || k >= all_hi);
                         #pragma unroll
                         for (int c = 0; c < C::DV / 64; c++) {
-                            const uint32_t at = vt + c * (kUnit * 128) + r * (16 * 128);
+                            const uint32_t at = piece_at(c, r);
                             if (none) {
                                 st_shared(at, make_uint4(0, 0, 0, 0));
                             } else if (some[r]) {
@@ -674,7 +694,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         group_sync();
                         for (int r = 0; r < 4; r++)
                             for (int c = 0; c < C::DV / 64 && some[r]; c++) {
-                                const uint4 v = ld_shared(vt + c * (kUnit * 128) + r * (16 * 128));
+                                const uint4 v = ld_shared(piece_at(c, r));
                                 if ((not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w)) & 0x80008000u)
                                     atomicOr(&sm.odd[half], 1ull << ((r0 >> 3) + 16 * r));
                             }
@@ -703,7 +723,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                                 uint32_t o[32];
                                 tc::ld_32x32b_x32(tl + C::O_COL + c, o);
                                 tc::wait_ld();
-                                const uint32_t vr = ring + s * C::ENTRY + (c / 64) * (kUnit * 128) + j * 128;
+                                const uint32_t vr = v_at[c / C::EC] + (c % C::EC / 64) * (kUnit * 128) + j * 128;
                                 #pragma unroll
                                 for (int q = 0; q < 4; q++) {
                                     const int un = (c % 64) / 8 + q;
@@ -728,7 +748,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         for (int r = 0; r < 4; r++)
                             for (int c = 0; c < C::DV / 64; c++)
                                 if ((odd >> ((r0 >> 3) + 16 * r)) & 1ull)
-                                    st_shared(vt + c * (kUnit * 128) + r * (16 * 128), make_uint4(0, 0, 0, 0));
+                                    st_shared(piece_at(c, r), make_uint4(0, 0, 0, 0));
                     }
                     if (odd || key < any_lo || key + kUnit > min(any_hi, end)) tc::fence_proxy_async_smem();   // V was written
                 }
@@ -748,7 +768,6 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             mine = (size_t)esize * (!direct ? whole ? at_slot * HD + part * C::DV : at_slot * C::DV
                                             : (size_t)tok * a.out_stride + (size_t)hq * HD + part * C::DV);
             pending = true;
-            e0 += (long long)(C::KE + 1) * w.nu;
             w.step();
             more = w.next();
         }
