@@ -714,13 +714,6 @@ __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
-
 template <int HD>
 __global__ void __launch_bounds__(32 * kFewWarps, HD == 512 ? 1 : 2)
 few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -839,12 +832,11 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
             if (!(e & 1)) valid = (valid & ~(1u << (n & 31))) | ((ok ? 1u : 0u) << (n & 31));
             // a page that is not there: past the map's last row, which TMA fills with zeros
             const int row = ok ? at_row : a.num_pages * d.nkv * d.ps;
-            // one box of 64 columns per lane: one instruction of the warp issues the entry
-            const uint32_t bar = bar0 + 8 * eslot;
-            if (lane == 0) mbar_arrive_expect_tx(bar, C::ENTRY);
-            __syncwarp();
-            if (lane < HD / 64)
-                tma_2d(ring + (uint32_t)(eslot * C::ENTRY + lane * (kBlk * 128)), (e & 1) ? &vmap : &kmap, 64 * lane, row, bar);
+            if (lane == 0) {
+                const uint32_t bar = bar0 + 8 * eslot;
+                mbar_arrive_expect_tx(bar, C::ENTRY);
+                tma_chunks(ring + (uint32_t)(eslot * C::ENTRY), (e & 1) ? &vmap : &kmap, row, 0, bar);
+            }
             eslot = eslot + 1 == C::NST ? 0 : eslot + 1;
             issued++;
         };
@@ -1429,8 +1421,7 @@ int g4b_paged_attn(const uint16_t* q, long long q_stride, const uint16_t* kc, co
     CUtensorMap km, vm;
     const uint64_t rows = (uint64_t)num_pages * nkv * page_size;
     for (int i = 0; i < 2; i++) {
-        st = tensor_map_2d(i ? &vm : &km, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, i ? vc : kc, hd, rows, (uint64_t)hd * 2, 64,
-                           kBlk, CU_TENSOR_MAP_SWIZZLE_128B);
+        st = tensor_map_chunks(i ? &vm : &km, i ? vc : kc, hd, rows, kBlk, hd / 64);
         if (st != G4B_OK) return st;
     }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

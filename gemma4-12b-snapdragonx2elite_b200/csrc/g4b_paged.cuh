@@ -135,6 +135,15 @@ __device__ __forceinline__ bool wait_short(uint32_t bar, uint32_t parity, volati
     return mbar_wait(bar, parity, abort, status);
 }
 
+// a box of a tensor_map_chunks map: rows from `row`, 64-element chunks from `chunk`
+__device__ __forceinline__ void tma_chunks(uint32_t dst, const CUtensorMap* map, int row, int chunk, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(chunk), "r"(bar)
+        : "memory");
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

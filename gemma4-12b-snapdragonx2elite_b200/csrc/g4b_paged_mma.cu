@@ -73,12 +73,6 @@ struct ManyCfg {
 
 namespace {
 
-__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
 __device__ __forceinline__ uint32_t ld_tmem_x1(uint32_t taddr) {
     uint32_t v;
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr) : "memory");
@@ -233,12 +227,14 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         bool ok = true;
         while (ok && w.next()) {
             const int head = w.head / C::CS, part = w.head % C::CS;
-            // An entry is EC / 64 column chunks of `boxes` boxes of `box` rows.  Each lane has one box of it: one
-            // instruction of the warp issues them all (one thread's loop over them took longer than the units' MMAs).
+            // A page gives `box` rows of a unit at a time.  One copy brings all of an entry's columns of a V box, and of a
+            // whole K unit; where a unit has several boxes K takes a copy per 64-column chunk as well, so that a
+            // chunk's 64 rows lie together.  Each lane has one copy: a copy's issue takes about 100 clocks.
             const int box = min(d.ps, kUnit), boxes = kUnit / box, lboxes = __ffs(boxes) - 1;
             const int my_p = lane & (boxes - 1), my_c = lane >> lboxes;
-            const bool issues = my_c < C::EC / 64;
-            const uint32_t my_dst = ring + my_c * (kUnit * 128) + my_p * box * 128;
+            const bool k_issues = boxes == 1 ? lane == 0 : my_c < C::EC / 64, v_issues = lane < boxes;
+            const uint32_t k_dst = ring + my_c * (kUnit * 128) + my_p * box * 128;
+            const uint32_t v_dst = ring + my_p * box * (C::EC * 2);
             int ids = -1, ids_at = -64;
             bool ids_pre = false;
             // unit u of the piece: K (all of hd) or V (this walk's columns)
@@ -267,9 +263,9 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     if (!ok) break;
                     if (lane == 0) mbar_arrive_expect_tx(full(first + s), C::ENTRY);
                     __syncwarp();
-                    if (issues)
-                        tma_box(my_dst + (first + s) * C::ENTRY, is_v ? &vmap : &kmap, x0 + e * C::EC + 64 * my_c, row,
-                                full(first + s));
+                    if (is_v ? v_issues : k_issues)
+                        tma_chunks((is_v ? v_dst : k_dst) + (first + s) * C::ENTRY, is_v ? &vmap : &kmap, row,
+                                   (x0 + e * C::EC) / 64 + (is_v ? 0 : my_c), full(first + s));
                     n = max(n, s + 1);
                     if (++s == slots) {
                         s = 0;
@@ -321,7 +317,13 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         };
         // A descriptor's address field counts 16 bytes and has room for all of shared memory: the descriptors of an
         // entry's tiles are its first one's plus a constant.
-        const uint64_t k_desc = tc::sdesc_sw128(ring, 16, 1024), v_desc = tc::sdesc_sw128(ring, kUnit * 128, 1024);
+        // V lies box by box: chunks of `box` rows, 16 keys (two groups of 8 rows of 128 bytes) at a time.
+        const int box = min(d.ps, kUnit);
+        const uint64_t k_desc = tc::sdesc_sw128(ring, 16, 1024), v_desc = tc::sdesc_sw128(ring, box * 128, 1024);
+        uint32_t v_off[kUnit / 16];
+        #pragma unroll
+        for (int k = 0; k < kUnit / 16; k++)
+            v_off[k] = (uint32_t)((16 * k) / box * box * (C::EC * 2) + (16 * k) % box * 128) / 16;
         const uint64_t q_desc = tc::sdesc_sw128(qs, 16, 1024);
         auto scores = [&](uint32_t i) {            // i: units before this one, all pieces'
             if (i >= 2) wait(b_read + 8u * (i & 1u), ((i >> 1) - 1) & 1u);     // its buffer's last scores have been read
@@ -358,9 +360,8 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 const uint64_t vd = v_desc + (uint64_t)(s * (C::ENTRY / 16));
                 if (elect_one()) {
                     #pragma unroll
-                    for (int k = 0; k < kUnit / 16; k++)  // 16 keys: two groups of 8 rows of 128 bytes
-                        tc::mma_f16_ts(tmem + C::O_COL + ve * C::EC, tmem + C::P_COL + 8 * k, vd + (uint64_t)(k * (2048 / 16)),
-                                       id_o, acc || k > 0);
+                    for (int k = 0; k < kUnit / 16; k++)
+                        tc::mma_f16_ts(tmem + C::O_COL + ve * C::EC, tmem + C::P_COL + 8 * k, vd + v_off[k], id_o, acc || k > 0);
                     if (ve == C::VE - 1) tc::commit(b_pv + 8u * ((it + u) & 1u));
                     tc::commit(empty(s));
                     if (ve == C::VE - 1 && u == w.nu - 1) tc::commit(b_o);
@@ -667,9 +668,11 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         v_at[ve] = ring + s * C::ENTRY;
                     }
                     // this thread's share: 16 bytes (r0 % 8) of keys r0 / 8 + 16 r in each 64-column chunk
-                    auto piece_at = [&](int c, int r) {
-                        return v_at[c / (C::EC / 64)] + c % (C::EC / 64) * (kUnit * 128) + r * (16 * 128) + r0 * 16;
+                    auto key_at = [&](int c, int k) {        // key k's 128 bytes of chunk c
+                        return v_at[c / (C::EC / 64)] + (k & ~(box - 1)) * (C::EC * 2) + c % (C::EC / 64) * box * 128 +
+                               (k & (box - 1)) * 128;
                     };
+                    auto piece_at = [&](int c, int r) { return key_at(c, (r0 >> 3) + 16 * r) + (r0 & 7) * 16; };
                     uint32_t bad = 0;
                     bool some[4];                            // key r is seen by some rows only
                     #pragma unroll
@@ -723,7 +726,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                                 uint32_t o[32];
                                 tc::ld_32x32b_x32(tl + C::O_COL + c, o);
                                 tc::wait_ld();
-                                const uint32_t vr = v_at[c / C::EC] + (c % C::EC / 64) * (kUnit * 128) + j * 128;
+                                const uint32_t vr = key_at(c / 64, j);
                                 #pragma unroll
                                 for (int q = 0; q < 4; q++) {
                                     const int un = (c % 64) / 8 + q;
@@ -792,8 +795,8 @@ int launch_many(const Args& a, cudaStream_t s) {
     CUtensorMap km, vm;
     const uint64_t rows = (uint64_t)a.num_pages * a.d.nkv * a.d.ps;
     for (int i = 0; i < 2; i++) {
-        const int st = tensor_map_2d(i ? &vm : &km, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, i ? a.vc : a.kc, a.d.hd, rows,
-                                     (uint64_t)a.d.hd * 2, 64, a.d.ps < kUnit ? a.d.ps : kUnit, CU_TENSOR_MAP_SWIZZLE_128B);
+        const int box = a.d.ps < kUnit ? a.d.ps : kUnit, chunks = (a.d.hd == 256 ? 256 : 128) / 64;   // of an entry
+        const int st = tensor_map_chunks(i ? &vm : &km, i ? a.vc : a.kc, a.d.hd, rows, box, i || box == kUnit ? chunks : 1);
         if (st != G4B_OK) return st;
     }
     const cudaError_t e = a.d.hd == 128 ? launch<128>(a, km, vm, s)
