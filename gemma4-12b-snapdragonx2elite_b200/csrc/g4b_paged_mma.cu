@@ -14,7 +14,7 @@
 // to 2^-18 of the maximum out of f16's subnormals).
 // K and V units come by TMA through one ring of 64-key buffers, issued ahead across pieces.
 //
-// Warps: 0-7 softmax, the mask, the rows' Q and the result; 8 TMA; 9 and 10 MMA issue.
+// Warps: 0-7 softmax, the mask, the rows' Q and the result; 8 and 11 the copies of K and V; 9 and 10 the MMAs.
 // Tensor memory's 512 columns: O 256, S 128, P 32 and the first 192 elements of Q; its others are in shared memory.  At hd
 // 512 O alone would fill them, so a tile is walked once for each half of the output columns (the scores are made twice).
 //
@@ -30,7 +30,7 @@ __device__ unsigned g_status_paged_mma;
 
 constexpr int kGroup = 128;             // softmax threads of a group: one per row
 constexpr int kSoft = 2 * kGroup;       // two groups
-constexpr int kManyThreads = kSoft + 96;    // and a warp each for TMA, scores and products
+constexpr int kManyThreads = kSoft + 128;   // and a warp each for K's copies, V's, the scores and the products
 constexpr float kLift = 4.f;            // log2 of the weight that a row's maximum gets when its base is set
 constexpr float kMost = 15.f;           // log2 of the largest weight before the base is set anew (f16: below 2^16)
 
@@ -220,78 +220,65 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
     unsigned* status = &g_status_paged_mma;
     const int pl = h->prefix_len, G = d.G;
 
-    if (warp == 8) {
-        // ---------------------------------------------------------------- TMA
-        int slot[2] = {0, 0}, used[2] = {0, 0};   // of K's and V's ring: the next slot; slots that were ever filled
-        uint32_t turn[2] = {0, 0};                // parity of the ring's round
+    if (warp == 8 || warp == 11) {
+        // ---------------------------------------------------------------- TMA: warp 8 K, warp 11 V
+        // (One warp for both took 1.3 us a unit, most of it issue and lookup latency: longer than the unit's MMAs.)
+        const bool is_v = warp == 11;
+        const int first = is_v ? C::NK : 0, slots = is_v ? C::NV : C::NK, entries = is_v ? C::VE : C::KE;
+        const CUtensorMap* map = is_v ? &vmap : &kmap;
+        int slot = 0, used = 0;                   // the ring's next slot; slots that were ever filled
+        uint32_t turn = 0;                        // parity of the ring's round
         bool ok = true;
+        // A page gives `box` rows of a unit at a time.  One copy brings all of an entry's columns of a V box, and of a
+        // whole K unit; where a unit has several boxes K takes a copy per 64-column chunk as well, so that a chunk's
+        // 64 rows lie together.  Each lane has one copy.
+        const int box = min(d.ps, kUnit), boxes = kUnit / box, lboxes = __ffs(boxes) - 1;
+        const int my_p = lane & (boxes - 1), my_c = is_v ? 0 : lane >> lboxes;
+        const bool issues = is_v || boxes == 1 ? lane < boxes : my_c < C::EC / 64;
+        const uint32_t my_dst = ring + first * C::ENTRY + (is_v ? my_p * box * (C::EC * 2) : my_c * (kUnit * 128) + my_p * box * 128);
         while (ok && w.next()) {
-            const int head = w.head / C::CS, part = w.head % C::CS;
-            // A page gives `box` rows of a unit at a time.  One copy brings all of an entry's columns of a V box, and of a
-            // whole K unit; where a unit has several boxes K takes a copy per 64-column chunk as well, so that a
-            // chunk's 64 rows lie together.  Each lane has one copy: a copy's issue takes about 100 clocks.
-            const int box = min(d.ps, kUnit), boxes = kUnit / box, lboxes = __ffs(boxes) - 1;
-            const int my_p = lane & (boxes - 1), my_c = lane >> lboxes;
-            const bool k_issues = boxes == 1 ? lane == 0 : my_c < C::EC / 64, v_issues = lane < boxes;
-            const uint32_t k_dst = ring + my_c * (kUnit * 128) + my_p * box * 128;
-            const uint32_t v_dst = ring + my_p * box * (C::EC * 2);
-            int ids = -1, ids_at = -64;
+            const int head = w.head / C::CS, chunk0 = (is_v ? w.head % C::CS * C::DV / 64 : 0) + my_c;
+            int ids = -1, ids_at = -64;           // 32 page ids from ids_at on, a lane each
             bool ids_pre = false;
-            // unit u of the piece: K (all of hd) or V (this walk's columns)
-            auto load = [&](int u, bool is_v) {
+            #pragma unroll 1
+            for (int u = 0; u < w.nu && ok; u++) {
                 const Unit un = unit_of(w.t, w.unit + u);
-                const int key = un.key, last = (key + kUnit - 1) >> d.lps;
-                if (un.pre != ids_pre || (key >> d.lps) < ids_at || last >= ids_at + 32) {
-                    // 32 page ids ahead; from two units before on, whose V may still be to come
+                const int page0 = un.key >> d.lps, last = (un.key + kUnit - 1) >> d.lps;
+                if (un.pre != ids_pre || last >= ids_at + 32) {
                     const int* table = un.pre ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
                     ids_pre = un.pre;
-                    ids_at = max(0, key - 2 * kUnit) >> d.lps;
+                    ids_at = page0;
                     ids = ids_at + lane < (un.pre ? d.pre_pages : d.own_pages) ? __ldg(table + ids_at + lane) : -1;
                 }
-                const int k = key + my_p * box;
+                const int k = un.key + my_p * box;
                 const int id = __shfl_sync(0xffffffffu, ids, (k >> d.lps) - ids_at);
                 const int at_row = cache_row(id, a.num_pages, d.nkv, d.lps, head, k);
                 const int row = at_row < 0 ? a.num_pages * d.nkv * d.ps : at_row;   // past the map: zeros
-                const int first = is_v ? C::NK : 0, slots = is_v ? C::NV : C::NK, x0 = is_v ? part * C::DV : 0;
-                int s = slot[is_v], n = used[is_v];
-                uint32_t t = turn[is_v];
                 #pragma unroll 1
-                for (int e = 0; e < (is_v ? C::VE : C::KE); e++) {
+                for (int e = 0; e < entries; e++) {
                     // from the second round on: the slot's MMAs of the round before are done
-                    if (n == slots)
-                        ok = __all_sync(0xffffffffu, wait_short(empty(first + s), t ^ 1u, abort, status));
+                    if (used == slots)
+                        ok = __all_sync(0xffffffffu, wait_short(empty(first + slot), turn ^ 1u, abort, status));
                     if (!ok) break;
-                    if (lane == 0) mbar_arrive_expect_tx(full(first + s), C::ENTRY);
+                    if (lane == 0) mbar_arrive_expect_tx(full(first + slot), C::ENTRY);
                     __syncwarp();
-                    if (is_v ? v_issues : k_issues)
-                        tma_chunks((is_v ? v_dst : k_dst) + (first + s) * C::ENTRY, is_v ? &vmap : &kmap, row,
-                                   (x0 + e * C::EC) / 64 + (is_v ? 0 : my_c), full(first + s));
-                    n = max(n, s + 1);
-                    if (++s == slots) {
-                        s = 0;
-                        t ^= 1u;
+                    if (issues)
+                        tma_chunks(my_dst + slot * C::ENTRY, map, row, chunk0 + e * (C::EC / 64), full(first + slot));
+                    used = max(used, slot + 1);
+                    if (++slot == slots) {
+                        slot = 0;
+                        turn ^= 1u;
                     }
                 }
-                slot[is_v] = s;
-                used[is_v] = n;
-                turn[is_v] = t;
-            };
-            // in the order of the MMAs: K runs two units ahead of V
-            #pragma unroll 1
-            for (int i = 0; i < 2 * (w.nu + 2) && ok; i++) {
-                const bool is_v = i & 1;
-                const int u = (i >> 1) - (is_v ? 2 : 0);
-                if (u >= 0 && u < w.nu) load(u, is_v);
             }
             w.step();
         }
         __syncwarp();
         // every copy lands before the CTA gives up its shared memory
         if (*abort)
-            for (int v = 0; v < 2; v++)
-                for (int s = 0; s < used[v]; s++)        // the slots before the next one were filled in this round
-                    mbar_wait_drain(full((v ? C::NK : 0) + s), s < slot[v] ? turn[v] : turn[v] ^ 1u, status);
-    } else if (warp >= 9) {
+            for (int s = 0; s < used; s++)        // the slots before the next one were filled in this round
+                mbar_wait_drain(full(first + s), s < slot ? turn : turn ^ 1u, status);
+    } else if (warp == 9 || warp == 10) {
         // ---------------------------------------------------------------- MMA: warp 9 the scores, warp 10 the products
         // Two warps, because one's waits would leave the tensor core without work: a unit's 1,100 clocks of MMAs took
         // 2,300 with one.
