@@ -114,17 +114,16 @@ int check_device(int* sm_count) {
 struct TmapKey {
     uintptr_t base;
     uint64_t dim0, dim1, stride1;
-    uint32_t box0, box1, dtype, swizzle, promo, box2 = 0;   // box2: of tensor_map_chunks, 0 for a 2-D map
+    uint32_t box0, box1, dtype, swizzle, promo;
     bool operator==(const TmapKey& o) const {
         return base == o.base && dim0 == o.dim0 && dim1 == o.dim1 && stride1 == o.stride1 && box0 == o.box0 &&
-               box1 == o.box1 && dtype == o.dtype && swizzle == o.swizzle && promo == o.promo &&
-               box2 == o.box2;
+               box1 == o.box1 && dtype == o.dtype && swizzle == o.swizzle && promo == o.promo;
     }
 };
 struct TmapKeyHash {
     size_t operator()(const TmapKey& k) const {
         size_t h = std::hash<uint64_t>()(k.base);
-        for (uint64_t v : {k.dim0, k.dim1, k.stride1, (uint64_t)k.box0 << 32 | k.box1, (uint64_t)k.box2 << 32 | (uint64_t)k.dtype << 16 | k.swizzle << 8 | k.promo})
+        for (uint64_t v : {k.dim0, k.dim1, k.stride1, (uint64_t)k.box0 << 32 | k.box1, (uint64_t)k.dtype << 16 | k.swizzle << 8 | k.promo})
             h = h * 1000003u ^ std::hash<uint64_t>()(v);
         return h;
     }
@@ -133,32 +132,15 @@ static std::mutex g_tmap_mu;
 static std::unordered_map<TmapKey, CUtensorMap, TmapKeyHash> g_tmaps;
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
-// The map of `key`, from the cache or encoded from the rest.
-static int tensor_map(CUtensorMap* out, const TmapKey& key, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
-                      const cuuint32_t* box) {
-    std::lock_guard<std::mutex> lk(g_tmap_mu);
-    auto it = g_tmaps.find(key);
-    if (it != g_tmaps.end()) {
-        *out = it->second;
-        return G4B_OK;
-    }
-    if (!g_encode) {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
-        if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn)
-            return fail(G4B_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-        g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
-    const cuuint32_t estr[3] = {1, 1, 1};
-    CUtensorMap m;
-    CUresult r = g_encode(&m, (CUtensorMapDataType)key.dtype, rank, reinterpret_cast<void*>(key.base), dims, strides, box,
-                          estr, CU_TENSOR_MAP_INTERLEAVE_NONE, (CUtensorMapSwizzle)key.swizzle,
-                          (CUtensorMapL2promotion)key.promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(G4B_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-    if (g_tmaps.size() > 8192) g_tmaps.clear();
-    g_tmaps.emplace(key, m);
-    *out = m;
+// g_encode, under g_tmap_mu
+static int find_encoder() {
+    if (g_encode) return G4B_OK;
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn)
+        return fail(G4B_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
     return G4B_OK;
 }
 
@@ -167,19 +149,43 @@ int tensor_map_2d(CUtensorMap* out, CUtensorMapDataType dtype, const void* base,
                   CUtensorMapL2promotion promo) {
     TmapKey key{(uintptr_t)base, dim0, dim1, stride1_bytes, box0, box1, (uint32_t)dtype, (uint32_t)swizzle,
                 (uint32_t)promo};
+    std::lock_guard<std::mutex> lk(g_tmap_mu);
+    auto it = g_tmaps.find(key);
+    if (it != g_tmaps.end()) {
+        *out = it->second;
+        return G4B_OK;
+    }
+    const int st = find_encoder();
+    if (st != G4B_OK) return st;
     const cuuint64_t dims[2] = {dim0, dim1};
     const cuuint64_t strides[1] = {stride1_bytes};
     const cuuint32_t box[2] = {box0, box1};
-    return tensor_map(out, key, 2, dims, strides, box);
+    const cuuint32_t estr[2] = {1, 1};
+    CUtensorMap m;
+    CUresult r = g_encode(&m, dtype, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          swizzle, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(G4B_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    if (g_tmaps.size() > 8192) g_tmaps.clear();
+    g_tmaps.emplace(key, m);
+    *out = m;
+    return G4B_OK;
 }
 
 int tensor_map_chunks(CUtensorMap* out, const void* base, uint64_t dim0, uint64_t dim1, uint32_t rows, uint32_t chunks) {
-    TmapKey key{(uintptr_t)base, dim0, dim1, dim0 * 2, 64, rows, (uint32_t)CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                (uint32_t)CU_TENSOR_MAP_SWIZZLE_128B, (uint32_t)CU_TENSOR_MAP_L2_PROMOTION_L2_256B, chunks};
+    {
+        std::lock_guard<std::mutex> lk(g_tmap_mu);
+        const int st = find_encoder();
+        if (st != G4B_OK) return st;
+    }
     const cuuint64_t dims[3] = {64, dim1, dim0 / 64};
     const cuuint64_t strides[2] = {dim0 * 2, 128};
     const cuuint32_t box[3] = {64, rows, chunks};
-    return tensor_map(out, key, 3, dims, strides, box);
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = g_encode(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(G4B_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return G4B_OK;
 }
 
 }  // namespace g4b

@@ -8,6 +8,7 @@
 #include <stdio.h>
 
 #include "g4b.h"
+#include "g4b_overlap.h"
 
 namespace g4b {
 
@@ -48,7 +49,8 @@ int tensor_map_2d(CUtensorMap* out, CUtensorMapDataType dtype, const void* base,
                   uint64_t stride1_bytes, uint32_t box0, uint32_t box1, CUtensorMapSwizzle swizzle,
                   CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 // The same array of f16 rows seen as [dim0 / 64 column chunks][dim1 rows][64]: a box of `chunks` x `rows` x 64 elements
-// lands in shared memory chunk by chunk, 128-byte rows swizzled, where a 2-D map takes a copy per chunk.
+// lands in shared memory chunk by chunk, 128-byte rows swizzled, where a 2-D map takes a copy per chunk.  Encoded anew by
+// every call.
 int tensor_map_chunks(CUtensorMap* out, const void* base, uint64_t dim0, uint64_t dim1, uint32_t rows, uint32_t chunks);
 
 #define G4B_ENTRY(opname)                                  \

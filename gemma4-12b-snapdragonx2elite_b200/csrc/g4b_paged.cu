@@ -55,17 +55,16 @@ static int make_dims(const char* op, int T, int B, int nH, int nkv, int hd, int 
     d.ps = ps;
     d.own_pages = own_pages;
     d.pre_pages = pre_pages;
-    d.window = window;
+    d.window = window < 0x40000000 ? window : 0;     // no position is as far as that from another
     while ((1 << d.lps) < ps) d.lps++;
     d.few = few_most(hd);
     d.cs = hd == 512 ? 2 : 1;
     d.ctas[0] = sms * few_per_sm(hd);
     d.ctas[1] = sms;
     const int rows = T * d.G;
-    const bool many = many_rows(hd);
     // tiles of sequences (one more each for the last, partial one) and of the prefix
-    d.max_tiles[0] = many ? (B + 1) * (d.few / kRowsS) : 2 * (rows / kRowsS) + B + 1;
-    d.max_tiles[1] = many ? 2 * (rows / kRowsP) + B + 1 : 0;
+    d.max_tiles[0] = (B + 1) * (d.few / kRowsS);
+    d.max_tiles[1] = 2 * (rows / kRowsP) + B + 1;
     size_t o = up256(sizeof(Hdr));
     auto take = [&](size_t bytes) {
         const size_t at = o;
@@ -94,7 +93,6 @@ static size_t work_bytes(const Dims& d, char* base, Work* w) {
     };
     Work x{};
     for (int k = 0; k < 2; k++) {
-        if (k == 1 && !many_rows(d.hd)) continue;
         const size_t rows = (size_t)d.ctas[k] * 2 * (k ? kRowsP : kRowsS);
         x.edge[k] = reinterpret_cast<float*>(take(rows * (k ? d.hd / d.cs : d.hd) * 4));
         x.edge_ml[k] = reinterpret_cast<float2*>(take(rows * 8));
@@ -122,7 +120,6 @@ struct PlanArgs {
     const int* prefix_len;
     void* plan;
     Dims d;
-    int many;
 };
 
 __device__ __forceinline__ int seq_of(const int* st, int B, int t) {   // the last b with st[b] <= t
@@ -183,12 +180,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         for (int i = tid; i < B; i += kPlanThreads) len[i] = min(max(__ldg(a.kv_len + i), 0), cap);
     }
     __syncthreads();
+    // position of row t of sequence b; -1 for all before its first (a window's start behind that stays within 32 bits)
+    auto pos_of = [&](int b, int t) { return max(-1, len[b] - st[b + 1] + t); };
     const int r_lo = st[0] * G, r_hi = st[B] * G;
-    const bool pre_many = a.many && r_hi - r_lo > d.few;
+    const bool pre_many = r_hi - r_lo > d.few;
     const int pre_rows = pre_many ? kRowsP : kRowsS;
     const int pre_tiles = pl > 0 ? (r_hi - r_lo + pre_rows - 1) / pre_rows : 0;
     auto alone = [&](int b) { return (st[b + 1] - st[b]) * G > kRowsAlone; };
-    auto many_of = [&](int b) { return a.many && (st[b + 1] - st[b]) * G > d.few; };
+    auto many_of = [&](int b) { return (st[b + 1] - st[b]) * G > d.few; };
     // first tile of each sequence: the prefix's come first
     int nt[2] = {pre_many ? 0 : pre_tiles, pre_many ? pre_tiles : 0};
     for (int i0 = 0; i0 < B; i0 += kPlanThreads) {
@@ -212,14 +211,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         int b = -1, pos = -1;
         if (live) {
             b = seq_of(st, B, t);
-            pos = len[b] - st[b + 1] + t;
+            pos = pos_of(b, t);
         }
         at<int>(a.plan, d.tok_seq)[t] = b;
         at<int>(a.plan, d.tok_pos)[t] = pos;
     }
     for (int r = gtid; r < d.T * G; r += gn) {
         int pre = -1;                // the row's prefix tile: kind in bit 31
-        if (pre_tiles && r >= r_lo && r < r_hi && !(a.many && alone(seq_of(st, B, r / G))))
+        if (pre_tiles && r >= r_lo && r < r_hi && !alone(seq_of(st, B, r / G)))
             pre = (int)((pre_many ? 0x80000000u : 0u) | (unsigned)((r - r_lo) / pre_rows));
         at<int>(a.plan, d.row_pre)[r] = pre;
     }
@@ -237,9 +236,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         int lo = 0x7fffffff, hi = 0;
         for (int b = seq_of(st, B, t0); b < B && st[b] <= t1; b++) {
             const int f = max(t0, st[b]), l = min(t1, st[b + 1] - 1);
-            if (l < f || (a.many && alone(b))) continue;
-            lo = min(lo, first_key(len[b] - st[b + 1] + f));
-            hi = max(hi, len[b] - st[b + 1] + l + 1);
+            if (l < f || alone(b)) continue;
+            lo = min(lo, first_key(pos_of(b, f)));
+            hi = max(hi, pos_of(b, l) + 1);
         }
         t.lo1 = lo / kUnit * kUnit;
         t.hi1 = min(pl, hi);
@@ -274,8 +273,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
                     t.seq = b0;
                     t.row0 = st[b0] * G + lr;
                     t.nrows = min(br, (st[b0 + 1] - st[b0]) * G - lr);
-                    const int p0 = len[b0] - st[b0 + 1] + t.row0 / G;
-                    const int p1 = len[b0] - st[b0 + 1] + (t.row0 + t.nrows - 1) / G;
+                    const int p0 = pos_of(b0, t.row0 / G), p1 = pos_of(b0, (t.row0 + t.nrows - 1) / G);
                     t.lo2 = max(0, first_key(p0) - pl) / kUnit * kUnit;
                     t.hi2 = p1 + 1 - pl;
                     t.n = max(0, (t.hi2 - t.lo2 + kUnit - 1) / kUnit);
@@ -506,6 +504,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
 // both ends of a rotation are its own.
 // head warps of a CTA, by what their registers leave room for twice per SM
 constexpr int stream_warps(int hd) { return hd == 512 ? 8 : 16; }
+constexpr int kStreamSmem = 110 * 1024;     // its ring: two CTAs' fit an SM
 
 template <int N, bool F32>
 __device__ __forceinline__ void lds_n(uint32_t at, float* v) {   // N = 2, 4, 8 elements
@@ -613,8 +612,8 @@ __global__ void __launch_bounds__(32 * (stream_warps(HD) + 1), HD == 512 ? 1 : 2
                 turn ^= 1u;
             }
         }
-        if (*abort)                  // what is in flight lands before the CTA gives up its shared memory
-            for (int k = 0; k < used; k++) mbar_wait_drain(full(k), k < s ? turn : turn ^ 1u, &g_status_paged);
+        // what is in flight lands before the CTA gives up its shared memory, whoever gives up waiting for it
+        for (int k = 0; k < used; k++) mbar_wait_drain(full(k), k < s ? turn : turn ^ 1u, &g_status_paged);
         return;
     }
     const int heads = d.nH + 2 * d.nkv;
@@ -1236,12 +1235,12 @@ template <int HD, bool XF32>
 static cudaError_t launch_append_hd(const AppendArgs& a, int sms, cudaStream_t s) {
     const int heads = a.d.nH + 2 * a.d.nkv, per = kAppendThreads / 32;
     const int bytes = stage_bytes(a.d, XF32 ? 4 : 2);
-    // two CTAs per SM, as many stages as their half of the shared memory holds; a token too wide for two stages takes
+    // as many stages as the ring holds; a token too wide for two stages takes
     // the other kernel, as a batch of few tokens does
-    const int stages = std::min(8, 110 * 1024 / bytes);
+    const int stages = std::min(8, kStreamSmem / bytes);
     if (a.d.T >= 2 * sms && stages >= 2) {
         cudaError_t e = cudaFuncSetAttribute(append_stream_kernel<HD, XF32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             stages * bytes);
+                                             kStreamSmem);
         if (e != cudaSuccess) return e;
         append_stream_kernel<HD, XF32><<<2 * sms, 32 * (stream_warps(HD) + 1), stages * bytes, s>>>(a, stages);
     } else {
@@ -1315,9 +1314,9 @@ int g4b_paged_plan(const int* q_start, const int* kv_len, const int* prefix_len,
     a.kv_len = kv_len;
     a.prefix_len = prefix_pages > 0 ? prefix_len : nullptr;
     a.plan = plan;
-    a.many = many_rows(hd) ? 1 : 0;
+    // (the limit is the same for every call: another thread's may come between it and the launch)
     const int smem = (3 * B + 1) * 4;
-    cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * kMaxSeqs + 1) * 4);
     if (e != cudaSuccess) return fail(G4B_E_CUDA, "paged_plan: %s", cudaGetErrorString(e));
     const int rows = T * a.d.G;
     const int grid = std::min(64, (rows + 4 * kPlanThreads - 1) / (4 * kPlanThreads));
@@ -1352,6 +1351,13 @@ int g4b_paged_append(const void* qkv, int dtype, long long row_stride, const flo
                     aligned16(kc) && aligned16(vc) && aligned16(q_out) && aligned16(plan),
                 G4B_E_ALIGN, "paged_append: qkv, the weights, the rotations, the caches, q_out and the plan must be "
                 "16-byte aligned");
+    const size_t cache = (size_t)num_pages * nkv * page_size * hd * 2, esz = dtype == G4B_DT_F32 ? 4 : 2;
+    const long long last = std::max((long long)nH * hd, std::max(koff, voff) + (long long)nkv * hd);
+    const Rows in{qkv, T, row_stride * (long long)esz, last * (long long)esz}, q{q_out, T, q_stride * 2, (long long)nH * hd * 2};
+    G4B_REQUIRE(!rows_overlap(flat(kc, cache), flat(vc, cache)) && !rows_overlap(q, in) &&
+                    !rows_overlap(q, flat(kc, cache)) && !rows_overlap(q, flat(vc, cache)) &&
+                    !rows_overlap(in, flat(kc, cache)) && !rows_overlap(in, flat(vc, cache)),
+                G4B_E_ARG, "paged_append: kc, vc, q_out and qkv overlap");
     a.plan = plan;
     a.qkv = qkv;
     a.qnw = qnw;
@@ -1403,6 +1409,12 @@ int g4b_paged_attn(const uint16_t* q, long long q_stride, const uint16_t* kc, co
     const size_t need = work_bytes(a.d, nullptr, nullptr);
     G4B_REQUIRE(workspace && aligned16(workspace) && ws_bytes >= need, G4B_E_WORKSPACE,
                 "paged_attn: needs a 16-byte aligned workspace of %zu bytes, got %zu", need, ws_bytes);
+    const size_t cache = (size_t)num_pages * nkv * page_size * hd * 2, osz = out_dtype == G4B_DT_F32 ? 4 : 2;
+    const long long wide = (long long)nH * hd;
+    const Rows to{out, T, out_stride * (long long)osz, wide * (long long)osz};
+    G4B_REQUIRE(!rows_overlap(to, Rows{q, T, q_stride * 2, wide * 2}) && !rows_overlap(to, flat(kc, cache)) &&
+                    !rows_overlap(to, flat(vc, cache)),
+                G4B_E_ARG, "paged_attn: out overlaps q or the caches");
     work_bytes(a.d, reinterpret_cast<char*>(workspace), &a.w);
     a.plan = plan;
     a.q = q;
@@ -1426,7 +1438,7 @@ int g4b_paged_attn(const uint16_t* q, long long q_stride, const uint16_t* kc, co
     }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     // no tile of many rows: neither a sequence nor the prefix has more rows than the batch
-    const bool many = many_rows(hd) && T * a.d.G > a.d.few;
+    const bool many = T * a.d.G > a.d.few;
     if (many) {
         st = launch_many(a, s);
         if (st != G4B_OK) return st;

@@ -150,8 +150,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// the many-rows kernel (g4b_paged_mma.cu): the head widths it has, its launch, its status word
-bool many_rows(int hd);
+// the many-rows kernel (g4b_paged_mma.cu): its launch, its status word
 int launch_many(const Args& a, cudaStream_t s);
 unsigned read_status_paged_mma();
 

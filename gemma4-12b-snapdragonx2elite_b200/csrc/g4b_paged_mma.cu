@@ -275,9 +275,8 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         }
         __syncwarp();
         // every copy lands before the CTA gives up its shared memory
-        if (*abort)
-            for (int s = 0; s < used; s++)        // the slots before the next one were filled in this round
-                mbar_wait_drain(full(first + s), s < slot ? turn : turn ^ 1u, status);
+        for (int s = 0; s < used; s++)            // the slots before the next one were filled in this round
+            mbar_wait_drain(full(first + s), s < slot ? turn : turn ^ 1u, status);
     } else if (warp == 9 || warp == 10) {
         // ---------------------------------------------------------------- MMA: warp 9 the scores, warp 10 the products
         // Two warps, because one's waits would leave the tensor core without work: a unit's 1,100 clocks of MMAs took
@@ -367,11 +366,10 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             it += w.nu;
             w.step();
         }
-        if (*abort) {
-            if (elect_one()) tc::commit(b_drain + 8u * products);
-            __syncwarp();
-            mbar_wait_drain(b_drain + 8u * products, 0, status);
-        }
+        // every MMA is done before the CTA gives up its tensor memory
+        if (elect_one()) tc::commit(b_drain + 8u * products);
+        __syncwarp();
+        mbar_wait_drain(b_drain + 8u * products, 0, status);
         __syncwarp();
     } else {
         // ---------------------------------------------------------------- softmax: two groups
@@ -767,8 +765,6 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
     tc::fence_after();
     if (warp == 9) tc::tmem_dealloc(tmem, 512);
 }
-
-bool many_rows(int hd) { return hd == 128 || hd == 256 || hd == 512; }
 
 template <int HD>
 static cudaError_t launch(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {

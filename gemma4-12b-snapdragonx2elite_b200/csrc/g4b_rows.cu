@@ -410,13 +410,19 @@ int g4b_rows_normadd_i8(const void* x, int x_dtype, const float* w_post, const f
     G4B_REQUIRE(x || !w_post, G4B_E_ARG, "rows_normadd_i8: w_post without x");
     G4B_REQUIRE(!x || dt_ok(x_dtype), G4B_E_ARG, "rows_normadd_i8: bad dtype %d", x_dtype);
     G4B_REQUIRE(M >= 1 && D >= 16 && D % 16 == 0, G4B_E_SHAPE, "rows_normadd_i8: M=%d D=%d (D a multiple of 16)", M, D);
+    const size_t n = (size_t)M * D;
+    G4B_REQUIRE(!h_out || h_out == h || !rows_overlap(flat(h_out, 4 * n), flat(h, 4 * n)), G4B_E_ARG,
+                "rows_normadd_i8: h_out overlaps h without being h");
     const auto aligned32 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; };
     G4B_REQUIRE(aligned32(x) && aligned32(w_post) && aligned32(h) && aligned32(h_out) && aligned32(w) && aligned16(A8) &&
                     ((uintptr_t)sa & 3u) == 0,
                 G4B_E_ALIGN, "rows_normadd_i8: x, the weights, h and h_out must be 32-byte aligned, A8 16-byte, sa 4-byte");
-    const size_t n = (size_t)M * D;
-    G4B_REQUIRE(!h_out || h_out == h || h_out + n <= h || h + n <= h_out, G4B_E_ARG,
-                "rows_normadd_i8: h_out overlaps h without being h");
+    const Rows read[] = {flat(x, n * (x_dtype == G4B_DT_F32 ? 4 : 2)), flat(w_post, 4 * (size_t)D), flat(w, 4 * (size_t)D)};
+    const Rows codes = flat(A8, n), scales = flat(sa, 4 * (size_t)M);
+    bool clash = rows_overlap(codes, scales);
+    for (const Rows& r : {flat(h, 4 * n), flat(h_out, 4 * n)}) clash |= rows_overlap(r, codes) || rows_overlap(r, scales);
+    for (const Rows& r : read) clash |= rows_overlap(r, codes) || rows_overlap(r, scales) || rows_overlap(r, flat(h_out, 4 * n));
+    G4B_REQUIRE(!clash, G4B_E_ARG, "rows_normadd_i8: what it writes overlaps what it reads");
     int sms = 148;
     int st = check_device(&sms);
     if (st != G4B_OK) return st;

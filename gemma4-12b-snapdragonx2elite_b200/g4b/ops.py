@@ -43,6 +43,8 @@ class _on:
     __slots__ = ("dev", "stream")
 
     def __init__(self, index: int, stream: Optional[torch.cuda.Stream]):
+        if stream is not None and stream.device_index != index:
+            raise ValueError(f"the stream is on cuda:{stream.device_index}, the call's tensors on cuda:{index}")
         self.dev = torch.cuda.device(index)
         self.stream = None if stream is None else torch.cuda.stream(stream)
 

@@ -11,7 +11,7 @@ the plan in device memory and the attention's workspace.  A step calls ``update`
 
 The layout of the batch and of the cache is described at "batches over a paged KV cache" in include/g4b.h.
 Every call is stream-ordered and can be captured; calls of one plan must be ordered among themselves, so
-two graphs that may run at once need a plan each.
+two graphs that may run at once need a plan each, and a plan lives at least as long as the graphs that use it.
 """
 from __future__ import annotations
 
@@ -40,6 +40,9 @@ class PagedPlan:
             # a plan of zeros is nobody's: a call before the first update() writes nothing
             self._plan = torch.zeros(plan, dtype=torch.uint8, device=self.device)
             self._ws = torch.empty(ws, dtype=torch.uint8, device=self.device)
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(self.index).synchronize()     # the zeros come before the calls of any stream
+            self._streams = {_raw_stream(self.index)}
         self._plan_ptr, self._ws_ptr, self._ws_bytes = self._plan.data_ptr(), self._ws.data_ptr(), ws
         self._table_shape, self._head_shape = (seqs, table_pages), (hd,)
 
@@ -70,6 +73,15 @@ class PagedPlan:
                 return 0
         return shape[0]
 
+    def _stream(self) -> int:
+        """The current stream's handle; its work is done before the plan's memory serves anything else."""
+        raw = _raw_stream(self.index)
+        if raw not in self._streams:
+            self._streams.add(raw)
+            for t in (self._plan, self._ws):
+                t.record_stream(torch.cuda.current_stream(self.index))
+        return raw
+
     def _elsewhere(self, stream) -> bool:
         return stream is not None or torch.cuda.current_device() != self.index
 
@@ -87,7 +99,7 @@ class PagedPlan:
             self._bad("paged_plan", q_start=q_start, kv_len=kv_len, prefix_len=prefix_len)
         L.check("g4b_paged_plan", self._lib.g4b_paged_plan(
             q_start.data_ptr(), kv_len.data_ptr(), _ptr(prefix_len), *self._sizes, self._plan_ptr, self._plan.numel(),
-            _raw_stream(index)))
+            self._stream()))
 
     def append(self, qkv: torch.Tensor, qnw: torch.Tensor, knw: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                kc: torch.Tensor, vc: torch.Tensor, table: torch.Tensor, koff: int, voff: int,
@@ -114,7 +126,7 @@ class PagedPlan:
         L.check("g4b_paged_append", self._lib.g4b_paged_append(
             qkv.data_ptr(), dtype, step, qnw.data_ptr(), knw.data_ptr(), cos.data_ptr(), sin.data_ptr(), rot[0],
             kc.data_ptr(), vc.data_ptr(), pages, table.data_ptr(), q_out.data_ptr(), q_step, *self._sizes[:5], koff, voff,
-            *self._sizes[5:], self._plan_ptr, _raw_stream(index)))
+            *self._sizes[5:], self._plan_ptr, self._stream()))
         return q_out
 
     def attend(self, q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, table: torch.Tensor,
@@ -139,5 +151,5 @@ class PagedPlan:
             self._bad("paged_attn", q=q, kc=kc, vc=vc, table=table, prefix_table=prefix_table, out=out)
         L.check("g4b_paged_attn", self._lib.g4b_paged_attn(
             q.data_ptr(), step, kc.data_ptr(), vc.data_ptr(), pages, table.data_ptr(), _ptr(prefix_table), out.data_ptr(),
-            dtype, out_step, scale, *self._sizes, self._plan_ptr, self._ws_ptr, self._ws_bytes, _raw_stream(index)))
+            dtype, out_step, scale, *self._sizes, self._plan_ptr, self._ws_ptr, self._ws_bytes, self._stream()))
         return out

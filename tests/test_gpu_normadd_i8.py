@@ -190,3 +190,37 @@ def test_a_batched_layer():
     eps = torch.finfo(y.dtype).eps / 2 + 2.0 ** -22
     assert ((y.to(F64) - ref).abs() <= eps * ref.abs() + 2.0 ** -25).all()
     assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+@pytest.mark.parametrize("D", [256, 3840, 40000])
+def test_rows_that_are_not_finite(D):
+    """A row with a NaN or an infinity: its residual, scale and codes are those of the three calls; the others' too."""
+    h, x, w = torch.randn(5, D, device=DEV), torch.randn(5, D, device=DEV), 1 + 0.1 * torch.randn(D, device=DEV)
+    x[1, 3], h[3, D - 1] = float("nan"), float("inf")
+    h2, h0, x0 = h.clone(), h.clone(), x.clone()
+    a8, sa = ops.rows_normadd_i8(x, h, w, w_post=w)
+    ops.rows_normadd(x, w, h2, 1.0)
+    b8, sb = ops.cast_i8(ops.rows_rmsnorm(h2, w))
+    for r in (1, 3):
+        assert torch.equal(torch.isfinite(h[r]), torch.isfinite(h2[r])) and not torch.isfinite(h[r]).all()
+        assert torch.equal(a8[r], b8[r]) and sa[r] == sb[r]
+    fine = [0, 2, 4]
+    _check(x0[fine], h0[fine], w, w, 1.0, h[fine], a8[fine], sa[fine])
+
+
+def test_captured_and_replayed():
+    M, D = 37, 3840
+    x, h, w = torch.randn(M, D, device=DEV).half(), torch.randn(M, D, device=DEV), 1 + 0.1 * torch.randn(D, device=DEV)
+    out, a8, sa = torch.empty_like(h), torch.empty(M, D, dtype=torch.int8, device=DEV), torch.empty(M, device=DEV)
+    ops.rows_normadd_i8(x, h, w, w_post=w, h_out=out, A8=a8, sa=sa)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.rows_normadd_i8(x, h, w, w_post=w, h_out=out, A8=a8, sa=sa)
+    for k in range(3):
+        h.mul_(-1.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(x, h, w, w, 1.0, out, a8, sa)
+        b8, sb = ops.rows_normadd_i8(x, h, w, w_post=w, h_out=torch.empty_like(h))
+        assert torch.equal(a8, b8) and torch.equal(sa, sb)

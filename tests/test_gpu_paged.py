@@ -480,3 +480,151 @@ def test_two_plans_at_once_on_two_streams():
         a.check(oa, qa)
         b.check(ob, qb)
         assert torch.equal(oa, outs[0][0]) and torch.equal(ob, outs[0][1])    # the same bits every time
+
+
+@pytest.mark.parametrize("nH,nkv,hd,new", [(16, 8, 256, 3), (16, 8, 256, 40), (4, 2, 512, 40), (8, 1, 128, 90)])
+def test_widest_windows_and_positions_below_zero(nH, nkv, hd, new):
+    """A window of 2^31 - 1 keys is none, before a sequence's first position too."""
+    outs = []
+    for window in (0, 2**31 - 1):
+        bt = Batch(nH, nkv, hd, 16, [new, 1], [new, 50], 0, window, seed=30).fill()
+        bt.kv_len[0] = new - 2
+        outs.append(_attend(bt, bt.queries()))
+    assert torch.equal(outs[0], outs[1]) and (outs[0][:2] == 0).all() and (outs[0][2:] != 0).any(-1).all()
+
+
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_as_many_sequences_as_a_plan_takes(prefix):
+    rng = np.random.default_rng(5)
+    new = rng.integers(0, 3, 4096)
+    total = new + prefix + rng.integers(0, 20, 4096)
+    bt = Batch(2, 1, 128, 16, new, total, prefix, seed=31).fill()
+    q = bt.queries()
+    bt.check(_attend(bt, q), q)
+
+
+def test_sequences_that_share_a_page():
+    bt = Batch(16, 8, 256, 32, [1, 2, 20], [70, 66, 90], 0, seed=32)
+    bt.ids[1:, :2] = bt.ids[0, :2]
+    bt.table.copy_(torch.from_numpy(bt.ids))
+    bt.fill()
+    q = bt.queries()
+    bt.check(_attend(bt, q), q)
+
+
+def test_queries_and_results_in_one_buffer():
+    bt = Batch(16, 8, 256, 32, [1, 40, 3], [90, 140, 33], 30, seed=33).fill()
+    wide = torch.cat((bt.queries(), torch.full((bt.T, 4096), 7.0, dtype=torch.float16, device=DEV)), 1)
+    q, out = wide[:, :4096], wide[:, 4096:]
+    before = q.clone()
+    bt.check(_attend(bt, q, out=out), before)
+    assert torch.equal(q, before)
+    with pytest.raises(L.G4BError):
+        _attend(bt, q, out=q)
+
+
+def test_a_plan_made_while_its_stream_is_busy():
+    """What the constructor queues on its own stream is done before another stream's calls."""
+    bt = Batch(16, 8, 256, 64, [1, 1], [65, 90], 0, seed=34).fill()
+    q, side = bt.queries(), torch.cuda.Stream()
+    out = torch.full((bt.T, 4096), 7.0, dtype=torch.float16, device=DEV)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)                           # some 50 ms
+    plan = PagedPlan(bt.T, bt.B, 16, 8, 256, 64, bt.own_pages, 0, 0, DEV)
+    plan.update(bt.q_start, bt.kv_len, stream=side)
+    plan.attend(q, bt.kc, bt.vc, bt.table, out=out, stream=side)
+    torch.cuda.synchronize()
+    bt.check(out, q)
+
+
+def test_a_plan_dropped_while_another_stream_works_with_it():
+    """Its memory serves nothing else before that work is done."""
+    bt = Batch(16, 8, 256, 64, [1] * 30, [900 + i for i in range(30)], 800, seed=35).fill()
+    q, side = bt.queries(), torch.cuda.Stream()
+    plan = bt.plan()
+    out = torch.full((bt.T, 4096), 7.0, dtype=torch.float16, device=DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        plan.attend(q, bt.kc, bt.vc, bt.table, bt.prefix_table, out=out)
+    sizes = plan._plan.numel(), plan._ws.numel()
+    del plan
+    other = [torch.zeros(n, dtype=torch.uint8, device=DEV) for n in sizes]
+    torch.cuda.synchronize()
+    bt.check(out, q)
+    assert all((x == 0).all() for x in other)
+
+
+def test_two_threads_with_other_sizes():
+    """Calls of two host threads whose kernels need different amounts of shared memory."""
+    import threading
+
+    cases = [Batch(4, 2, 256, 16, [150, 150], [150, 150], 0, seed=36),
+             Batch(16, 8, 256, 16, [300] + [0] * 500, [300] * 501, 0, seed=37)]
+    jobs, errors = [], []
+    for bt in cases:
+        nq, nk = bt.nH * bt.hd, bt.nkv * bt.hd
+        w, rot = torch.ones(bt.hd, device=DEV), torch.ones(bt.own_pages * 16, bt.hd, device=DEV)
+        args = (bt.randn(bt.T, nq + 2 * nk), w, w, rot, rot, bt.kc, bt.vc, bt.table, nq, nq + nk)
+        jobs.append((bt, bt.plan(), args, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def run(bt, plan, args, stream):
+        try:
+            for _ in range(200):
+                plan.update(bt.q_start, bt.kv_len, stream=stream)
+                plan.append(*args, stream=stream)
+        except Exception as e:                               # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for bt, _, _, _ in jobs:
+        pg, sl = bt.places(0, bt.total[0])
+        assert torch.isfinite(bt.kc[pg, :, sl]).all() and torch.isfinite(bt.vc[pg, :, sl]).all()
+
+
+@pytest.mark.parametrize("T,hd,nH,nkv", [(6, 256, 16, 8), (320, 128, 8, 1)])
+def test_a_captured_step_of_append_and_attention(T, hd, nH, nkv):
+    """Plan, append, attention in one graph, replayed while the sequences grow: the bits of eager calls."""
+    n = T // 2
+    a, b = (Batch(nH, nkv, hd, 32, [n, n], [400, 400], 20, seed=38) for _ in range(2))
+    nq, nk = nH * hd, nkv * hd
+    qkv = a.randn(a.T, nq + 2 * nk)
+    w = 1 + 0.1 * a.randn(hd)
+    rot = a.randn((a.own_pages + a.pre_pages) * 32, hd)
+    for bt in (a, b):
+        for c in (bt.kc, bt.vc):
+            c.copy_(torch.linspace(-1, 1, c.numel(), device=DEV).half().view(c.shape))
+    out = [torch.empty(a.T, nq, dtype=torch.float16, device=DEV) for _ in range(2)]
+
+    def step(bt, plan, o):
+        plan.update(bt.q_start, bt.kv_len, bt.prefix_len)
+        q = plan.append(qkv, w, w, rot, rot, bt.kc, bt.vc, bt.table, nq, nq + nk)
+        plan.attend(q, bt.kc, bt.vc, bt.table, bt.prefix_table, out=o)
+
+    plans = [a.plan(), b.plan()]
+    step(a, plans[0], out[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(a, plans[0], out[0])
+    for k, total in enumerate(([n + 20, n + 21], [n + 40, n + 20], [n + 100, n + 190])):
+        for bt in (a, b):
+            bt.kv_len.copy_(torch.tensor(total, dtype=torch.int32))
+        qkv.mul_(1.5 - k)
+        graph.replay()
+        if k == 0:                                           # the eager and the warm-up call wrote a's pages only
+            step(b, plans[1], out[1])
+            b.kc.copy_(a.kc)
+            b.vc.copy_(a.vc)
+        step(b, plans[1], out[1])
+        torch.cuda.synchronize()
+        if k:
+            assert torch.equal(out[0], out[1]) and torch.equal(a.kc, b.kc) and torch.equal(a.vc, b.vc)
+    assert L.query(L.Q_KERNEL_STATUS) == 0

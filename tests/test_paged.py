@@ -159,3 +159,78 @@ def test_spans_cover_the_line_of_work(host):
                 host.span(off, int(k), u, o.ctypes.data)
                 assert o[0] == owner[off] and o[1] == owner[off + k - 1] and o[1] < ctas
             off += int(k)
+
+
+@pytest.fixture(scope="module")
+def overlap(tmp_path_factory):
+    d = tmp_path_factory.mktemp("overlap")
+    src, so = d / "overlap.cpp", d / "overlap.so"
+    src.write_text('#include "g4b_overlap.h"\nextern "C" int overlap(long long p, long long n, long long s, long long w, '
+                   "long long q, long long m, long long t, long long v) { return g4b::rows_overlap("
+                   "{reinterpret_cast<void*>(p), n, s, w}, {reinterpret_cast<void*>(q), m, t, v}); }\n")
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-I", CSRC, str(src), "-o", str(so)], check=True)
+    lib = C.CDLL(str(so))
+    lib.overlap.argtypes = [C.c_longlong] * 8
+    return lib.overlap
+
+
+def test_overlap_of_rows(overlap):
+    """Against the sets of bytes, for buffers of one stride; differing strides may only err towards an overlap."""
+    rng = np.random.default_rng(1)
+    seen = set()
+    for _ in range(4000):
+        n, m, s, t = (int(x) for x in rng.integers(1, 6, 4))
+        s, t = 8 * s, 8 * (s if rng.random() < 0.7 else t)
+        w, v = int(rng.integers(1, s + 1)), int(rng.integers(1, t + 1))
+        p, q = (int(x) for x in 100 + rng.integers(0, 120, 2))
+        a = {p + i * s + j for i in range(n) for j in range(w)}
+        b = {q + i * t + j for i in range(m) for j in range(v)}
+        got = overlap(p, n, s, w, q, m, t, v)
+        assert got == bool(a & b) if s == t else got >= bool(a & b), (p, n, s, w, q, m, t, v)
+        seen.add((s == t, got))
+    assert len(seen) == 4
+    assert not overlap(0, 1, 8, 8, 0, 1, 8, 8)               # a buffer that is not given
+
+
+FAR = 1 << 40      # addresses that nothing reads: a call that is refused launches nothing
+
+
+def test_buffers_that_overlap_are_refused():
+    lib, s = L.load(), _sizes(prefix_pages=0)
+    q, kc, vc, out, ws = FAR, FAR + (1 << 32), FAR + (2 << 32), FAR + (3 << 32), FAR + (4 << 32)
+
+    def attn(q=q, kc=kc, vc=vc, out=out, out_dtype=1, stride=4096):
+        return lib.g4b_paged_attn(q, stride, kc, vc, 8, FAR, None, out, out_dtype, stride, 1.0, *s, FAR, ws, 1 << 40, None)
+
+    for bad in (dict(out=q), dict(out=q + 2 * 4096), dict(out=kc + 4096), dict(out=vc - 64), dict(out=q - 64),
+                dict(out=q + 4096, stride=8192), dict(out=q + 2 * 4096, stride=8192, out_dtype=0)):
+        assert attn(**bad) == L.G4B_E_ARG, bad
+        assert "overlap" in L.last_error()
+
+    def append(qkv=q, kc=kc, vc=vc, q_out=out):
+        return lib.g4b_paged_append(qkv, 1, 8192, ws, ws, ws, ws, 384, kc, vc, 8, ws, q_out, 4096, *s[:5], 4096, 6144,
+                                    *s[5:], ws, None)
+
+    for bad in (dict(vc=kc), dict(vc=kc + 64), dict(q_out=q), dict(q_out=kc), dict(qkv=vc + 128)):
+        assert append(**bad) == L.G4B_E_ARG, bad
+        assert "overlap" in L.last_error()
+
+
+def test_normadd_i8_refuses_buffers_that_overlap():
+    x, h, w, h_out, a8, sa = (FAR + (i << 32) for i in range(6))
+    M, D = 4, 256
+    good = dict(x=x, w_post=w + 4096, h=h, h_out=h_out, w=w, a8=a8, sa=sa)
+    for bad in (dict(x=h_out), dict(x=h, h_out=h), dict(w=h_out + 64), dict(w_post=h_out), dict(a8=h), dict(a8=x + 32),
+                dict(sa=a8 + 64), dict(sa=w), dict(a8=h_out + 4 * M * D - 32), dict(h_out=h + 32)):
+        p = dict(good, **bad)
+        assert L.load().g4b_rows_normadd_i8(p["x"], 1, p["w_post"], p["h"], p["h_out"], 1.0, p["w"], p["a8"], p["sa"], M, D,
+                                            None) == L.G4B_E_ARG, bad
+        assert "overlap" in L.last_error()
+
+
+def test_a_stream_of_another_device_is_refused():
+    from types import SimpleNamespace
+
+    from g4b import ops
+    with pytest.raises(ValueError, match="cuda:1"):
+        ops._on(0, SimpleNamespace(device_index=1))
