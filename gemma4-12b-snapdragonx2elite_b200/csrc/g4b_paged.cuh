@@ -135,6 +135,20 @@ __device__ __forceinline__ bool wait_short(uint32_t bar, uint32_t parity, volati
     return mbar_wait(bar, parity, abort, status);
 }
 
+// The same for a whole warp in little code: a loop's waits with the timer inlined spread it over so many cache lines of
+// instructions that a wait already over cost 290 clocks.  Bounded by its tries: each takes 40 clocks (0.08 s in all) to as
+// long as the hardware holds a warp back.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort, unsigned* status) {
+    #pragma unroll 1
+    for (int i = 0; i < 1 << 22; i++) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if ((i & 255) == 255 && __any_sync(0xffffffffu, *abort)) return false;
+    }
+    *abort = 1;
+    atomicOr(status, kStatusTimeout);
+    return false;
+}
+
 // a box of a tensor_map_chunks map: rows from `row`, 64-element chunks from `chunk`
 __device__ __forceinline__ void tma_chunks(uint32_t dst, const CUtensorMap* map, int row, int chunk, uint32_t bar) {
     asm volatile(

@@ -258,7 +258,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 for (int e = 0; e < entries; e++) {
                     // from the second round on: the slot's MMAs of the round before are done
                     if (used == slots)
-                        ok = __all_sync(0xffffffffu, wait_short(empty(first + slot), turn ^ 1u, abort, status));
+                        ok = wait_warp(empty(first + slot), turn ^ 1u, abort, status);
                     if (!ok) break;
                     if (lane == 0) mbar_arrive_expect_tx(full(first + slot), C::ENTRY);
                     __syncwarp();
@@ -289,7 +289,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         uint32_t it = 0, piece = 0;                // units and pieces so far
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, ok && wait_short(bar, parity, abort, status));
+            ok = ok && wait_warp(bar, parity, abort, status);
             tc::fence_after();
         };
         auto entry = [&]() {                       // the next entry of this warp's ring, once it has landed
@@ -337,11 +337,14 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             }
         };
         auto product = [&](int u) {
-            wait(b_p, (it + u) & 1u);
-            const int acc = u > 0 || *(volatile int*)&sm.acc;
+            int acc = 1;
             #pragma unroll
             for (int ve = 0; ve < C::VE; ve++) {
-                const int s = entry();
+                const int s = entry();             // (V is there long before the weights: that wait comes first)
+                if (ve == 0) {
+                    wait(b_p, (it + u) & 1u);
+                    if (u == 0) acc = *(volatile int*)&sm.acc;
+                }
                 if (!ok) return;
                 const uint64_t vd = v_desc + (uint64_t)(s * (C::ENTRY / 16));
                 if (elect_one()) {
@@ -392,7 +395,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         // the same named barriers to the end; it writes no result.
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, ok && wait_short(bar, parity, abort, status));
+            ok = ok && wait_warp(bar, parity, abort, status);
         };
         // The product of a unit is added, waited for by the next unit's group.  (A parity tells a barrier's phase from the
         // one before only: with a barrier for each group's units, none is skipped.)
@@ -604,26 +607,13 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 if (it > 0) wait(b_base + 8u * (half ^ 1), ((it - 1) >> 1) & 1u);
                 const float from = u > 0 ? sm.base[half ^ 1][r0] : -INFINITY;
                 if (m != from && l != 0.f) l *= exp2_approx(m - from);
-                const bool set = u == 0 || top > from + kMost, scale = set && from != -INFINITY;
+                // A warp that has a row to rescale takes the base after every row's maximum that has grown: it is the warp
+                // that pays, and this way seldom twice.
+                const bool any = __any_sync(0xffffffffu, top > from + kMost && from != -INFINITY);
+                const bool set = u == 0 || from == -INFINITY || (any && top > from + kLift), scale = set && from != -INFINITY;
                 m = set ? top - kLift : from;
                 sm.base[half][r0] = m;
                 arrive(b_base + 8u * half);
-                bool added = u == 0;  // the unit before is in O, and its P may be written over
-                if (__any_sync(0xffffffffu, scale)) {
-                    const float f = scale ? exp2_approx(from - m) : 1.f;
-                    l *= f;
-                    wait_pv(it - 1);
-                    added = true;
-                    #pragma unroll 1
-                    for (int c = 0; c < C::DV; c += 32) {
-                        uint32_t o[32];
-                        tc::ld_32x32b_x32(tl + C::O_COL + c, o);
-                        tc::wait_ld();
-                        #pragma unroll
-                        for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                        tc::st_32x32b_x32(tl + C::O_COL + c, o);
-                    }
-                }
                 const float base = m == -INFINITY ? 0.f : m;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
                 #pragma unroll
@@ -636,10 +626,29 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         const __half2 h2 = __floats2half2_rn(e0x, e1x);
                         x[0][16 * k + j] = *reinterpret_cast<const uint32_t*>(&h2);   // P over the scores it is made of
                     }
+                if (scale) l *= exp2_approx(from - m);
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                if (u == 0 && it > 0) wait_pv(it - 1);     // of the piece before: done, but its phase is counted
-                else if (!added) wait_pv(it - 1);
+                // The unit before is in O, and its P may be written over.  (Behind a piece's first unit it is the piece before's:
+                // done, but its phase is counted.)
+                if (it > 0) wait_pv(it - 1);
                 tc::st_32x32b_x32(tl + C::P_COL, x[0]);
+                if (any) {
+                    // the next 32 columns come while these are stored
+                    const float f = scale ? exp2_approx(from - m) : 1.f;
+                    uint32_t o[2][32];
+                    tc::ld_32x32b_x32(tl + C::O_COL, o[0]);
+                    #pragma unroll 1
+                    for (int c = 0; c < C::DV; c += 64) {
+                        #pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            tc::wait_ld();
+                            if (k == 0 || c + 64 < C::DV) tc::ld_32x32b_x32(tl + C::O_COL + c + 32 * (k + 1), o[k ^ 1]);
+                            #pragma unroll
+                            for (int j = 0; j < 32; j++) o[k][j] = __float_as_uint(__uint_as_float(o[k][j]) * f);
+                            tc::st_32x32b_x32(tl + C::O_COL + c + 32 * k, o[k]);
+                        }
+                    }
+                }
                 if (u == 0 && r0 == 0) *(volatile int*)&sm.acc = 0;
                 if (edge) {
                     // Values that no row sees become zeros; values that only some rows see and that are not
