@@ -51,7 +51,9 @@ struct ManyCfg {
     // the shared part of Q, which is idle then
     static constexpr int STAGE = 32 * 128;
     static constexpr bool STAGE_IN_Q = HD == 512;
-    static constexpr int BUF = NST * ENTRY + QS_BYTES + (STAGE_IN_Q ? 0 : 8 * STAGE);
+    // at hd 256 the first group has a second one each, for its second chunk of Q
+    static constexpr int STAGES = HD == 256 ? 12 : 8;
+    static constexpr int BUF = NST * ENTRY + QS_BYTES + (STAGE_IN_Q ? 0 : STAGES * STAGE);
     static constexpr int O_COL = 0, S_COL = DV, P_COL = S_COL + 2 * kUnit, Q_COL = P_COL + kUnit / 2;
     static_assert(Q_COL + QT / 2 <= 512, "tensor memory columns");
     // (the stages are the last two 64-element chunks of Q's shared part, which are written last)
@@ -389,7 +391,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
-        const uint32_t stage = stages + warp * C::STAGE;
+        const uint32_t stage = stages + (C::STAGES == 12 && half == 0 ? 2 * warp : C::STAGES - 8 + warp) * C::STAGE;
         uint32_t it = 0, pieces = 0;              // units and pieces so far
         // A wait that ran out clears ok.  The warp then walks on without waiting, so that the warps meet at
         // the same named barriers to the end; it writes no result.
@@ -403,60 +405,71 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             wait(b_pv + 8u * (unit & 1u), (unit >> 1) & 1u);
             tc::fence_after();
         };
-        // Q of the piece that w stands at
+        // Q of the piece that w stands at: its rows into tensor memory (two elements per column) and, past QT, shared
+        // memory.  All that has a place at once is on its way at once (a chunk after the other took 1,650 clocks each).
+        // Eight lanes read 128 bytes of a row; a stage turns rows over lanes into a row per lane.
         unsigned alive = 0;      // this warp's rows that the piece is for: a prefix tile may span rows that are not
-        auto load_q = [&]() {
-            const int row = w.t.row0 + min(r0, w.t.nrows - 1);
-            alive = __ballot_sync(0xffffffffu, r0 < w.t.nrows &&
-                                                   (w.t.seq >= 0 || __ldg(at<int>(a.plan, d.row_pre) + row) != -1));
-            // Q's rows into tensor memory (two elements per column) and, past QT, shared memory.  Eight lanes read 128
-            // bytes of a row; the stage turns rows over lanes into a row per lane.
-            {
-                const long long mine = ((long long)(row / G) * a.q_stride + (long long)((w.head / C::CS) * G + row % G) * HD) * 2;
-                const char* qb = reinterpret_cast<const char*>(a.q) + (lane & 7) * 16;
-                // chunk c: 64 elements.  A loop that stays one: code that runs once comes from memory as slowly as data
-                // does, and two chunks' loads at once cost more in instructions than they hid.
-                constexpr int NC = HD / 128;                   // chunks of this half
+        auto load_q = [&](int row) {
+            const long long mine = ((long long)(row / G) * a.q_stride + (long long)((w.head / C::CS) * G + row % G) * HD) * 2;
+            const char* qb = reinterpret_cast<const char*>(a.q) + (lane & 7) * 16;
+            auto fetch = [&](int c, uint32_t to) {             // chunk c: 64 elements
+                #pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int r = 4 * i + (lane >> 3);         // of the warp's rows
+                    const char* src = qb + __shfl_sync(0xffffffffu, mine, r) + c * 128;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + r * 128 + (((lane & 7) ^ (r & 7)) << 4)),
+                                 "l"(src), "r"((alive >> r) & 1u ? 16 : 0)      // 0: zeros
+                                 : "memory");
+                }
+            };
+            auto landed = [&]() {
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncwarp();
+            };
+            auto to_tmem = [&](int c, uint32_t from) {
+                uint32_t v[32];
+                #pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const uint4 y = ld_shared(from + lane * 128 + ((j ^ (lane & 7)) << 4));
+                    v[4 * j] = y.x;
+                    v[4 * j + 1] = y.y;
+                    v[4 * j + 2] = y.z;
+                    v[4 * j + 3] = y.w;
+                }
+                tc::st_32x32b_x32(tl + C::Q_COL + 32 * c, v);
+                __syncwarp();
+            };
+            constexpr int QC = C::QT / 64;                     // chunks in tensor memory
+            auto shared_of = [&](int c) { return qs + (c - QC) * (kRowsP * 128) + wq * (32 * 128); };
+            constexpr int NC = HD / 128;                       // chunks of this half
+            // (loops that stay loops: code that runs once comes from memory as slowly as data does)
+            if constexpr (!C::STAGE_IN_Q) {
                 #pragma unroll 1
                 for (int n = 0; n < NC; n++) {
-                    const int c = C::STAGE_IN_Q ? half + 2 * n : half * NC + n;
-                    // (at hd 512 the chunks from the third on may go where the stages are: those are done with then)
-                    if (C::STAGE_IN_Q && n == 2) named_bar_sync(1, kSoft);
-                    uint4 x[8];
-                    #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int r = 4 * i + (lane >> 3);     // of the warp's rows
-                        const long long o = __shfl_sync(0xffffffffu, mine, r);
-                        x[i] = (alive >> r) & 1u ? __ldg(reinterpret_cast<const uint4*>(qb + o + c * 128))
-                                                 : make_uint4(0, 0, 0, 0);
-                    }
-                    const bool in_tmem = c < C::QT / 64;
-                    const uint32_t to_row = in_tmem ? stage : qs + (c - C::QT / 64) * (kRowsP * 128) + wq * (32 * 128);
-                    #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int r = 4 * i + (lane >> 3);
-                        st_shared(to_row + r * 128 + (((lane & 7) ^ (r & 7)) << 4), x[i]);
-                    }
-                    __syncwarp();
-                    if (in_tmem) {
-                        uint32_t v[32];
-                        #pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const uint4 y = ld_shared(stage + lane * 128 + ((j ^ (lane & 7)) << 4));
-                            v[4 * j] = y.x;
-                            v[4 * j + 1] = y.y;
-                            v[4 * j + 2] = y.z;
-                            v[4 * j + 3] = y.w;
-                        }
-                        tc::st_32x32b_x32(tl + C::Q_COL + 32 * c, v);
-                        __syncwarp();
+                    const int c = half * NC + n;
+                    fetch(c, c < QC ? stage + n * C::STAGE : shared_of(c));
+                }
+                landed();
+                #pragma unroll 1
+                for (int n = 0; n < NC && half * NC + n < QC; n++) to_tmem(half * NC + n, stage + n * C::STAGE);
+            } else {
+                // chunks by turns; the last one of each half goes where the stages are, when those are done with
+                #pragma unroll 1
+                for (int n = 0; n < NC; n++) {
+                    const int c = half + 2 * n;
+                    if (n == NC - 1) named_bar_sync(1, kSoft);
+                    fetch(c, c < QC ? stage : shared_of(c));
+                    if (c < QC) {
+                        landed();
+                        to_tmem(c, stage);
                     }
                 }
-                if constexpr (HD > C::QT) tc::fence_proxy_async_smem();
-                tc::wait_st();
-                tc::fence_before();
-                arrive(b_q);
+                landed();
             }
+            if constexpr (HD > C::QT) tc::fence_proxy_async_smem();
+            tc::wait_st();
+            tc::fence_before();
+            arrive(b_q);
         };
         // A piece's result is written after the next piece's Q has been loaded (its scores are made meanwhile), except
         // at hd 512, where the stages lie in Q's place.
@@ -468,17 +481,55 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         float2* ml = nullptr;                     // its (base, sum), null where the result is finished here,
         int esize = 4;                            // the bytes of an element
         for (;;) {
+            // What the next piece needs from memory is asked for before the result of the last one is written.
+            const int part = w.head % C::CS, nrows = w.t.nrows, row = w.t.row0 + min(r0, nrows - 1);
+            const int tok = row / G, hq = (w.head / C::CS) * G + row % G;
+            const int u0 = (int)((it ^ (uint32_t)half) & 1u);        // this group's first unit
+            // page ids of a unit, one per box, in the first lanes; fetched a unit ahead
+            const int box = min(d.ps, kUnit), boxes = kUnit / box;
+            auto page_of = [&](int u) {
+                if (u >= w.nu) return -1;
+                const Unit un = unit_of(w.t, w.unit + u);
+                const int idx = (un.key + (lane & 3) * box) >> d.lps;
+                const int* table = un.pre ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
+                return lane < boxes && idx < (un.pre ? d.pre_pages : d.own_pages) ? __ldg(table + idx) : -1;
+            };
+            int page = -1, vlo = 0, vhi = 0;          // the positions that this row sees, [vlo, vhi)
+            if (more) {
+                const int pos = __ldg(at<int>(a.plan, d.tok_pos) + tok);
+                const int pre = w.t.seq >= 0 ? 0 : __ldg(at<int>(a.plan, d.row_pre) + row);
+                page = page_of(u0);
+                const bool live = r0 < nrows && pre != -1;
+                alive = __ballot_sync(0xffffffffu, live);
+                vhi = live ? pos + 1 : 0;
+                vlo = live && d.window > 0 ? max(0, pos + 1 - d.window) : 0;
+            }
             // the last unit's scores, which may be the other group's, are made: Q may be written over
             if (pending) wait(b_s + 8u * ((it - 1) & 1u), ((it - 1) >> 1) & 1u);
-            if (!C::STAGE_IN_Q && more) load_q();
+            if (!C::STAGE_IN_Q && more) load_q(row);
+            // Both groups' sums, on the last unit's base.  Behind this wait every warp has taken up the last piece, and has
+            // read what is shared about it: a piece of one unit, which one group does alone, has a barrier for that.
             if (pending) {
-                // both groups' sums, on the last unit's base
                 wait(b_base + 8u * ((it - 1) & 1u), ((it - 1) >> 1) & 1u);
                 const float last = sm.base[(it - 1) & 1][r0];
                 if (m != last && l != 0.f) l *= exp2_approx(m - last);
                 m = last;
                 sm.sum[half][r0] = l;
-                named_bar_sync(1, kSoft);
+            }
+            if (more && half == 0) {
+                const bool live = (alive >> lane) & 1u;
+                // what all rows see, what any row sees
+                const int4 seen = make_int4(__reduce_max_sync(0xffffffffu, vlo), __reduce_min_sync(0xffffffffu, live ? vhi : 0x7fffffff),
+                                            __reduce_min_sync(0xffffffffu, live ? vlo : 0x7fffffff), __reduce_max_sync(0xffffffffu, vhi));
+                if (lane == 0) {
+                    sm.red[wq][0] = seen.x;
+                    sm.red[wq][1] = seen.y;
+                    sm.red[wq][2] = seen.z;
+                    sm.red[wq][3] = seen.w;
+                }
+            }
+            named_bar_sync(1, kSoft);
+            if (pending) {
                 l = sm.sum[0][r0] + sm.sum[1][r0];
                 wait(b_o, (pieces - 1) & 1u);
                 tc::fence_after();
@@ -497,12 +548,15 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         uint32_t y[32];
                         tc::ld_32x32b_x32(tl + C::O_COL + c + 32, y);
                         tc::wait_ld();
+                        // (two to an instruction: the conversion of one has a quarter of the rate)
+                        auto pair = [](float lo, float hi) {
+                            const __half2 h2 = __floats2half2_rn(lo, hi);
+                            return *reinterpret_cast<const uint32_t*>(&h2);
+                        };
                         #pragma unroll
                         for (int j = 0; j < 16; j++) {
-                            v[j] = pack_half2(__float2half_rn(__uint_as_float(v[2 * j])),
-                                              __float2half_rn(__uint_as_float(v[2 * j + 1])));
-                            y[j] = pack_half2(__float2half_rn(__uint_as_float(y[2 * j]) * inv),
-                                              __float2half_rn(__uint_as_float(y[2 * j + 1]) * inv));
+                            v[j] = pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                            y[j] = pair(__uint_as_float(y[2 * j]) * inv, __uint_as_float(y[2 * j + 1]) * inv);
                         }
                         #pragma unroll
                         for (int j = 0; j < 16; j++) v[16 + j] = y[j];
@@ -524,26 +578,10 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 tc::fence_before();
                 if (C::STAGE_IN_Q) named_bar_sync(1, kSoft);   // every stage has been emptied
             }
-            if (C::STAGE_IN_Q && more) load_q();
+            if (C::STAGE_IN_Q && more) load_q(row);
             if (!more) break;
-            const int part = w.head % C::CS, nrows = w.t.nrows, row = w.t.row0 + min(r0, nrows - 1);
-            const int tok = row / G, hq = (w.head / C::CS) * G + row % G;
             mask = alive;
-            const bool live = (mask >> lane) & 1u;
-            // the positions that this row sees, [vlo, vhi)
-            const int pos = __ldg(at<int>(a.plan, d.tok_pos) + tok);
-            const int vhi = live ? pos + 1 : 0, vlo = live && d.window > 0 ? max(0, pos + 1 - d.window) : 0;
-            // what all rows see, what any row sees
-            int all_lo = __reduce_max_sync(0xffffffffu, vlo), all_hi = __reduce_min_sync(0xffffffffu, live ? vhi : 0x7fffffff);
-            int any_lo = __reduce_min_sync(0xffffffffu, live ? vlo : 0x7fffffff), any_hi = __reduce_max_sync(0xffffffffu, vhi);
-            named_bar_sync(1, kSoft);             // the piece before has been read out of sm.red
-            if (lane == 0 && half == 0) {
-                sm.red[wq][0] = all_lo;
-                sm.red[wq][1] = all_hi;
-                sm.red[wq][2] = any_lo;
-                sm.red[wq][3] = any_hi;
-            }
-            named_bar_sync(1, kSoft);
+            int all_lo = 0, all_hi = 0x7fffffff, any_lo = 0x7fffffff, any_hi = 0;
             #pragma unroll
             for (int i = 0; i < 4; i++) {
                 all_lo = max(all_lo, sm.red[i][0]);
@@ -551,20 +589,10 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 any_lo = min(any_lo, sm.red[i][2]);
                 any_hi = max(any_hi, sm.red[i][3]);
             }
-            // page ids of a unit, one per box, in the first lanes; fetched a unit ahead
-            const int box = min(d.ps, kUnit), boxes = kUnit / box;
-            auto page_of = [&](int u) {
-                if (u >= w.nu) return -1;
-                const Unit un = unit_of(w.t, w.unit + u);
-                const int idx = (un.key + (lane & 3) * box) >> d.lps;
-                const int* table = un.pre ? a.pre_table : a.table + (size_t)w.t.seq * d.own_pages;
-                return lane < boxes && idx < (un.pre ? d.pre_pages : d.own_pages) ? __ldg(table + idx) : -1;
-            };
+            if (w.nu == 1) named_bar_sync(1, kSoft);
             m = -INFINITY;
             l = 0.f;
             const uint32_t it0 = it;
-            const int u0 = (int)((it0 ^ (uint32_t)half) & 1u);       // this group's first unit
-            int page = page_of(u0);
             #pragma unroll 1
             for (int u = u0; u < w.nu; u += 2) {
                 it = it0 + u;
