@@ -432,7 +432,7 @@ template <int N>
 __device__ __forceinline__ void store_half(uint16_t* p, const float (&v)[N]) {
     uint32_t w[N / 2];
     #pragma unroll
-    for (int j = 0; j < N / 2; j++) w[j] = pack_half2(__float2half_rn(v[2 * j]), __float2half_rn(v[2 * j + 1]));
+    for (int j = 0; j < N / 2; j++) w[j] = half_pair(v[2 * j], v[2 * j + 1]);
     if constexpr (N == 4) {
         *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     } else {
@@ -533,7 +533,7 @@ template <int N>
 __device__ __forceinline__ void store_half_n(uint16_t* p, const float* v) {
     uint32_t w[N / 2];
     #pragma unroll
-    for (int j = 0; j < N / 2; j++) w[j] = pack_half2(__float2half_rn(v[2 * j]), __float2half_rn(v[2 * j + 1]));
+    for (int j = 0; j < N / 2; j++) w[j] = half_pair(v[2 * j], v[2 * j + 1]);
     if constexpr (N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     else if constexpr (N == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(p) = w[0];
@@ -1023,8 +1023,8 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
                         make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
                 } else {
                     uint2 p;
-                    p.x = pack_half2(__float2half_rn(v[0] * inv), __float2half_rn(v[1] * inv));
-                    p.y = pack_half2(__float2half_rn(v[2] * inv), __float2half_rn(v[3] * inv));
+                    p.x = half_pair(v[0] * inv, v[1] * inv);
+                    p.y = half_pair(v[2] * inv, v[3] * inv);
                     *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(a.out) + at0) = p;
                 }
             } else {

@@ -548,15 +548,10 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         uint32_t y[32];
                         tc::ld_32x32b_x32(tl + C::O_COL + c + 32, y);
                         tc::wait_ld();
-                        // (two to an instruction: the conversion of one has a quarter of the rate)
-                        auto pair = [](float lo, float hi) {
-                            const __half2 h2 = __floats2half2_rn(lo, hi);
-                            return *reinterpret_cast<const uint32_t*>(&h2);
-                        };
                         #pragma unroll
                         for (int j = 0; j < 16; j++) {
-                            v[j] = pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-                            y[j] = pair(__uint_as_float(y[2 * j]) * inv, __uint_as_float(y[2 * j + 1]) * inv);
+                            v[j] = half_pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                            y[j] = half_pair(__uint_as_float(y[2 * j]) * inv, __uint_as_float(y[2 * j + 1]) * inv);
                         }
                         #pragma unroll
                         for (int j = 0; j < 16; j++) v[16 + j] = y[j];
@@ -651,8 +646,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         const float e0x = exp2_approx(fmaf(__uint_as_float(x[k][2 * j]), a.scale, -base));
                         const float e1x = exp2_approx(fmaf(__uint_as_float(x[k][2 * j + 1]), a.scale, -base));
                         sum[j & 3] += e0x + e1x;
-                        const __half2 h2 = __floats2half2_rn(e0x, e1x);
-                        x[0][16 * k + j] = *reinterpret_cast<const uint32_t*>(&h2);   // P over the scores it is made of
+                        x[0][16 * k + j] = half_pair(e0x, e1x);       // P over the scores it is made of
                     }
                 if (scale) l *= exp2_approx(from - m);
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
