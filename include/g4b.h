@@ -543,7 +543,9 @@ G4B_API int g4b_attn_prefill(const void* q, int dtype, int q_stride, int M, cons
  * g4b_paged_plan reads q_start, kv_len and *prefix_len once and lays the work of the attention out over the
  * SMs.  The later calls take the same sizes; given a plan of other sizes they write nothing and raise
  * G4B_Q_KERNEL_STATUS bit 1.  Sizes: hd 128, 256 or 512; nH a multiple of nkv; B <= 4096;
- * (table_pages + prefix_pages) * page_size <= 2^30; window 0 (none) or the keys a token sees, itself included. */
+ * (table_pages + prefix_pages) * page_size <= 2^30; window 0 (none) or the keys a token sees, itself included.
+ * Buffers, their rows and the plan are 16-byte aligned.  A plan lives in the caller's memory (g4b_paged_plan_bytes); calls
+ * that share one are ordered by the caller, calls with plans of their own may run at once. */
 G4B_API size_t g4b_paged_plan_bytes(int T, int B, int nH, int nkv, int hd, int page_size, int table_pages,
                                     int prefix_pages, int window);
 G4B_API int g4b_paged_plan(const int* q_start, const int* kv_len, const int* prefix_len, int T, int B, int nH, int nkv,
@@ -559,7 +561,7 @@ G4B_API int g4b_paged_plan(const int* q_start, const int* kv_len, const int* pre
  * with the rotation rows p of cos_tab / sin_tab [n_pos, hd] f32, n_pos >= the tables' positions.  Keys and
  * values at positions below *prefix_len are not written (the shared pages hold them).  qkv f32 or f16 with
  * row_stride elements between rows, q_out f16 with q_stride; strides and offsets multiples of 8.  No two
- * tokens of a call may have the same place in the cache. */
+ * tokens of a call may have the same place in the cache; kc, vc, q_out and qkv may not overlap (G4B_E_ARG). */
 G4B_API int g4b_paged_append(const void* qkv, int dtype, long long row_stride, const float* qnw, const float* knw,
                              const float* cos_tab, const float* sin_tab, int n_pos, uint16_t* kc, uint16_t* vc,
                              int num_pages, const int* table, uint16_t* q_out, long long q_stride, int T, int B, int nH,
@@ -570,7 +572,9 @@ G4B_API int g4b_paged_append(const void* qkv, int dtype, long long row_stride, c
  *   out[t, h*hd ..] = sum_j softmax_j(scale * q_t,h . k_j) v_j over the positions j <= p, j > p - window if window > 0.
  * The prefix's keys and values are read once for the rows of all sequences, a sequence's own once for its rows.
  * A token that sees no key gets zeros.  q f16 [T, q_stride]; out f16 or f32 [T, out_stride]; strides multiples of 8.
- * f32 scores, maxima, sums and accumulators.  The workspace (g4b_paged_workspace_bytes) needs no
+ * f32 scores, maxima, sums and accumulators; the weights are rounded to f16 where a sequence (or the prefix) has more than
+ * 8 rows (16 at hd 128), and enter as f16 hi + lo pairs elsewhere.  out may not overlap q or the caches (G4B_E_ARG);
+ * columns of one buffer may hold both.  The workspace (g4b_paged_workspace_bytes) needs no
  * initialisation; calls that share one, or a plan, must be ordered. */
 G4B_API size_t g4b_paged_workspace_bytes(int T, int B, int nH, int nkv, int hd, int page_size, int table_pages,
                                          int prefix_pages, int window);
@@ -602,8 +606,9 @@ G4B_API int g4b_gelumul(const void* gate, const void* up, int dtype, void* out, 
  *   y  = h' * rsqrt(mean(h'^2) + 1e-6) * w
  *   sa[m] = max(max_k |y[m,k]| / 127, 1e-12),  A8[m,k] = clamp(round_half_even(y[m,k] / sa[m]), -127, 127)
  * x f32 or f16; h, w_post, w f32.  h' goes to h_out, which may be h itself (in place) but not overlap it
- * otherwise; NULL: it is not stored.  x, w_post, h, h_out and w are 32-byte aligned.  The codes are formed without rounding y first, so one may differ by a
- * step from the three calls' where y / sa is next to a half.  D is a multiple of 16. */
+ * otherwise; NULL: it is not stored.  Nothing else that is written may overlap what is read.  x, w_post, h, h_out and w are
+ * 32-byte aligned, A8 16-byte.  The codes are formed without rounding y first, so one may differ by a step from the three
+ * calls' where y / sa is next to a half.  D is a multiple of 16. */
 G4B_API int g4b_rows_normadd_i8(const void* x, int x_dtype, const float* w_post, const float* h, float* h_out, float scl,
                                 const float* w, int8_t* A8, float* sa, int M, int D, g4b_stream_t stream);
 
