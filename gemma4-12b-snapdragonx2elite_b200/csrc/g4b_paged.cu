@@ -27,6 +27,11 @@ static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 // CTAs of the few-rows kernel per SM: two where the stages of two fit an SM's shared memory (hd 128, 256)
 static int few_per_sm(int hd) { return hd == 512 ? 1 : 2; }
 
+// The join kernel's warps per CTA, and its CTAs per SM.  They are there early and wait: with four or eight an SM, 64 users
+// of a long prefix take 101 and 107 us instead of 100, 128 users at hd 128 29 and 32 instead of 27; with one, chunks
+// under a window 214 instead of 196.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinPerSm = 2;
+
 // Checks the sizes and lays the plan out for `sms` SMs.  No device is needed: a caller that will launch asks
 // check_device() last, when every argument has been looked at.
 static int make_dims(const char* op, int T, int B, int nH, int nkv, int hd, int ps, int own_pages, int pre_pages,
@@ -61,6 +66,7 @@ static int make_dims(const char* op, int T, int B, int nH, int nkv, int hd, int 
     d.cs = hd == 512 ? 2 : 1;
     d.ctas[0] = sms * few_per_sm(hd);
     d.ctas[1] = sms;
+    d.join_ctas = sms * kJoinPerSm;
     const int rows = T * d.G;
     // tiles of sequences (one more each for the last, partial one) and of the prefix
     d.max_tiles[0] = (B + 1) * (d.few / kRowsS);
@@ -77,7 +83,8 @@ static int make_dims(const char* op, int T, int B, int nH, int nkv, int hd, int 
     for (int k = 0; k < 2; k++) {
         d.start[k] = take((size_t)d.ctas[k] * sizeof(Start));
         d.tiles[k] = take((size_t)d.max_tiles[k] * sizeof(Tile));
-        d.joins[k] = take((size_t)d.max_tiles[k] * nkv * sizeof(int2));
+        // a list has an entry per group of eight rows, or at most join_ctas smaller ones
+        d.joins[k] = take(std::max((size_t)d.max_tiles[k] * nkv * ((k ? kRowsP : kRowsS) / kJoinWarps), (size_t)d.join_ctas) * sizeof(int2));
     }
     d.bytes = o;
     d.sig = sig_of(d);
@@ -158,7 +165,7 @@ __device__ X block_scan(X v, X init, X* warp_buf, X* total, F op) {   // exclusi
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     extern __shared__ int sm[];
     __shared__ long long wbuf[kPlanThreads / 32];
-    __shared__ int ibuf[kPlanThreads / 32], s_joins;
+    __shared__ int ibuf[kPlanThreads / 32], s_joins, s_rows[4];
     const Dims& d = a.d;
     const int B = d.B, G = d.G, tid = threadIdx.x;
     int* st = sm;                    // [B + 1] first row of each sequence
@@ -342,22 +349,40 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
             h->wt[kind] = run;
             h->u[kind] = u;
         }
-        // what is left to the join kernel
+        // What is left to the join kernel: groups of 1, 2, 4 or 8 rows, the smallest of which there is one per CTA at
+        // most (a CTA's warps share a group's rows), or 8.
         if (tid == 0) s_joins = 0;
+        if (tid < 4) s_rows[tid] = 0;
         __syncthreads();
-        for (int i = tid; i < nt[kind] * d.nkv; i += kPlanThreads) {
+        auto left_of = [&](int i) {          // rows left of tile i / nkv for KV head i % nkv
             const Tile& t = tiles[i / d.nkv];
-            if (t.seq < 0) continue;
+            if (t.seq < 0) return 0;
             const int walks = kind ? d.cs : 1, head = i % d.nkv;
             bool left = !(t.solo && t.n > 0);
             for (int k = 0; k < walks && !left; k++) {
                 const Span sp = span_of((long long)(head * walks + k) * run + t.off, t.n, u);
                 left = sp.c0 != sp.c1;
             }
-            if (left) at<int2>(a.plan, d.joins[kind])[atomicAdd(&s_joins, 1)] = make_int2(i / d.nkv, head);
+            return left ? t.nrows : 0;
+        };
+        const int pairs = nt[kind] * d.nkv;
+        for (int i = tid; i < pairs; i += kPlanThreads) {
+            const int n = left_of(i);
+            for (int k = 0; k < 4 && n > 0; k++) atomicAdd(&s_rows[k], (n + (1 << k) - 1) >> k);
         }
         __syncthreads();
-        if (tid == 0) h->nj[kind] = s_joins;
+        int lr = 0;
+        while (lr < 3 && s_rows[lr] > d.join_ctas) lr++;
+        for (int i = tid; i < pairs; i += kPlanThreads) {
+            const int n = (left_of(i) + (1 << lr) - 1) >> lr;
+            const int at0 = n > 0 ? atomicAdd(&s_joins, n) : 0;
+            for (int k = 0; k < n; k++) at<int2>(a.plan, d.joins[kind])[at0 + k] = make_int2(i / d.nkv, k << 16 | i % d.nkv);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            h->nj[kind] = s_joins;
+            h->rj[kind] = 1 << lr;
+        }
         for (int c = tid; c < d.ctas[kind]; c += kPlanThreads) {
             Start s{};
             s.head = -1;
@@ -1056,11 +1081,9 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
 
 // ------------------------------------------------------------------ join
 // out = sum_p V_p 2^(m_p - M) / sum_p l_p 2^(m_p - M) over the partials of a row's prefix tile and of its own tile, for
-// the rows that no whole tile wrote; a row with no key at all becomes zeros.  The plan lists the (tile, KV head) pairs;
-// a CTA takes eight rows of one at a time.  Where there are fewer rows than warps, several warps share a row's partials:
+// the rows that no whole tile wrote; a row with no key at all becomes zeros.  The plan lists groups of rows of a (tile,
+// KV head) pair; a CTA takes a group at a time.  Where it has fewer rows than warps, several warps share a row's partials:
 // a decode token over a long prefix has twenty or so, and their loads are what takes time here.
-constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
-constexpr int kJoinSubs = kRowsP / kJoinWarps;       // groups of eight rows in a many-rows tile
 
 template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
@@ -1069,17 +1092,16 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
     const Dims& d = a.d;
     const Hdr* h = hdr_of(a.plan);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int n0 = h->sig == d.sig ? h->nj[0] : 0, items = n0 + (h->sig == d.sig ? h->nj[1] * kJoinSubs : 0);
+    const int n0 = h->sig == d.sig ? h->nj[0] : 0, items = n0 + (h->sig == d.sig ? h->nj[1] : 0);
     bool waited = false;
     for (int it = blockIdx.x; it < items; it += gridDim.x) {
         // the plan's part first: no kernel before this one writes it
-        const int kind = it >= n0, e = kind ? (it - n0) / kJoinSubs : it, sub = kind ? (it - n0) % kJoinSubs : 0;
-        const int2 pair = at<int2>(a.plan, d.joins[kind])[e];
-        const Tile t = at<Tile>(a.plan, d.tiles[kind])[pair.x];
-        const int head = pair.y, rows = min(kJoinWarps, t.nrows - sub * kJoinWarps);
-        if (rows <= 0) continue;
+        const int kind = it >= n0, most = h->rj[kind];
+        const int2 entry = at<int2>(a.plan, d.joins[kind])[kind ? it - n0 : it];
+        const Tile t = at<Tile>(a.plan, d.tiles[kind])[entry.x];
+        const int head = entry.y & 0xffff, row_a = (entry.y >> 16) * most, rows = min(most, t.nrows - row_a);
         const int share = rows > 4 ? 1 : rows > 2 ? 2 : rows > 1 ? 4 : 8;       // warps per row
-        const int r = sub * kJoinWarps + warp / share;
+        const int r = row_a + warp / share;
         const bool busy = r < t.nrows && warp / share < rows;
         const int row = t.row0 + min(r, t.nrows - 1), tok = row / d.G, hq = head * d.G + row % d.G;
         // A many-rows tile of a wide head is walked once per part of the columns; this lane's part may have been cut
@@ -1230,8 +1252,8 @@ static cudaError_t launch_few(const Args& a, const CUtensorMap& km, const CUtens
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) return e;
-    const long long most = ((long long)a.d.max_tiles[0] + (long long)a.d.max_tiles[1] * kJoinSubs) * a.d.nkv;
-    return launch_pdl(join_kernel<HD>, dim3((unsigned)std::min(most, 2LL * a.d.ctas[0])), kJoinThreads, 0, s, a);
+    const int most = a.d.T * a.d.nH;      // a group has a row at least
+    return launch_pdl(join_kernel<HD>, dim3((unsigned)std::min(most, a.d.join_ctas)), kJoinThreads, 0, s, a);
 }
 
 template <int HD, bool XF32>

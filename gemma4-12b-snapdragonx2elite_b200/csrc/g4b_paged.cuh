@@ -71,7 +71,8 @@ struct Hdr {
     int prefix_len;
     int tok_lo, tok_hi;              // rows of the token buffers that belong to a sequence
     int nt[2];                       // tiles: [0] few rows, [1] many rows
-    int nj[2];                       // (tile, KV head) pairs whose rows the join kernel finishes
+    int nj[2];                       // entries of the join kernel's lists,
+    int rj[2];                       // and the rows that one stands for
     long long wt[2];                 // units of one KV head
     long long u[2];                  // units per CTA
 };
@@ -84,6 +85,7 @@ struct Dims {
     int cs;                          // walks per many-rows tile: parts of hd's output columns
     int ctas[2];                     // stretches per kind
     int max_tiles[2];
+    int join_ctas;                   // CTAs of the join kernel that are there at once
     size_t tok_seq, tok_pos, row_pre, start[2], tiles[2], joins[2], bytes;
     unsigned sig;
 };

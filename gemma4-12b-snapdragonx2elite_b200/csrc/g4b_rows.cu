@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(1024) rows_normadd_i8_long_kernel(const NormI8
 
 // Threads and groups per thread.  Few rows (latency): as many threads as there are groups, up to a block.  Many rows:
 // three groups per thread, so that several blocks share an SM and one's loads cover another's reductions; 8,192 rows of
-// 3,840 f16: 59 us (5.87 TB/s, 0.90 of the measured copy rate), against 63 us with two groups and 95 us with one
+// 3,840 f16: 57 us (6.1 TB/s, 0.93 of the measured copy rate), against 63 us with two groups and 95 us with one
 // 16-byte group of four per thread.  Up to 256 groups one each is as fast (8,192 x 1,024: 18.5 us against 18.8).
 template <bool XF32>
 static void launch_normadd_i8(const NormI8Args& a, int M, int sms, cudaStream_t s) {

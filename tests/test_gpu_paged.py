@@ -628,3 +628,26 @@ def test_a_captured_step_of_append_and_attention(T, hd, nH, nkv):
         if k:
             assert torch.equal(out[0], out[1]) and torch.equal(a.kc, b.kc) and torch.equal(a.vc, b.vc)
     assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+@pytest.mark.parametrize("nH,nkv,hd", HEADS)
+@pytest.mark.parametrize("new,total,prefix", [
+    ([1] * 64, [400 + 9 * i for i in range(64)], 300),        # joins of single rows and of small groups
+    ([1] * 200, [301 + i for i in range(200)], 300),
+    ([16] * 30, [2000] * 30, 0),
+    ([150, 400, 1, 0, 33], [900, 1000, 801, 5, 833], 800),    # and of tiles of 128 rows
+])
+def test_plan_and_workspace_stay_inside_their_bytes(nH, nkv, hd, new, total, prefix):
+    bt = Batch(nH, nkv, hd, 32, new, total, prefix, seed=40).fill()
+    q, plan = bt.queries(), bt.plan()
+    guarded = []
+    for name in ("_plan", "_ws"):
+        n = getattr(plan, name).numel()
+        room = torch.full((n + 65536,), 0xA5, dtype=torch.uint8, device=DEV)
+        setattr(plan, name, room[:n])
+        setattr(plan, name + "_ptr", room.data_ptr())
+        guarded.append((room, n))
+    plan.update(bt.q_start, bt.kv_len, bt.prefix_len)
+    bt.check(_attend(bt, q, plan), q)
+    for room, n in guarded:
+        assert (room[n:] == 0xA5).all()
