@@ -119,7 +119,11 @@ static size_t work_bytes(const Dims& d, char* base, Work* w) {
 // trusted with an address: starts are made non-decreasing and cut to [0, T], lengths to the tables'
 // capacity.
 constexpr int kPlanThreads = 1024;
-constexpr long long kPieceCostS = 2, kPieceCostP = 3;
+// A tile's start and end cost about as much as this many of its units (rows in, masks, result out): they count as its
+// work, or a causal prompt's short first tiles, twenty to a stretch, make the slowest CTA (2 prompts of 4,096: with none
+// 369 us at hd 256 and 221 at hd 128, with 5 units 310 and 125, with 8 to 10 293 and 122; ragged decode, 48 tokens: with
+// none 143 us, with 2 units 140).  A border inside a tile costs its CTA another start and another partial.
+constexpr int kTileCostS = 2, kTileCostP = 8, kBorderCostS = 2, kBorderCostP = 3;
 
 struct PlanArgs {
     const int* q_start;
@@ -267,7 +271,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         const bool pre_here = pre_tiles > 0 && (kind == 1) == pre_many;
         const auto add = [](long long x, long long y) { return x + y; };
         const int heads = d.nkv * (kind ? d.cs : 1), ctas = d.ctas[kind];
-        long long work = 0;                  // units of one head
+        long long work = 0, filled = 0;      // units of one head, tiles that have any
         for (int i0 = 0; i0 < nt[kind]; i0 += kPlanThreads) {
             const int i = i0 + tid;
             Tile t{};
@@ -302,11 +306,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
             long long all;
             block_scan((long long)t.n, 0LL, wbuf, &all, add);
             work += all;
+            block_scan(t.n > 0 ? 1LL : 0LL, 0LL, wbuf, &all, add);
+            filled += all;
         }
         __syncthreads();
         // Equal stretches of the line of all heads' units, wherever their borders fall; or, if every tile can have
-        // CTAs of its own, the shortest stretch for which they suffice when each tile starts at a border.  A border
-        // inside a tile costs its CTA another start and another partial, about kPieceCost units.
+        // CTAs of its own, the shortest stretch for which they suffice when each tile starts at a border.
+        const int cost = kind ? kTileCostP : kTileCostS;
         long long u = max(1LL, (work * heads + ctas - 1) / ctas);
         bool aligned = false;
         {
@@ -317,7 +323,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
                 block_scan(n, 0LL, wbuf, &all, add);
                 return all * heads;
             };
-            const long long most = u + (kind ? kPieceCostP : kPieceCostS);
+            const long long most = u + (kind ? kBorderCostP : kBorderCostS);
             if (work > 0 && stretches(most) <= ctas) {
                 long long lo = u, hi = most;
                 while (lo < hi) {
@@ -327,13 +333,15 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
                 }
                 u = lo;
                 aligned = true;
+            } else {
+                u = max(1LL, ((work + (long long)cost * filled) * heads + ctas - 1) / ctas);
             }
         }
         long long run = 0;
         for (int i0 = 0; i0 < nt[kind]; i0 += kPlanThreads) {
             const int i = i0 + tid;
             const int n = i < nt[kind] ? tiles[i].n : 0;
-            const int idle = aligned ? (int)((u - n % u) % u) : 0;
+            const int idle = aligned ? (int)((u - n % u) % u) : n > 0 ? cost : 0;
             long long all;
             const long long exc = block_scan((long long)n + idle, 0LL, wbuf, &all, add);
             if (i < nt[kind]) {
@@ -398,7 +406,16 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
                 }
                 s.tile = lo;
                 s.unit = (int)(rem - tiles[lo].off);
-                s.t = tiles[lo];
+                if (s.unit >= tiles[lo].n) {     // between two tiles
+                    s.skip = tiles[lo].n + tiles[lo].idle - s.unit;
+                    s.unit = 0;
+                    if (++s.tile == nt[kind]) {
+                        s.tile = 0;
+                        s.head++;
+                    }
+                    if (s.skip >= u || at0 + s.skip >= total) s.head = -1;
+                }
+                s.t = tiles[s.tile];
             }
             at<Start>(a.plan, d.start[kind])[c] = s;
         }
@@ -709,7 +726,7 @@ __global__ void __launch_bounds__(32 * (stream_warps(HD) + 1), HD == 512 ? 1 : 2
 // gets from its accumulator layout to an operand's by movmatrix.  P enters as f16 hi + lo, since these
 // MMAs are not what bounds the kernel.  The four warps of a CTA take every fourth block of 16 keys, each
 // with its own ring of TMA-filled buffers, its own running maximum and sum: no CTA barrier until the
-// partials of the warps are added at a piece's end.  48 decode tokens over 868 MB of ragged keys and values: 144 us, 0.92
+// partials of the warps are added at a piece's end.  48 decode tokens over 868 MB of ragged keys and values: 140 us, 0.95
 // of the measured copy rate.
 constexpr int kFewWarps = 4;
 constexpr int kBlk = 16;             // keys per block (one page always holds a block: page_size >= 16)
@@ -781,7 +798,7 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
     const int ntiles = h->nt[0];
     const Tile* tiles = at<Tile>(a.plan, d.tiles[0]);
     const int* tok_pos = at<int>(a.plan, d.tok_pos);
-    long long left = min(u_all, wt * d.nkv - (long long)blockIdx.x * u_all);
+    long long left = min(u_all, wt * d.nkv - (long long)blockIdx.x * u_all) - st.skip;
     int head = st.head, ti = st.tile, unit = st.unit;
     int entry = 0;                       // ring position of the next entry to consume; runs on over pieces
     uint32_t phase = 0;                  // parity bit per ring position

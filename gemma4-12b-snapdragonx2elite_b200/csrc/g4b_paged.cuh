@@ -12,7 +12,8 @@
 // the other such sequences in tiles against the prefix; with more (a prompt's chunk) it fills tiles by itself,
 // which read the prefix and then its own keys.  The units of all tiles and KV heads
 // form one line that is cut into equal lengths, one per CTA, whatever the lengths of the sequences: a CTA
-// walks its stretch piece by piece.  Where that costs no more (few tiles, many CTAs) every tile starts at a border.  A tile that lies in one CTA's stretch is finished there; one that
+// walks its stretch piece by piece.  (A tile counts for a few units more than it has: its start and end take time too.)
+// Where that costs no more (few tiles, many CTAs) every tile starts at a border.  A tile that lies in one CTA's stretch is finished there; one that
 // crosses a border leaves a partial (running maximum, sum, weighted values) in the edge slots of each CTA,
 // and the join kernel adds them.
 #pragma once
@@ -45,7 +46,8 @@ struct __align__(16) Tile {
     int n1, lo1, hi1;   // prefix keys [lo1, hi1); lo1 is a multiple of kUnit
     int lo2, hi2;       // own keys [lo2, hi2), counted from the prefix's end; lo2 is a multiple of kUnit
     int solo;        // its rows have keys in no other tile: a whole tile writes the output itself
-    int idle;        // units behind it that are nobody's work: they align the next tile with a stretch's start
+    int idle;        // units behind it that are nobody's work: what the tile costs besides its units, or what aligns the
+                     // next one with a stretch's start
     int pad;
     long long off;   // units of the tiles before it, their idle ones included
     long long pad2;
@@ -62,7 +64,8 @@ __host__ __device__ __forceinline__ Unit unit_of(const Tile& t, int u) {
 }
 
 struct Start {       // where a CTA's stretch begins
-    int head, tile, unit, pad;   // head: KV head * walks per tile + walk; -1: nothing to do
+    int head, tile, unit;        // head: KV head * walks per tile + walk; -1: nothing to do
+    int skip;                    // idle units before that
     Tile t;                      // tiles[tile]
 };
 

@@ -25,7 +25,7 @@
 // (1,270 and 550 at hd 128): the product of a unit waits for its weights, whose place is free when the product before is
 // done, and each such hand-over from warp to warp and back is 150 to 300 clocks.  Deeper or shallower rings change
 // nothing.  Between two pieces pass 10,000 clocks or so: Q in, the masks, the result out.  Two prompts of 4,096 tokens
-// over 16 heads of 256 (8 KV heads): 367 us, 0.45 of the measured bf16 rate; of 128 (8 heads, 1 KV head): 222 us.
+// over 16 heads of 256 (8 KV heads): 293 us, 0.57 of the measured bf16 rate; of 128 (8 heads, 1 KV head): 122 us.
 #include "g4b_paged.cuh"
 #include "g4b_tcgen05.cuh"
 
@@ -133,7 +133,7 @@ struct Walk {
         head = st.head;
         ti = st.tile;
         unit = st.unit;
-        left = min(h->u[1], h->wt[1] * a.d.nkv * a.d.cs - (long long)blockIdx.x * h->u[1]);
+        left = min(h->u[1], h->wt[1] * a.d.nkv * a.d.cs - (long long)blockIdx.x * h->u[1]) - st.skip;
         return true;
     }
     __device__ __forceinline__ bool next() {
