@@ -25,7 +25,7 @@
 // (1,270 and 550 at hd 128): the product of a unit waits for its weights, whose place is free when the product before is
 // done, and each such hand-over from warp to warp and back is 150 to 300 clocks.  Deeper or shallower rings change
 // nothing.  Between two pieces pass 10,000 clocks or so: Q in, the masks, the result out.  Two prompts of 4,096 tokens
-// over 16 heads of 256 (8 KV heads): 293 us, 0.57 of the measured bf16 rate; of 128 (8 heads, 1 KV head): 122 us.
+// over 16 heads of 256 (8 KV heads): 286 us, 0.58 of the measured bf16 rate; of 128 (8 heads, 1 KV head): 123 us.
 #include "g4b_paged.cuh"
 #include "g4b_tcgen05.cuh"
 
@@ -696,22 +696,27 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     };
                     auto piece_at = [&](int c, int r) { return key_at(c, (r0 >> 3) + 16 * r) + (r0 & 7) * 16; };
                     uint32_t bad = 0;
-                    bool some[4];                            // key r is seen by some rows only
+                    bool some[4], none[4], clear = false;    // key r is seen by some rows only, by none
                     #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const int k = key + (r0 >> 3) + 16 * r;
-                        const bool none = k < any_lo || k >= min(any_hi, end);
-                        some[r] = !none && (k < all_lo || k >= all_hi);
+                        none[r] = k < any_lo || k >= min(any_hi, end);
+                        some[r] = !none[r] && (k < all_lo || k >= all_hi);
+                        clear |= none[r];
+                    }
+                    #pragma unroll
+                    for (int c = 0; c < C::DV / 64; c += 2) {
+                        uint4 v[8];                          // eight loads under way, needed or not
                         #pragma unroll
-                        for (int c = 0; c < C::DV / 64; c++) {
-                            const uint32_t at = piece_at(c, r);
-                            if (none) {
-                                st_shared(at, make_uint4(0, 0, 0, 0));
-                            } else if (some[r]) {
-                                const uint4 v = ld_shared(at);
-                                bad |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
-                            }
-                        }
+                        for (int i = 0; i < 8; i++) v[i] = ld_shared(piece_at(c + (i >> 2), i & 3));
+                        #pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if (some[i & 3]) bad |= not_finite(v[i].x) | not_finite(v[i].y) | not_finite(v[i].z) | not_finite(v[i].w);
+                    }
+                    if (clear) {
+                        #pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            for (int c = 0; c < C::DV / 64 && none[r]; c++) st_shared(piece_at(c, r), make_uint4(0, 0, 0, 0));
                     }
                     unsigned long long odd = 0;
                     if (any_of_group((bad & 0x80008000u) != 0, group_bar)) {
