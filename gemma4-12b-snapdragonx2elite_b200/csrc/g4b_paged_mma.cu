@@ -21,11 +21,12 @@
 // The weights P are rounded to f16, the type of V, as the tensor core needs one type for both: 2^-11 of each
 // weight, unbiased; sums and maxima are f32.
 //
-// What bounds it: neither the tensor core nor memory.  A unit takes 1,460 clocks at hd 256, of which the MMAs are 1,100
-// (1,270 and 550 at hd 128): the product of a unit waits for its weights, whose place is free when the product before is
+// What bounds it: neither the tensor core nor memory.  A unit takes 1,410 clocks at hd 256, of which the MMAs are 1,100
+// (1,300 and 550 at hd 128): the product of a unit waits for its weights, whose place is free when the product before is
 // done, and each such hand-over from warp to warp and back is 150 to 300 clocks.  Deeper or shallower rings change
-// nothing.  Between two pieces pass 10,000 clocks or so: Q in, the masks, the result out.  Two prompts of 4,096 tokens
-// over 16 heads of 256 (8 KV heads): 286 us, 0.58 of the measured bf16 rate; of 128 (8 heads, 1 KV head): 123 us.
+// nothing.  Between two pieces pass 12,000 clocks at hd 256 (16,000 before Q's chunks came all at once): Q in, the masks,
+// the result out.  Two prompts of 4,096 tokens over 16 heads of 256 (8 KV heads): 286 us, 0.58 of the measured bf16
+// rate; of 128 (8 heads, 1 KV head): 123 us.
 #include "g4b_paged.cuh"
 #include "g4b_tcgen05.cuh"
 

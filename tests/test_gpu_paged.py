@@ -651,3 +651,21 @@ def test_plan_and_workspace_stay_inside_their_bytes(nH, nkv, hd, new, total, pre
     bt.check(_attend(bt, q, plan), q)
     for room, n in guarded:
         assert (room[n:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("nH,nkv,hd,new", [(16, 8, 256, 4), (4, 2, 512, 3), (8, 1, 128, 2), (16, 8, 256, 70), (16, 1, 512, 20),
+                                           (8, 1, 128, 40)])
+@pytest.mark.parametrize("prefix", [0, 50])
+def test_values_before_the_window_do_not_reach_a_row(nH, nkv, hd, new, prefix):
+    """A key and value that are not finite, at the one position that only the first token's window still holds."""
+    window = 20
+    bt = Batch(nH, nkv, hd, 16, [new, 1], [new + 60, 90], prefix, window, seed=41).fill()
+    q = bt.queries()
+    clean = _attend(bt, q).clone()
+    bt.check(clean, q)
+    pg, sl = bt.place(0, 60 - window + 1)
+    assert prefix == 0 or 60 - window + 1 < prefix
+    bt.kc[pg, :, sl] = float("inf")
+    bt.vc[pg, :, sl] = float("nan")
+    out = _attend(bt, q)
+    assert torch.equal(out[1:], clean[1:]) and not torch.isfinite(out[0]).any()
