@@ -201,6 +201,11 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
     const uint32_t b_q = b_s + 72;                                   // the piece's Q is there
     const uint32_t b_o = b_s + 80;                                   // the piece's products are all added
     const uint32_t b_drain = b_s + 88;                               // [2] winding down
+    // The piece's result has been read out of O.  Each group reads half of the columns, for as long as its stores take, and
+    // the group that has the next piece's first unit goes on alone: its weights (b_p) say nothing of the other group's
+    // reading.  So a piece's first product, which overwrites all of O, waits here for the eight warps; later ones, and the
+    // rescaling before them, come behind that product.
+    const uint32_t b_out = b_s + 104;
     if (tid == 0) {
         for (int i = 0; i < 2 * C::NST; i++) mbar_init(bar0 + 8u * i, 1);
         for (int i = 0; i < 2; i++) {
@@ -214,6 +219,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         mbar_init(b_o, 1);
         mbar_init(b_drain, 1);
         mbar_init(b_drain + 8, 1);
+        mbar_init(b_out, kSoft / 32);
         fence_mbar_init();
         sm.abort = 0;
     }
@@ -347,6 +353,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
         };
         auto product = [&](int u) {
             int acc = 1;
+            if (u == 0 && piece > 1) wait(b_out, piece & 1u);      // (piece counts this one: the last but one's phase)
             #pragma unroll
             for (int ve = 0; ve < C::VE; ve++) {
                 const int s = entry();             // (V is there long before the weights: that wait comes first)
@@ -563,6 +570,10 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         #pragma unroll
                         for (int j = 0; j < 16; j++) v[16 + j] = y[j];
                     }
+                    if (c + per == (half + 1) * DH) {
+                        tc::fence_before();           // this warp has read O, for the product that overwrites it
+                        arrive(b_out);
+                    }
                     #pragma unroll
                     for (int j = 0; j < 8; j++)
                         st_shared(stage + lane * 128 + ((j ^ (lane & 7)) << 4),
@@ -735,6 +746,10 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                     if (odd) {
                         tc::wait_st();                       // P, read back below
                         if (u == 0) {
+                            if (pieces > 0) {                // the other group's columns too are overwritten
+                                wait(b_out, (pieces - 1) & 1u);
+                                tc::fence_after();
+                            }
                             uint32_t z[32];
                             #pragma unroll
                             for (int j = 0; j < 32; j++) z[j] = 0;

@@ -669,3 +669,50 @@ def test_values_before_the_window_do_not_reach_a_row(nH, nkv, hd, new, prefix):
     bt.vc[pg, :, sl] = float("nan")
     out = _attend(bt, q)
     assert torch.equal(out[1:], clean[1:]) and not torch.isfinite(out[0]).any()
+
+
+LONG = [(16, 8, 256, 0, torch.float16), (16, 8, 256, 1000, torch.float32), (8, 1, 128, 0, torch.float32),
+        (8, 1, 128, 1000, torch.float16), (4, 2, 512, 0, torch.float16)]
+
+
+@pytest.mark.parametrize("nH,nkv,hd,prefix,dtype", LONG)
+def test_long_prompts_give_every_cta_many_tiles(nH, nkv, hd, prefix, dtype):
+    """Several tiles a CTA, of several units each, the result of one read out while the next one's first products are
+    made: against the definition, and the same bits every time beside a stream that keeps the memory busy."""
+    bt = Batch(nH, nkv, hd, 64, [4096, 4096], [prefix + 4096, prefix + 4096], prefix, seed=50).fill()
+    q, plan = bt.queries(), bt.plan()
+    first = _attend(bt, q, plan, dtype)
+    bt.check(first, q)
+    side, a = torch.cuda.Stream(), torch.empty(1 << 28, dtype=torch.uint8, device=DEV)
+    b, outs = torch.empty_like(a), [torch.empty_like(first) for _ in range(10)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            for _ in range(40):
+                b.copy_(a)
+        for o in outs:
+            o.fill_(7.0)
+            plan.attend(q, bt.kc, bt.vc, bt.table, bt.prefix_table, out=o)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, first) for o in outs)
+    assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+@pytest.mark.parametrize("nH,nkv,hd", [(16, 8, 256), (8, 1, 128), (4, 2, 512)])
+def test_values_outside_the_window_of_many_tiles(nH, nkv, hd):
+    """Infinite values every 500 positions, which only some rows of a tile see, in its first unit too: a row that sees
+    none has the bits that it has without them."""
+    n, window = 4096, 150
+    bt = Batch(nH, nkv, hd, 32, [n, n], [n, n], 0, window, seed=51).fill()
+    q, plan = bt.queries(), bt.plan()
+    clean = _attend(bt, q, plan)
+    bt.check(clean, q)
+    at = torch.arange(250, n, 500, device=DEV)
+    for b in range(2):
+        pg, sl = bt.places(b, n)
+        bt.vc[pg[at], :, sl[at]] = float("inf")
+    pos = torch.arange(n, device=DEV)
+    sees = ((at <= pos[:, None]) & (at > pos[:, None] - window)).any(1).repeat(2)
+    for _ in range(20):
+        out = _attend(bt, q, plan)
+        assert torch.equal(out[~sees], clean[~sees]) and not torch.isfinite(out[sees]).any()
