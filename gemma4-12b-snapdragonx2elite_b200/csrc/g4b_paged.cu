@@ -15,13 +15,6 @@ constexpr float kEps = 1e-6f;    // vk/attn.comp:25, vk/prepkv.comp:21
 __device__ unsigned g_status_paged;
 
 // ------------------------------------------------------------------ sizes
-static unsigned sig_of(const Dims& d) {
-    unsigned h = 2166136261u;
-    for (int v : {d.T, d.B, d.nH, d.nkv, d.hd, d.ps, d.own_pages, d.pre_pages, d.window, d.ctas[0], d.ctas[1]})
-        h = (h ^ (unsigned)v) * 16777619u;
-    return h | 1u;
-}
-
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 // CTAs of the few-rows kernel per SM: two where the stages of two fit an SM's shared memory (hd 128, 256)
@@ -87,7 +80,7 @@ static int make_dims(const char* op, int T, int B, int nH, int nkv, int hd, int 
         d.joins[k] = take(std::max((size_t)d.max_tiles[k] * nkv * ((k ? kRowsP : kRowsS) / kJoinWarps), (size_t)d.join_ctas) * sizeof(int2));
     }
     d.bytes = o;
-    d.sig = sig_of(d);
+    d.key = {{kPlanMagic, T, B, nH, nkv, hd, ps, own_pages, pre_pages, d.window, d.ctas[0], d.ctas[1]}};
     return G4B_OK;
 }
 
@@ -421,7 +414,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         }
     }
     if (tid == 0) {
-        h->sig = d.sig;
+        h->key = d.key;
         h->prefix_len = pl;
         h->tok_lo = st[0];
         h->tok_hi = st[B];
@@ -500,10 +493,10 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     float v[PER];
     load_n<PER, XF32>(a.qkv, (long long)t * a.row_stride + lane * PER +
                       (is_q ? (long long)j * HD : (is_v ? a.voff : a.koff) + (long long)kv * HD), v);
-    const unsigned sig = h->sig;
+    const bool fits = plan_fits(h, d);
     const int prefix_len = h->prefix_len;
     const int b = __ldg(at<int>(a.plan, d.tok_seq) + t), pos = __ldg(at<int>(a.plan, d.tok_pos) + t);
-    if (sig != d.sig) {
+    if (!fits) {
         if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(&g_status_paged, kStatusPlan);
         return;
     }
@@ -596,7 +589,7 @@ __global__ void __launch_bounds__(32 * (stream_warps(HD) + 1), HD == 512 ? 1 : 2
     const Dims& d = a.d;
     const Hdr* h = hdr_of(a.plan);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (h->sig != d.sig) {
+    if (!plan_fits(h, d)) {
         if (blockIdx.x == 0 && tid == 0) atomicOr(&g_status_paged, kStatusPlan);
         return;
     }
@@ -771,7 +764,7 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
     const Hdr* h = hdr_of(a.plan);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
     pdl_launch_dependents();
-    if (h->sig != d.sig) {
+    if (!plan_fits(h, d)) {
         if (blockIdx.x == 0 && tid == 0) atomicOr(&g_status_paged, kStatusPlan);
         pdl_wait();
         return;
@@ -1109,7 +1102,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
     const Dims& d = a.d;
     const Hdr* h = hdr_of(a.plan);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int n0 = h->sig == d.sig ? h->nj[0] : 0, items = n0 + (h->sig == d.sig ? h->nj[1] : 0);
+    const bool fits = plan_fits(h, d);
+    const int n0 = fits ? h->nj[0] : 0, items = n0 + (fits ? h->nj[1] : 0);
     bool waited = false;
     for (int it = blockIdx.x; it < items; it += gridDim.x) {
         // the plan's part first: no kernel before this one writes it

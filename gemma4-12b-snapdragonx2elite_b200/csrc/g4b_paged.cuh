@@ -70,7 +70,7 @@ struct Start {       // where a CTA's stretch begins
 };
 
 struct Hdr {
-    unsigned sig;                    // of the sizes the plan was made for
+    PlanKey key;                     // the sizes the plan was made for
     int prefix_len;
     int tok_lo, tok_hi;              // rows of the token buffers that belong to a sequence
     int nt[2];                       // tiles: [0] few rows, [1] many rows
@@ -90,7 +90,7 @@ struct Dims {
     int max_tiles[2];
     int join_ctas;                   // CTAs of the join kernel that are there at once
     size_t tok_seq, tok_pos, row_pre, start[2], tiles[2], joins[2], bytes;
-    unsigned sig;
+    PlanKey key;
 };
 
 __host__ __device__ inline const Hdr* hdr_of(const void* plan) { return reinterpret_cast<const Hdr*>(plan); }
@@ -102,6 +102,9 @@ template <typename X>
 __host__ __device__ inline const X* at(const void* plan, size_t off) {
     return reinterpret_cast<const X*>(reinterpret_cast<const char*>(plan) + off);
 }
+
+// The plan is one that was made for this call's sizes: all its offsets and row numbers are taken from it.
+__device__ __forceinline__ bool plan_fits(const Hdr* h, const Dims& d) { return same_plan(h->key, d.key); }
 
 // The workspace: edge slots of both kinds ([cta][2][rows][columns of a walk] sums, [cta][2][rows] (max, sum)), then,
 // where there is a prefix, one slot per (segment kind, token, head) for whole tiles.

@@ -177,7 +177,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     // The next kernel may begin: it reads nothing of this one, and waits for its end before it ends itself.
     pdl_launch_dependents();
-    if (h->sig != d.sig) {
+    if (!plan_fits(h, d)) {
         if (blockIdx.x == 0 && tid == 0) atomicOr(&g_status_paged_mma, kStatusPlan);
         return;
     }

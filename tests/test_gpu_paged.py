@@ -716,3 +716,32 @@ def test_values_outside_the_window_of_many_tiles(nH, nkv, hd):
     for _ in range(20):
         out = _attend(bt, q, plan)
         assert torch.equal(out[~sees], clean[~sees]) and not torch.isfinite(out[sees]).any()
+
+
+def test_a_plan_of_sizes_whose_hash_was_the_same():
+    """Two batches that differ in tokens, sequences and tables: neither call takes the other's plan."""
+    def made(T, table, prefix):
+        return PagedPlan(T, T, 16, 8, 256, 64, table, prefix, 1024, DEV)
+
+    t32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    for mine, other in (((67, 29, 16), (128, 12, 32)), ((128, 12, 32), (67, 29, 16))):
+        plan, wrong = made(*mine), made(*other)
+        n = other[0]
+        wrong.update(torch.arange(n + 1, dtype=torch.int32, device=DEV), t32(*[1100] * n), t32(1000))
+        room = torch.zeros(plan._plan.numel() + wrong._plan.numel(), dtype=torch.uint8, device=DEV)
+        room[:wrong._plan.numel()] = wrong._plan
+        plan._plan, plan._plan_ptr = room, room.data_ptr()
+        T, table, prefix = mine
+        kc = torch.zeros(prefix + T * table, 8, 64, 256, dtype=torch.float16, device=DEV)
+        vc = torch.zeros_like(kc)
+        ids = torch.arange(prefix, prefix + T * table, dtype=torch.int32, device=DEV).view(T, table)
+        pre = torch.arange(prefix, dtype=torch.int32, device=DEV)
+        out = torch.full((T, 4096), 7.0, dtype=torch.float16, device=DEV)
+        q, w = torch.ones_like(out), torch.ones(256, device=DEV)
+        rot = torch.ones((table + prefix) * 64, 256, device=DEV)
+        plan.attend(q, kc, vc, ids, pre, out=out)
+        torch.cuda.synchronize()
+        assert (out == 7).all() and L.query(L.Q_KERNEL_STATUS) == 2
+        plan.append(torch.ones(T, 8192, device=DEV), w, w, rot, rot, kc, vc, ids, 4096, 6144, q_out=out)
+        torch.cuda.synchronize()
+        assert (out == 7).all() and not kc.any() and not vc.any() and L.query(L.Q_KERNEL_STATUS) == 2

@@ -234,3 +234,26 @@ def test_a_stream_of_another_device_is_refused():
     from g4b import ops
     with pytest.raises(ValueError, match="cuda:1"):
         ops._on(0, SimpleNamespace(device_index=1))
+
+
+# sizes whose hash to a word was the same for 148 SMs, as in PlanKey: T, B, nH, nkv, hd, page_size, tables, window, CTAs
+TWINS = ((67, 67, 16, 8, 256, 64, 29, 16, 1024, 296, 148), (128, 128, 16, 8, 256, 64, 12, 32, 1024, 296, 148))
+
+
+def test_a_plan_is_taken_for_its_own_sizes_only(tmp_path):
+    src, so = tmp_path / "key.cpp", tmp_path / "key.so"
+    src.write_text('#include "g4b_pages.h"\nextern "C" int same(const int* a, const int* b) {\n'
+                   "g4b::pg::PlanKey x{}, y{};\n"
+                   "for (int i = 0; i < 12; i++) { x.v[i] = a[i]; y.v[i] = b[i]; }\n"
+                   "return g4b::pg::same_plan(x, y); }\nextern \"C\" int magic() { return g4b::pg::kPlanMagic; }\n")
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-I", CSRC, str(src), "-o", str(so)], check=True)
+    lib = C.CDLL(str(so))
+    key = lambda *v: (C.c_int * 12)(*v)  # noqa: E731
+    a, b = (key(lib.magic(), *t) for t in TWINS)
+    assert lib.magic() != 0 and lib.same(a, a) and lib.same(b, b) and not lib.same(a, b)
+    for i in range(12):                      # no field may differ, by however little
+        for bit in (0, 1, 8, 31):
+            c = key(*a)
+            c[i] = np.int32(np.uint32(c[i]) ^ np.uint32(1 << bit))
+            assert not lib.same(a, c) and not lib.same(c, a)
+    assert not lib.same(key(*[0] * 12), a)
