@@ -40,6 +40,9 @@ constexpr int kSoft = 2 * kGroup;       // two groups
 constexpr int kManyThreads = kSoft + 128;   // and a warp each for K's copies, V's, the scores and the products
 constexpr float kLift = 4.f;            // log2 of the weight that a row's maximum gets when its base is set
 constexpr float kMost = 15.f;           // log2 of the largest weight before the base is set anew (f16: below 2^16)
+// From a base of this size on, an f32 step is no longer small beside a weight's exponent, and the exact product in
+// x scale - base may lie steps above its rounded maximum: it is rounded as that one was before the base is taken off.
+constexpr float kFar = 4194304.f;
 
 template <int HD>
 struct ManyCfg {
@@ -650,19 +653,29 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 if (m != from && l != 0.f) l *= exp2_approx(m - from);
                 // A warp that has a row to rescale takes the base after every row's maximum that has grown: it is the warp
                 // that pays, and this way seldom twice.
-                const bool any = __any_sync(0xffffffffu, top > from + kMost && from != -INFINITY);
-                const bool set = u == 0 || from == -INFINITY || (any && top > from + kLift), scale = set && from != -INFINITY;
+                // (differences: a sum of the base and 15 may round up past the largest weight)
+                const bool any = __any_sync(0xffffffffu, top - from > kMost && from != -INFINITY);
+                const bool set = u == 0 || from == -INFINITY || (any && top - from > kLift), scale = set && from != -INFINITY;
                 m = set ? top - kLift : from;
                 sm.base[half][r0] = m;
                 arrive(b_base + 8u * half);
-                const float base = m == -INFINITY ? 0.f : m;
+                const float base0 = m == -INFINITY ? 0.f : m;
+                const bool far = fabsf(base0) >= kFar;
+                if (__any_sync(0xffffffffu, far)) {
+                    #pragma unroll
+                    for (int k = 0; k < 2; k++)
+                        #pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if (far) x[k][j] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(x[k][j]), a.scale), base0));
+                }
+                const float slope = far ? 1.f : a.scale, base = far ? 0.f : base0;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
                 #pragma unroll
                 for (int k = 0; k < 2; k++)
                     #pragma unroll
                     for (int j = 0; j < 16; j++) {
-                        const float e0x = exp2_approx(fmaf(__uint_as_float(x[k][2 * j]), a.scale, -base));
-                        const float e1x = exp2_approx(fmaf(__uint_as_float(x[k][2 * j + 1]), a.scale, -base));
+                        const float e0x = exp2_approx(fmaf(__uint_as_float(x[k][2 * j]), slope, -base));
+                        const float e1x = exp2_approx(fmaf(__uint_as_float(x[k][2 * j + 1]), slope, -base));
                         sum[j & 3] += e0x + e1x;
                         x[0][16 * k + j] = half_pair(e0x, e1x);       // P over the scores it is made of
                     }

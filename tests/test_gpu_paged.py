@@ -745,3 +745,45 @@ def test_a_plan_of_sizes_whose_hash_was_the_same():
         plan.append(torch.ones(T, 8192, device=DEV), w, w, rot, rot, kc, vc, ids, 4096, 6144, q_out=out)
         torch.cuda.synchronize()
         assert (out == 7).all() and not kc.any() and not vc.any() and L.query(L.Q_KERNEL_STATUS) == 2
+
+
+@pytest.mark.parametrize("nH,nkv,hd", [(16, 8, 256), (8, 1, 128), (4, 2, 512)])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_prompts_whose_scores_are_of_the_largest(nH, nkv, hd, sign):
+    """As above, where rows share a tile: equal scores far from zero give equal weights, the values' running mean."""
+    n = 300
+    bt = Batch(nH, nkv, hd, 64, [n], [n], 0, seed=52).fill()
+    bt.kc.copy_(torch.where(torch.isnan(bt.kc), bt.kc, torch.full_like(bt.kc, sign * 60000.0)))
+    out = _attend(bt, torch.full_like(bt.queries(), 200.0)).view(n, nH, hd).to(F64)
+    pg, sl = bt.places(0, n)
+    v = bt.vc[pg, :, sl].to(F64).repeat_interleave(nH // nkv, 1)
+    count = torch.arange(1, n + 1, dtype=F64, device=DEV)[:, None, None]
+    mean, a = v.cumsum(0) / count, v.abs().cumsum(0) / count
+    assert ((out - mean).abs() <= 2.0 ** -11 * mean.abs() + 2 * (2.0 ** -11 + 2.0 ** -20) * a + 2.0 ** -25).all()
+    assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+@pytest.mark.parametrize("nH,nkv,hd", [(16, 8, 256), (8, 1, 128), (4, 2, 512)])
+@pytest.mark.parametrize("step", [1, 2, 3])
+def test_large_scores_that_grow(nH, nkv, hd, step):
+    """Scores of 2^27 to 2^28 that grow by 16 steps with every unit: all are multiples of 16, so every sum is exact in
+    32 bits, and with scale log2(e) = 1 a weight of a smaller score is at most 2^-16.  Only a row's largest count."""
+    n, scale = 600, float(np.float32(np.log(2)))
+    assert np.float32(scale) * np.float32(1.4426950408889634) == 1
+    bt = Batch(nH, nkv, hd, 64, [n], [n], 0, seed=53).fill()
+    pg, sl = bt.places(0, n)
+    grown = 16.0 * step * (torch.arange(n, device=DEV) // 64)
+    q = torch.full_like(bt.queries(), 512.0)
+    big = 156_000_000 // (512 * (hd - 1)) // 8 * 8           # f16 holds multiples of 8 up to 2^14
+    q.view(n, nH, hd)[:, :, 0] = 1.0
+    bt.kc[pg, :, sl] = float(big)
+    bt.kc[pg, :, sl, 0] = grown.half()[:, None]
+    assert 2 ** 27 <= 512 * (hd - 1) * big and 512 * (hd - 1) * big + 1000 < 2 ** 28
+    out = _attend(bt, q, scale=scale).view(n, nH, hd).to(F64)
+    s = torch.where(torch.tril(torch.ones(n, n, dtype=torch.bool, device=DEV)), grown.to(F64), -torch.inf)
+    p = torch.exp2(s - s.amax(1, keepdim=True))
+    p /= p.sum(1, keepdim=True)
+    v = bt.vc[pg, :, sl].to(F64).repeat_interleave(nH // nkv, 1)
+    ref, a = torch.einsum("ij,jhd->ihd", p, v), torch.einsum("ij,jhd->ihd", p, v.abs())
+    assert ((out - ref).abs() <= 2.0 ** -11 * ref.abs() + 2 * (2.0 ** -11 + 2.0 ** -20) * a + 2.0 ** -25).all()
+    assert L.query(L.Q_KERNEL_STATUS) == 0
