@@ -11,15 +11,21 @@
 // unit i + 1 waited for the product of unit i - 1.)
 // m is a base, 2^4 under the maximum seen when it was set: O is rescaled only where a row's weights would pass
 // 2^15, the last power of two of f16 (a larger weight's relative rounding is the same; the 2^4 keep weights down
-// to 2^-18 of the maximum out of f16's subnormals).
+// to 2^-18 of the maximum out of f16's subnormals, a low part's down to 2^-7).
 // K and V units come by TMA through a ring each, issued ahead across pieces.
 //
 // Warps: 0-7 softmax, the mask, the rows' Q and the result; 8 and 11 the copies of K and V; 9 and 10 the MMAs.
-// Tensor memory's 512 columns: O 256, S 128, P 32 and the first 192 elements of Q; its others are in shared memory.  At hd
-// 512 O alone would fill them, so a tile is walked once for each half of the output columns (the scores are made twice).
+// Tensor memory's 512 columns: O 256, S 128, P 32 and the first 192 elements of Q (64 and 128 where P has two parts); its
+// others are in shared memory.  At hd 512 O alone would fill them, so a tile is walked once for each half of the output
+// columns (the scores are made twice).
 //
-// The weights P are rounded to f16, the type of V, as the tensor core needs one type for both: 2^-11 of each
-// weight, unbiased; sums and maxima are f32.
+// The tensor core needs one type for P and V, so the weights enter as f16.  For an f16 result as one: 2^-11 of each
+// weight, at most what the result's own rounding is, and a row's sum is of the rounded weights, so that what they have in
+// common cancels (the error against 64 bits is 1.11 to 1.13 times that of 32-bit weights with the result rounded to f16; with
+// the sum of the unrounded ones 1.22 to 1.34 times).  For an f32 result as two, a high and a low part: 2^-22 of each
+// weight, and 8 products a unit where there were 4 (2 prompts of 4,096 at hd 256 339 us instead of 277, at hd 128 150
+// instead of 131).  Either way weights below 2^-29 of the largest that its row had seen when its base was set count as
+// nothing.  Maxima, sums and accumulators are f32.
 //
 // What bounds it: neither the tensor core nor memory.  A unit takes 1,410 clocks at hd 256, of which the MMAs are 1,100
 // (1,300 and 550 at hd 128): the product of a unit waits for its weights, whose place is free when the product before is
@@ -44,27 +50,29 @@ constexpr float kMost = 15.f;           // log2 of the largest weight before the
 // x scale - base may lie steps above its rounded maximum: it is rounded as that one was before the base is taken off.
 constexpr float kFar = 4194304.f;
 
-template <int HD>
+template <int HD, bool PAIR>
 struct ManyCfg {
     static constexpr int DV = HD < 256 ? HD : 256;      // output columns of a walk
     static constexpr int CS = HD / DV;                  // walks per tile
-    static constexpr int QT = HD == 128 ? 128 : 192;    // elements of Q in tensor memory; the rest in shared memory
+    static constexpr int PC = PAIR ? 2 : 1;             // f16 parts of a weight
+    // elements of Q in tensor memory; the rest in shared memory
+    static constexpr int QT = HD == 128 || PAIR ? 128 : 192;
     // A ring entry is 64 keys of EC elements; a unit's K is KE of them and its V (a walk's columns) VE.  K and V have a
     // ring each: then the one warp that consumes a ring sees every phase of its barriers.
     static constexpr int EC = HD == 512 ? 128 : DV;
     static constexpr int KE = HD / EC, VE = DV / EC;
     static constexpr int ENTRY = kUnit * EC * 2;
-    static constexpr int NK = HD == 128 ? 5 : HD == 256 ? 3 : 6, NV = HD == 128 ? 5 : HD == 256 ? 2 : 3;
+    static constexpr int NK = HD == 128 ? 5 : HD == 256 ? 3 : PAIR ? 5 : 6, NV = HD == 128 ? 5 : HD == 256 ? 2 : 3;
     static constexpr int NST = NK + NV;
     static constexpr int QS_BYTES = kRowsP * (HD - QT) * 2;
     // a warp's 32 rows x 128 bytes on their way between rows in memory and rows in lanes; at hd 512 they lie in
     // the shared part of Q, which is idle then
     static constexpr int STAGE = 32 * 128;
     static constexpr bool STAGE_IN_Q = HD == 512;
-    // at hd 256 the first group has a second one each, for its second chunk of Q
-    static constexpr int STAGES = HD == 256 ? 12 : 8;
+    // where three chunks of Q go to tensor memory the first group has a second one each, for its second chunk
+    static constexpr int STAGES = HD == 256 && QT == 192 ? 12 : 8;
     static constexpr int BUF = NST * ENTRY + QS_BYTES + (STAGE_IN_Q ? 0 : STAGES * STAGE);
-    static constexpr int O_COL = 0, S_COL = DV, P_COL = S_COL + 2 * kUnit, Q_COL = P_COL + kUnit / 2;
+    static constexpr int O_COL = 0, S_COL = DV, P_COL = S_COL + 2 * kUnit, Q_COL = P_COL + PC * kUnit / 2;
     static_assert(Q_COL + QT / 2 <= 512, "tensor memory columns");
     // (the stages are the last two 64-element chunks of Q's shared part, which are written last)
     static_assert(!STAGE_IN_Q || (QS_BYTES >= 8 * STAGE && 8 * STAGE == 2 * kRowsP * 128), "the stages fit");
@@ -113,6 +121,11 @@ __device__ __forceinline__ uint4 ld_shared(uint32_t at) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
+}
+// Both halves of a pair added to an f32, an instruction each.  (Converted first they cost 8 % of a causal prompt's time at
+// hd 128; like this the sum of the rounded weights is as fast as that of the unrounded ones.)
+__device__ __forceinline__ void add_pair(float& sum, uint32_t h2) {
+    asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %1;\n\tadd.rn.f32.f16 %0, a, %0;\n\tadd.rn.f32.f16 %0, b, %0;\n\t}" : "+f"(sum) : "r"(h2));
 }
 // bit 15 of a half is set where the f16 value is not finite (its exponent field overflows by one)
 __device__ __forceinline__ uint32_t not_finite(uint32_t v) { return (v & 0x7fff7fffu) + 0x04000400u; }
@@ -169,10 +182,10 @@ struct Walk {
 
 }  // namespace
 
-template <int HD>
+template <int HD, bool PAIR>
 __global__ void __launch_bounds__(kManyThreads, 1)
 many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    using C = ManyCfg<HD>;
+    using C = ManyCfg<HD, PAIR>;
     extern __shared__ __align__(1024) uint8_t smem[];
     auto& sm = *reinterpret_cast<typename C::Small*>(smem + C::BUF);
     const Dims& d = a.d;
@@ -368,8 +381,11 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 const uint64_t vd = v_desc + (uint64_t)(s * (C::ENTRY / 16));
                 if (elect_one()) {
                     #pragma unroll
-                    for (int k = 0; k < kUnit / 16; k++)
-                        tc::mma_f16_ts(tmem + C::O_COL + ve * C::EC, tmem + C::P_COL + 8 * k, vd + v_off[k], id_o, acc || k > 0);
+                    for (int p = 0; p < C::PC; p++)            // the weights' high parts, the low ones
+                        #pragma unroll
+                        for (int k = 0; k < kUnit / 16; k++)
+                            tc::mma_f16_ts(tmem + C::O_COL + ve * C::EC, tmem + C::P_COL + p * (kUnit / 2) + 8 * k, vd + v_off[k],
+                                           id_o, acc || p + k > 0);
                     if (ve == C::VE - 1) tc::commit(b_pv + 8u * ((it + u) & 1u));
                     tc::commit(empty(s));
                     if (ve == C::VE - 1 && u == w.nu - 1) tc::commit(b_o);
@@ -463,12 +479,12 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
             if constexpr (!C::STAGE_IN_Q) {
                 #pragma unroll 1
                 for (int n = 0; n < NC; n++) {
-                    const int c = half * NC + n;
+                    const int c = half + 2 * n;
                     fetch(c, c < QC ? stage + n * C::STAGE : shared_of(c));
                 }
                 landed();
                 #pragma unroll 1
-                for (int n = 0; n < NC && half * NC + n < QC; n++) to_tmem(half * NC + n, stage + n * C::STAGE);
+                for (int n = 0; n < NC && half + 2 * n < QC; n++) to_tmem(half + 2 * n, stage + n * C::STAGE);
             } else {
                 // chunks by turns; the last one of each half goes where the stages are, when those are done with
                 #pragma unroll 1
@@ -670,14 +686,21 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 }
                 const float slope = far ? 1.f : a.scale, base = far ? 0.f : base0;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t low[32];
                 #pragma unroll
                 for (int k = 0; k < 2; k++)
                     #pragma unroll
                     for (int j = 0; j < 16; j++) {
                         const float e0x = exp2_approx(fmaf(__uint_as_float(x[k][2 * j]), slope, -base));
                         const float e1x = exp2_approx(fmaf(__uint_as_float(x[k][2 * j + 1]), slope, -base));
-                        sum[j & 3] += e0x + e1x;
-                        x[0][16 * k + j] = half_pair(e0x, e1x);       // P over the scores it is made of
+                        const uint32_t h2 = half_pair(e0x, e1x);
+                        x[0][16 * k + j] = h2;                        // P over the scores it is made of
+                        if constexpr (PAIR) {
+                            sum[j & 3] += e0x + e1x;
+                            low[16 * k + j] = half_pair(e0x - h_lo(h2), e1x - h_hi(h2));
+                        } else {
+                            add_pair(sum[j & 3], h2);
+                        }
                     }
                 if (scale) l *= exp2_approx(from - m);
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -685,6 +708,7 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                 // done, but its phase is counted.)
                 if (it > 0) wait_pv(it - 1);
                 tc::st_32x32b_x32(tl + C::P_COL, x[0]);
+                if constexpr (PAIR) tc::st_32x32b_x32(tl + C::P_COL + kUnit / 2, low);
                 if (any) {
                     // the next 32 columns come while these are stored
                     const float f = scale ? exp2_approx(from - m) : 1.f;
@@ -773,9 +797,13 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
                         }
                         for (unsigned long long rest = odd; rest; rest &= rest - 1) {
                             const int j = __ffsll((long long)rest) - 1;
-                            const uint32_t pj = ld_tmem_x1(tl + C::P_COL + j / 2);
-                            tc::wait_ld();
-                            const float pf = j & 1 ? h_hi(pj) : h_lo(pj);
+                            float pf = 0.f;
+                            #pragma unroll
+                            for (int p = 0; p < C::PC; p++) {
+                                const uint32_t pj = ld_tmem_x1(tl + C::P_COL + p * (kUnit / 2) + j / 2);
+                                tc::wait_ld();
+                                pf += j & 1 ? h_hi(pj) : h_lo(pj);
+                            }
                             const bool sees = key + j >= vlo && key + j < min(vhi, end) && ((there >> (j / box)) & 1u);
                             #pragma unroll 1
                             for (int c = 0; c < C::DV; c += 32) {
@@ -839,9 +867,11 @@ many_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid
 
 template <int HD>
 static cudaError_t launch(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(many_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, ManyCfg<HD>::SMEM);
+    const auto kernel = a.out_f32 ? many_kernel<HD, true> : many_kernel<HD, false>;
+    const int smem = a.out_f32 ? ManyCfg<HD, true>::SMEM : ManyCfg<HD, false>::SMEM;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    many_kernel<HD><<<a.d.ctas[1], kManyThreads, ManyCfg<HD>::SMEM, s>>>(a, km, vm);
+    kernel<<<a.d.ctas[1], kManyThreads, smem, s>>>(a, km, vm);
     return cudaGetLastError();
 }
 

@@ -787,3 +787,60 @@ def test_large_scores_that_grow(nH, nkv, hd, step):
     ref, a = torch.einsum("ij,jhd->ihd", p, v), torch.einsum("ij,jhd->ihd", p, v.abs())
     assert ((out - ref).abs() <= 2.0 ** -11 * ref.abs() + 2 * (2.0 ** -11 + 2.0 ** -20) * a + 2.0 ** -25).all()
     assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+RUNS = [([600, 90], [600, 300], 0, 0),                            # prompts
+        ([200, 70], [900, 800], 300, 257),                        # chunks under a window
+        ([1] * 70, [801 + i for i in range(70)], 800, 0),         # many users of a prefix
+        ([1, 3, 2], [500, 700, 60], 40, 0)]                       # and a few rows by themselves
+
+
+def _whole_scores(bt, n):
+    """Keys, and queries, of -1, 0 and 1: scores are whole numbers, exact in any order."""
+    ints = lambda *s: torch.randint(-1, 2, s, generator=bt.g, device=DEV).half()  # noqa: E731
+    bt.kc.copy_(torch.where(torch.isnan(bt.kc), bt.kc, ints(*bt.kc.shape)))
+    return ints(bt.T, n)
+
+
+@pytest.mark.parametrize("nH,nkv,hd", [(16, 8, 256), (8, 1, 128), (4, 2, 512), (16, 1, 512)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("new,total,prefix,window", RUNS)
+def test_an_f32_result_has_weights_of_more_bits_than_f16(nH, nkv, hd, dtype, new, total, prefix, window):
+    """With exact scores the error of the weights and of the sums is left, whichever kernel a row gets.  On a weight p_j:
+    its f16 (2^-11, for an f16 result) or its two f16 parts (2^-22), 2^-29 of the row's largest where a part is below f16's
+    normal range, the exponential (2^-22), the slope's two roundings over the distance to the maximum (2^-23 of it, in
+    powers of two).  On the sums: at most one truncation (2^-22) of the running sum for every eight keys (two products each
+    of 16), rescaling and joining (2^-20)."""
+    bt = Batch(nH, nkv, hd, 32, new, total, prefix, window, seed=54).fill()
+    q, scale = _whole_scores(bt, nH * hd), 0.25
+    out = _attend(bt, q, out_dtype=dtype, scale=scale).view(bt.T, nH, hd).to(F64)
+    half, bits = torch.finfo(dtype).eps / 2, 2.0 ** (-22 if dtype == torch.float32 else -11)
+    for b in range(bt.B):
+        n, t0, G = new[b], int(bt.start[b]), nH // nkv
+        pg, sl = bt.places(b, total[b])
+        k, v = (c[pg, :, sl].to(F64).repeat_interleave(G, 1) for c in (bt.kc, bt.vc))
+        pos, j = torch.arange(total[b] - n, total[b], device=DEV)[:, None], torch.arange(total[b], device=DEV)
+        see = (j <= pos) & (j > pos - window) if window else j <= pos
+        s = torch.einsum("mhd,jhd->mhj", q[t0:t0 + n].to(F64).view(n, nH, hd), k) * scale
+        s = torch.where(see[:, None], s, torch.full_like(s, -torch.inf))
+        far = (s.amax(-1, keepdim=True) - s) * 1.4427
+        p = torch.softmax(s, -1)
+        dp = torch.where(see[:, None], p * (bits + 2.0 ** -22 + 2.0 ** -23 * far) + 2.0 ** -29, torch.zeros_like(p))
+        ref, a = torch.einsum("mhj,jhd->mhd", p, v), torch.einsum("mhj,jhd->mhd", p, v.abs())
+        lim = 2 * torch.einsum("mhj,jhd->mhd", dp, v.abs()) + a * (see.sum(1)[:, None, None] / 8 * 2.0 ** -22 + 2.0 ** -20)
+        err = (out[t0:t0 + n] - ref).abs()
+        lim = lim + half * ref.abs() + 2.0 ** -25
+        assert (err <= lim).all(), f"{(err / lim).max().item():.2f} of the tolerance"
+    assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+@pytest.mark.parametrize("nH,nkv,hd", [(16, 8, 256), (8, 1, 128), (4, 2, 512), (16, 1, 512)])
+@pytest.mark.parametrize("new,total,prefix,window", RUNS)
+def test_equal_values_come_out_as_they_are(nH, nkv, hd, new, total, prefix, window):
+    """A row divides by the sum of the weights that its products had: where all values are the same, their roundings
+    cancel.  What is left, under 2^-15 by the sums' part of the bound above, is less than half a step of f16."""
+    bt = Batch(nH, nkv, hd, 32, new, total, prefix, window, seed=55).fill()
+    q, value = _whole_scores(bt, nH * hd), bt.randn(nkv, hd).half()
+    bt.vc.copy_(torch.where(torch.isnan(bt.vc), bt.vc, value[:, None]))
+    out = _attend(bt, q, scale=0.25).view(bt.T, nkv, nH // nkv, hd)
+    assert torch.equal(out, value[None, :, None].expand_as(out))
