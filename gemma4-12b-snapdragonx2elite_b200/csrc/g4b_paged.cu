@@ -717,11 +717,13 @@ __global__ void __launch_bounds__(32 * (stream_warps(HD) + 1), HD == 512 ? 1 : 2
 //   S^T [16 keys x 8 rows] = K [16 x hd] Q^T,   O^T [hd x 8] += V^T [hd x 16 keys] P^T
 // K and V fragments come from shared memory by ldmatrix (transposed for V), Q stays in registers, and P^T
 // gets from its accumulator layout to an operand's by movmatrix.  P enters as f16 hi + lo, since these
-// MMAs are not what bounds the kernel.  The four warps of a CTA take every fourth block of 16 keys, each
+// MMAs are not what bounds the kernel, and 2^15 times too large, as far as f16 goes: a weight then counts down to 2^-40 of
+// the row's largest (without that to 2^-25: a hundred thousand keys just below are lost, a percent of a long row).  The four warps of a CTA take every fourth block of 16 keys, each
 // with its own ring of TMA-filled buffers, its own running maximum and sum: no CTA barrier until the
 // partials of the warps are added at a piece's end.  48 decode tokens over 868 MB of ragged keys and values: 140 us, 0.95
 // of the measured copy rate.
 constexpr int kFewWarps = 4;
+constexpr float kFewLift = 15.f, kFewDrop = 0x1p-15f;
 constexpr int kBlk = 16;             // keys per block (one page always holds a block: page_size >= 16)
 
 template <int HD>
@@ -932,8 +934,9 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
                 const float mu = mn == -INFINITY ? 0.f : mn;     // nothing seen yet: weights 2^-inf = 0
                 corr[i] = exp2_approx(m[i] - mu);
                 m[i] = mn;
-                x[i] = exp2_approx(x[i] - mu);
-                x[2 + i] = exp2_approx(x[2 + i] - mu);
+                // (the difference first: at scores far from zero a base less 15 may be no f32)
+                x[i] = exp2_approx(x[i] - mu + kFewLift);
+                x[2 + i] = exp2_approx(x[2 + i] - mu + kFewLift);
                 l[i] = fmaf(l[i], corr[i], x[i] + x[2 + i]);
             }
             const __half2 h0 = __floats2half2_rn(x[0], x[1]), h1 = __floats2half2_rn(x[2], x[3]);
@@ -1044,7 +1047,7 @@ few_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_
             float L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
             #pragma unroll
             for (int w = 0; w < kFewWarps; w++) {
-                const float f = exp2_approx(s_m[w][r] - mu);
+                const float f = exp2_approx(s_m[w][r] - mu) * kFewDrop;
                 L = fmaf(s_l[w][r], f, L);
                 const float4 p = *reinterpret_cast<const float4*>(parts + w * WP + r * C::PITCH + c);
                 v[0] = fmaf(p.x, f, v[0]);

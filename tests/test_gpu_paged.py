@@ -844,3 +844,24 @@ def test_equal_values_come_out_as_they_are(nH, nkv, hd, new, total, prefix, wind
     bt.vc.copy_(torch.where(torch.isnan(bt.vc), bt.vc, value[:, None]))
     out = _attend(bt, q, scale=0.25).view(bt.T, nkv, nH // nkv, hd)
     assert torch.equal(out, value[None, :, None].expand_as(out))
+
+
+@pytest.mark.parametrize("nH,nkv,hd,new", [(16, 8, 256, 1), (8, 1, 128, 2), (4, 2, 512, 3), (16, 1, 512, 1), (8, 1, 128, 20)])
+@pytest.mark.parametrize("prefix", [0, 100_000])
+def test_many_small_weights_add_up(nH, nkv, hd, new, prefix):
+    """One key 26 powers of two above 131,071 others: each of them weighs nothing beside it, together they are 2^-9.  All
+    weights are powers of two and every sum is exact, so only the result's rounding and the division are left."""
+    n, scale = 1 << 17, float(np.float32(np.log(2)))
+    bt = Batch(nH, nkv, hd, 1024, [new], [n + new - 1], prefix, seed=56)
+    for c in (bt.kc, bt.vc):
+        c.zero_()
+    pg, sl = bt.place(0, 70_000)
+    bt.kc[pg, :, sl, 0] = 26.0
+    bt.vc.fill_(1.0)
+    bt.vc[pg, :, sl] = 0.0
+    q = torch.zeros(bt.T, nH * hd, dtype=torch.float16, device=DEV)
+    q.view(bt.T, nH, hd)[:, :, 0] = 1.0
+    out = _attend(bt, q, out_dtype=torch.float32, scale=scale).view(new, -1).to(F64)
+    rest = (torch.arange(new, device=DEV)[:, None] + n - 1) * 2.0 ** -26
+    assert ((out - rest / (1 + rest)).abs() <= 2.0 ** -20 * rest).all()
+    assert L.query(L.Q_KERNEL_STATUS) == 0
