@@ -224,3 +224,31 @@ def test_captured_and_replayed():
         _check(x, h, w, w, 1.0, out, a8, sa)
         b8, sb = ops.rows_normadd_i8(x, h, w, w_post=w, h_out=torch.empty_like(h))
         assert torch.equal(a8, b8) and torch.equal(sa, sb)
+
+
+@pytest.mark.parametrize("D", [256, 3840, 9600, 40000])
+def test_rows_below_the_smallest_scale(D):
+    """Rows whose largest magnitude is under 127e-12 have the scale 1e-12 and codes that are no longer spread over the whole
+    range: h of 5e-14 has y of 5e-11 (eps alone makes the norm's factor 1000) and the code 50."""
+    g = torch.Generator(device=DEV).manual_seed(D)
+    size = torch.tensor([1e-20, 4e-16, 5e-14, 1e-13, 1.2e-13], device=DEV)
+    h = (2 * torch.rand(5, D, generator=g, device=DEV) - 1) * size[:, None]
+    h[:, 5] = size
+    w = torch.ones(D, device=DEV)
+    a8, sa = ops.rows_normadd_i8(None, h, w)
+    assert (sa == np.float32(1e-12)).all()
+    y = h.to(F64) * (h.to(F64).pow(2).mean(-1, keepdim=True) + 1e-6).rsqrt()
+    code = y / 1e-12
+    assert ((a8.to(F64) - code).abs() <= 0.5 + code.abs() * 2.0 ** -19).all()
+    assert (a8[:2] == 0).all() and a8[2, 5] == 50 and a8[3, 5] == 100 and a8[4, 5] == 120
+
+
+def test_large_values_and_zeros_each_by_itself():
+    D = 256
+    h = torch.zeros(4, D, device=DEV)
+    h[1], h[2], h[3, 7] = 1e18, 1e-20, -1e15
+    a8, sa = ops.rows_normadd_i8(torch.zeros(4, D, device=DEV), h, torch.ones(D, device=DEV))
+    assert (a8[0] == 0).all() and (a8[1] == 127).all() and (a8[2] == 0).all()
+    assert a8[3, 7] == -127 and (a8[3].abs().sum() == 127)
+    assert sa[0] == np.float32(1e-12) and sa[2] == np.float32(1e-12)
+    assert abs(sa[1].item() * 127 - 1) < 1e-5 and abs(sa[3].item() * 127 / 16 - 1) < 1e-5
