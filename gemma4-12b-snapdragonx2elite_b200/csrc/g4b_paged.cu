@@ -477,7 +477,7 @@ __device__ __forceinline__ void store_half(uint16_t* p, const float (&v)[N]) {
     }
 }
 
-// Few tokens: one warp per head, a token's heads over several CTAs (blockIdx.y); latency is what counts.  Lane l holds
+// Few tokens, or few heads: one warp per head, a token's heads over several CTAs (blockIdx.y); latency is what counts.  Lane l holds
 // elements l * PER .. of the head; element i's rotation partner i +- hd/2 is in lane l ^ 16.
 template <int HD, bool XF32>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     store_half<PER>(dst + lane * PER, v);
 }
 
-// Many tokens: HBM-bound on q|k|v in and out, so the rows stream through shared memory.  A warp of each persistent
+// Many tokens of many heads: HBM-bound on q|k|v in and out, so the rows stream through shared memory.  A warp of each persistent
 // CTA copies a token's q, k, v and rotation rows into a ring of stages (bulk copies, 32 tokens' places looked up
 // at once), the others take the heads from there.  Lane l holds elements l * PER/2 .. of both halves of a head, so that
 // both ends of a rotation are its own.  Five prompts of 300 to 1,600 tokens, 129 MB in and out: 32 us, 0.61 of the measured
@@ -1274,10 +1274,14 @@ template <int HD, bool XF32>
 static cudaError_t launch_append_hd(const AppendArgs& a, int sms, cudaStream_t s) {
     const int heads = a.d.nH + 2 * a.d.nkv, per = kAppendThreads / 32;
     const int bytes = stage_bytes(a.d, XF32 ? 4 : 2);
-    // as many stages as the ring holds; a token too wide for two stages takes
-    // the other kernel, as a batch of few tokens does
+    // As many stages as the ring holds; a token too wide for two stages takes the other kernel.  So do tokens with fewer
+    // heads than this kernel has head warps, some of which would stand idle (8 / 1 heads of 128, 9,472 tokens: 27.0 us
+    // against 23.4; 4 / 2 of 256, 4,736: 17.7 against 15.2), and batches of few elements: the two are level at 3 to 7 M
+    // (16 / 8 heads of 256, f16: 444 tokens 7.6 us against 6.7, 592 8.0 against 8.7, 1,184 12.4 against 15.2; 8 / 8 of
+    // 128: 1,184 tokens 7.6 against 7.5, 2,368 12.5 against 13.5; 16 / 1 of 512: 296 tokens 8.7 against 8.9, 1,184 18.1
+    // against 26.1; 4 / 2 of 512: 1,184 tokens 12.6 against 11.5, 3,832 25.8 against 31.5).
     const int stages = std::min(8, kStreamSmem / bytes);
-    if (a.d.T >= 2 * sms && stages >= 2) {
+    if (stages >= 2 && heads >= stream_warps(HD) && (long long)a.d.T * heads * HD >= 1 << 22) {
         cudaError_t e = cudaFuncSetAttribute(append_stream_kernel<HD, XF32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              kStreamSmem);
         if (e != cudaSuccess) return e;

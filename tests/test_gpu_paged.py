@@ -865,3 +865,83 @@ def test_many_small_weights_add_up(nH, nkv, hd, new, prefix):
     rest = (torch.arange(new, device=DEV)[:, None] + n - 1) * 2.0 ** -26
     assert ((out - rest / (1 + rest)).abs() <= 2.0 ** -20 * rest).all()
     assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+def _append_case(nH, nkv, hd, dtype, page, new, total, prefix, keqv, seed):
+    bt = Batch(nH, nkv, hd, page, new, total, prefix, seed=seed, front=1, back=2)
+    nq, nk = nH * hd, nkv * hd
+    koff, voff = nq, nq if keqv else nq + nk
+    qkv = (bt.randn(bt.T, nq + 2 * nk + 16) * torch.exp(bt.randn(bt.T, 1))).to(dtype)[:, :-16]
+    qnw, knw = 1 + 0.2 * bt.randn(hd), 1 + 0.2 * bt.randn(hd)
+    n_pos = (bt.own_pages + bt.pre_pages) * page
+    inv = 10000.0 ** (-torch.arange(0, hd, 2, device=DEV, dtype=F64) / hd)
+    ang = torch.arange(n_pos, device=DEV, dtype=F64)[:, None] * torch.cat((inv, inv))
+    return bt, (qkv, qnw, knw, ang.cos().float(), ang.sin().float()), koff, voff
+
+
+@pytest.mark.parametrize("nH,nkv,hd,new", [
+    (16, 8, 256, [600, 0, 5, 700]), (16, 8, 256, [300, 7, 204]), (16, 8, 256, [300, 7, 203]),   # on either side of the rule
+    (16, 1, 512, [500, 1, 90]), (8, 8, 128, [1400, 2, 300]), (16, 2, 128, [900, 800, 30]),
+    (8, 1, 128, [4000, 90]), (4, 2, 512, [900, 300]), (16, 8, 512, [200, 150])])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("prefix,keqv", [(0, False), (40, True)])
+def test_append_of_long_prompts(nH, nkv, hd, new, dtype, prefix, keqv):
+    """Batches that go to the kernel whose rows stream through shared memory, and their neighbours that do not."""
+    rng = np.random.default_rng(hd)
+    total = [prefix + int(rng.integers(0, 90)) + n for n in new]
+    total[0] = max(new[0], prefix - 20 + new[0])              # its first tokens lie inside the prefix
+    bt, args, koff, voff = _append_case(nH, nkv, hd, dtype, 32, new, total, prefix, keqv, seed=60)
+    q_out = torch.full((bt.T, nH * hd), 7.0, dtype=torch.float16, device=DEV)
+    bt.plan().append(*args, bt.kc, bt.vc, bt.table, koff, voff, q_out=q_out)
+    torch.cuda.synchronize()
+    (q, qm), (k, km), (v, vm), pos = _append_reference(bt, *args, koff, voff)
+    lo, hi = int(bt.start[0]), int(bt.start[-1])
+    _close16(q_out.view(bt.T, nH, hd)[lo:hi], q[lo:hi], qm[lo:hi], "q")
+    assert (q_out[:lo] == 7).all() and (q_out[hi:] == 7).all()
+    written = torch.zeros(bt.pages, 32, dtype=torch.bool, device=DEV)
+    for b in range(bt.B):
+        t0, n = int(bt.start[b]), new[b]
+        pg, sl = bt.places(b, total[b])
+        at = torch.arange(total[b] - n, total[b], device=DEV)
+        own = at >= prefix
+        pg, sl, t = pg[at[own]], sl[at[own]], torch.arange(t0, t0 + n, device=DEV)[own]
+        written[pg, sl] = True
+        _close16(bt.kc[pg, :, sl], k[t], km[t], "k")
+        _close16(bt.vc[pg, :, sl], v[t], vm[t], "v")
+    for c in (bt.kc, bt.vc):
+        assert torch.isnan(c.permute(0, 2, 1, 3)[~written]).all()
+    assert L.query(L.Q_KERNEL_STATUS) == 0
+
+
+def test_two_threads_with_long_prompts_of_other_sizes():
+    """Two host threads whose appends stream through different amounts of shared memory."""
+    import threading
+
+    cases = [_append_case(16, 8, 256, torch.float16, 32, [700], [700], 0, False, 61),
+             _append_case(16, 1, 512, torch.float32, 32, [500, 40], [500, 40], 0, False, 62)]
+    jobs, errors = [], []
+    for bt, args, koff, voff in cases:
+        plan, out = bt.plan(), torch.empty(bt.T, bt.nH * bt.hd, dtype=torch.float16, device=DEV)
+        jobs.append((bt, plan, (*args, bt.kc, bt.vc, bt.table, koff, voff, out), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def run(bt, plan, args, stream):
+        try:
+            for _ in range(100):
+                plan.append(*args, stream=stream)
+        except Exception as e:                               # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors and L.query(L.Q_KERNEL_STATUS) == 0
+    for bt, _, args, _ in jobs:
+        (q, qm), (k, km), _, _ = _append_reference(bt, *args[:5], args[8], args[9])
+        lo, hi = int(bt.start[0]), int(bt.start[-1])
+        _close16(args[10].view(bt.T, bt.nH, bt.hd)[lo:hi], q[lo:hi], qm[lo:hi], "q")
+        pg, sl = bt.places(0, bt.total[0])
+        _close16(bt.kc[pg, :, sl], k[1:1 + bt.total[0]], km[1:1 + bt.total[0]], "k")
