@@ -945,3 +945,53 @@ def test_two_threads_with_long_prompts_of_other_sizes():
         _close16(args[10].view(bt.T, bt.nH, bt.hd)[lo:hi], q[lo:hi], qm[lo:hi], "q")
         pg, sl = bt.places(0, bt.total[0])
         _close16(bt.kc[pg, :, sl], k[1:1 + bt.total[0]], km[1:1 + bt.total[0]], "k")
+
+
+@pytest.mark.parametrize("nH,nkv,hd,new", [(16, 8, 256, 70), (16, 1, 512, 20), (4, 2, 512, 90), (8, 1, 128, 40)])
+@pytest.mark.parametrize("prefix", [0, 50])
+def test_values_out_of_sight_do_not_reach_an_f32_row(nH, nkv, hd, new, prefix):
+    """A value that is not finite where only a tile's first token sees it, and one that only its last token sees."""
+    window = 20
+    bt = Batch(nH, nkv, hd, 16, [new, 1], [new + 60, 90], prefix, window, seed=63).fill()
+    q = bt.queries()
+    clean = _attend(bt, q, out_dtype=torch.float32)
+    bt.check(clean, q)
+    for p, value in ((60 - window + 1, float("nan")), (new + 59, float("inf"))):
+        pg, sl = bt.place(0, p)
+        bt.kc[pg, :, sl], bt.vc[pg, :, sl] = float("inf"), value
+    out = _attend(bt, q, out_dtype=torch.float32)
+    blind = [i for i in range(bt.T) if i not in (0, new - 1)]
+    assert torch.equal(out[blind], clean[blind]) and not torch.isfinite(out[[0, new - 1]]).any()
+
+
+@pytest.mark.parametrize("nH,nkv,hd", [(16, 8, 256), (8, 1, 128), (4, 2, 512)])
+def test_an_infinity_leaves_the_rows_that_do_not_see_it_exact(nH, nkv, hd):
+    """The last token's value is infinite, which only its own row sees: f32 rows of the same tile are as exact as elsewhere."""
+    n = 100
+    bt = Batch(nH, nkv, hd, 32, [n], [n], 0, seed=64).fill()
+    q = _whole_scores(bt, nH * hd)
+    pg, sl = bt.place(0, n - 1)
+    bt.vc[pg, :, sl] = float("inf")
+    out = _attend(bt, q, out_dtype=torch.float32, scale=0.25).view(n, nH, hd).to(F64)
+    pg, sl = bt.places(0, n)
+    k, v = (c[pg, :, sl].to(F64).repeat_interleave(nH // nkv, 1) for c in (bt.kc, bt.vc))
+    see = torch.tril(torch.ones(n, n, dtype=torch.bool, device=DEV))[:-1, :-1]
+    s = torch.einsum("mhd,jhd->mhj", q.to(F64).view(n, nH, hd), k)[:-1, :, :-1] * 0.25
+    p = torch.softmax(torch.where(see[:, None], s, -torch.inf), -1)
+    ref, a = (torch.einsum("mhj,jhd->mhd", p, x[:-1]) for x in (v, v.abs()))
+    # weights 2^-21 and the slope over a distance of at most 2^7 steps (2^-16), sums 2^-18
+    assert ((out[:-1] - ref).abs() <= 2.0 ** -15 * a + 2.0 ** -29 * v[:-1].abs().sum(0)).all()
+    assert not torch.isfinite(out[-1]).any()
+
+
+@pytest.mark.parametrize("nH,nkv,hd", [(16, 8, 256), (8, 1, 128), (4, 2, 512)])
+def test_f32_results_at_scores_of_the_largest(nH, nkv, hd):
+    n = 300
+    bt = Batch(nH, nkv, hd, 64, [n], [n], 0, seed=65).fill()
+    bt.kc.copy_(torch.where(torch.isnan(bt.kc), bt.kc, torch.full_like(bt.kc, -60000.0)))
+    out = _attend(bt, torch.full_like(bt.queries(), 200.0), out_dtype=torch.float32).view(n, nH, hd).to(F64)
+    pg, sl = bt.places(0, n)
+    v = bt.vc[pg, :, sl].to(F64).repeat_interleave(nH // nkv, 1)
+    count = torch.arange(1, n + 1, dtype=F64, device=DEV)[:, None, None]
+    # equal weights, each a power of two: n / 8 truncations of the running sums are left
+    assert ((out - v.cumsum(0) / count).abs() <= (n / 8 * 2.0 ** -22 + 2.0 ** -20) * v.abs().cumsum(0) / count + 2.0 ** -25).all()
