@@ -1,5 +1,6 @@
 // g4b_paged.cu -- a batch of sequences over a paged f16 KV cache: the plan of the batch, the append of its new
-// keys and values with norm and rotation, and its attention, with a prefix that all sequences share read once.
+// keys and values with norm and rotation, and its attention, with a prefix that all sequences share read for many of
+// their rows at a time.
 //
 // The cache is [num_pages, nkv, page_size, hd] f16: the engine's per-head cache rows (src/vk_engine.py:281-282)
 // cut into pages.  The arithmetic per token and head is that of vk/prepkv.comp and vk/attn.comp.

@@ -521,8 +521,8 @@ G4B_API int g4b_attn_prefill(const void* q, int dtype, int q_stride, int M, cons
 
 /* ------------------------------------------------------------ batches over a paged KV cache */
 /* The engine serves one sequence from a contiguous cache (src/vk_engine.py:281-282, 416-417).  These calls
- * serve a ragged batch of B sequences whose caches are made of pages, with a prefix that all of them share
- * kept, and read, once.
+ * serve a ragged batch of B sequences whose caches are made of pages, with a prefix that all of them share kept
+ * once and read for many of their rows at a time.
  *
  *   cache         kc, vc [num_pages, nkv, page_size, hd] f16; page_size a power of two, 16 to 1024
  *   tokens        the sequences' new tokens back to back: sequence b has rows q_start[b] .. q_start[b+1] - 1
@@ -570,13 +570,16 @@ G4B_API int g4b_paged_append(const void* qkv, int dtype, long long row_stride, c
 
 /* Attention of the new tokens over their sequences' pages: for the token in row t at position p, query head h,
  *   out[t, h*hd ..] = sum_j softmax_j(scale * q_t,h . k_j) v_j over the positions j <= p, j > p - window if window > 0.
- * The prefix's keys and values are read once for the rows of all sequences, a sequence's own once for its rows.
+ * Keys and values are read per tile of rows (row: a token and one of the query heads on a KV head), mostly from L2 after
+ * the first time.  The rows of all sequences of up to 64 share tiles of 128 against the prefix, and each of the
+ * sequences reads its own keys once per tile of 8 (up to 8 rows, or 16 at hd 128) or of 128.  A sequence of more than 64
+ * rows reads the prefix and its own keys once per 128 of them.  At hd 512 a tile of 128 reads its keys twice.
  * A token that sees no key gets zeros.  q f16 [T, q_stride]; out f16 or f32 [T, out_stride]; strides multiples of 8.
  * f32 scores, maxima, sums and accumulators.  The weights enter as f16 hi + lo pairs; for an f16 result, where a sequence
  * (or the prefix) has more than 8 rows (16 at hd 128), as one f16 each, and their sum is of the rounded weights.
  * Weights down to 2^-40 of a row's largest count, 2^-29 where rows share a tile.  out may not overlap q or the caches (G4B_E_ARG);
- * columns of one buffer may hold both.  The workspace (g4b_paged_workspace_bytes) needs no
- * initialisation; calls that share one, or a plan, must be ordered. */
+ * columns of one buffer may hold both.  The workspace (g4b_paged_workspace_bytes: with a
+ * prefix 8 bytes per element of out, and 22 to 50 MB for the SMs) needs no initialisation; calls that share one, or a plan, must be ordered. */
 G4B_API size_t g4b_paged_workspace_bytes(int T, int B, int nH, int nkv, int hd, int page_size, int table_pages,
                                          int prefix_pages, int window);
 G4B_API int g4b_paged_attn(const uint16_t* q, long long q_stride, const uint16_t* kc, const uint16_t* vc, int num_pages,
