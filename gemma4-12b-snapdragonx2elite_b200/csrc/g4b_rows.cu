@@ -409,7 +409,9 @@ int g4b_rows_normadd_i8(const void* x, int x_dtype, const float* w_post, const f
     G4B_REQUIRE(h && w && A8 && sa, G4B_E_ARG, "rows_normadd_i8: NULL pointer");
     G4B_REQUIRE(x || !w_post, G4B_E_ARG, "rows_normadd_i8: w_post without x");
     G4B_REQUIRE(!x || dt_ok(x_dtype), G4B_E_ARG, "rows_normadd_i8: bad dtype %d", x_dtype);
-    G4B_REQUIRE(M >= 1 && D >= 16 && D % 16 == 0, G4B_E_SHAPE, "rows_normadd_i8: M=%d D=%d (D a multiple of 16)", M, D);
+    // (the loops over a long row count in 32 bits, a block's step beyond its end)
+    G4B_REQUIRE(M >= 1 && D >= 16 && D % 16 == 0 && D <= 1 << 30, G4B_E_SHAPE,
+                "rows_normadd_i8: M=%d D=%d (D a multiple of 16, at most 2^30)", M, D);
     const size_t n = (size_t)M * D;
     G4B_REQUIRE(!h_out || h_out == h || !rows_overlap(flat(h_out, 4 * n), flat(h, 4 * n)), G4B_E_ARG,
                 "rows_normadd_i8: h_out overlaps h without being h");

@@ -612,7 +612,7 @@ G4B_API int g4b_gelumul(const void* gate, const void* up, int dtype, void* out, 
  * x f32 or f16; h, w_post, w f32.  h' goes to h_out, which may be h itself (in place) but not overlap it
  * otherwise; NULL: it is not stored.  Nothing else that is written may overlap what is read.  x, w_post, h, h_out and w are
  * 32-byte aligned, A8 16-byte.  The codes are formed without rounding y first, so one may differ by a step from the three
- * calls' where y / sa is next to a half.  D is a multiple of 16. */
+ * calls' where y / sa is next to a half.  D is a multiple of 16, at most 2^30. */
 G4B_API int g4b_rows_normadd_i8(const void* x, int x_dtype, const float* w_post, const float* h, float* h_out, float scl,
                                 const float* w, int8_t* A8, float* sa, int M, int D, g4b_stream_t stream);
 

@@ -257,3 +257,11 @@ def test_a_plan_is_taken_for_its_own_sizes_only(tmp_path):
             c[i] = np.int32(np.uint32(c[i]) ^ np.uint32(1 << bit))
             assert not lib.same(a, c) and not lib.same(c, a)
     assert not lib.same(key(*[0] * 12), a)
+
+
+def test_rows_too_long_to_count_are_refused():
+    x, h, w, h_out, a8, sa = (FAR + (i << 36) for i in range(6))
+    f = L.load().g4b_rows_normadd_i8
+    for d in ((1 << 30) + 16, 2**31 - 16):
+        assert f(x, 1, None, h, h_out, 1.0, w, a8, sa, 1, d, None) == L.G4B_E_SHAPE and "2^30" in L.last_error()
+    assert f(x, 1, None, h, h_out, 1.0, w, h + 32, sa, 1, 1 << 30, None) == L.G4B_E_ARG      # that size is looked at further
