@@ -29,6 +29,8 @@ class PagedPlan:
         self.T, self.B, self.nH, self.nkv, self.hd = tokens, seqs, nH, nkv, hd
         self.page_size, self.table_pages, self.prefix_pages, self.window = page_size, table_pages, prefix_pages, window
         dev = torch.device(device)
+        if dev.type != "cuda":
+            raise ValueError(f"a paged plan lives on a CUDA device, not on {dev}")
         self.index = torch.cuda.current_device() if dev.index is None else dev.index
         self.device = torch.device("cuda", self.index)
         self._lib = L.load()

@@ -265,3 +265,10 @@ def test_rows_too_long_to_count_are_refused():
     for d in ((1 << 30) + 16, 2**31 - 16):
         assert f(x, 1, None, h, h_out, 1.0, w, a8, sa, 1, d, None) == L.G4B_E_SHAPE and "2^30" in L.last_error()
     assert f(x, 1, None, h, h_out, 1.0, w, h + 32, sa, 1, 1 << 30, None) == L.G4B_E_ARG      # that size is looked at further
+
+
+def test_a_plan_on_the_host_is_refused():
+    from g4b.paged import PagedPlan
+    for device in ("cpu", "meta"):
+        with pytest.raises(ValueError, match=device):
+            PagedPlan(1, 1, 16, 8, 256, 64, 1, device=device)
