@@ -478,8 +478,8 @@ __device__ __forceinline__ void store_half(uint16_t* p, const float (&v)[N]) {
     }
 }
 
-// Few tokens, or few heads: one warp per head, a token's heads over several CTAs (blockIdx.y); latency is what counts.  Lane l holds
-// elements l * PER .. of the head; element i's rotation partner i +- hd/2 is in lane l ^ 16.
+// Few tokens, or few heads: one warp per head, a token's heads over several CTAs (blockIdx.y); latency is what counts.
+// Lane l holds elements l * PER .. of the head; element i's rotation partner i +- hd/2 is in lane l ^ 16.
 template <int HD, bool XF32>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
     constexpr int PER = HD / 32;
@@ -719,8 +719,8 @@ __global__ void __launch_bounds__(32 * (stream_warps(HD) + 1), HD == 512 ? 1 : 2
 // K and V fragments come from shared memory by ldmatrix (transposed for V), Q stays in registers, and P^T
 // gets from its accumulator layout to an operand's by movmatrix.  P enters as f16 hi + lo, since these
 // MMAs are not what bounds the kernel, and 2^15 times too large, as far as f16 goes: a weight then counts down to 2^-40 of
-// the row's largest (without that to 2^-25: a hundred thousand keys just below are lost, a percent of a long row).  The four warps of a CTA take every fourth block of 16 keys, each
-// with its own ring of TMA-filled buffers, its own running maximum and sum: no CTA barrier until the
+// the row's largest (without that to 2^-25: a hundred thousand keys just below are lost, a percent of a long row).  The
+// four warps of a CTA take every fourth block of 16 keys, each with its own ring of TMA-filled buffers, its own running maximum and sum: no CTA barrier until the
 // partials of the warps are added at a piece's end.  48 decode tokens over 868 MB of ragged keys and values: 140 us, 0.95
 // of the measured copy rate.
 constexpr int kFewWarps = 4;

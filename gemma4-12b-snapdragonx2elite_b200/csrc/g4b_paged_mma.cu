@@ -1,4 +1,4 @@
-// g4b_paged_mma.cu -- attention over the paged cache where many rows share the keys: a prefix read for all
+// g4b_paged_mma.cu -- attention over the paged cache where many rows share the keys: a prefix read for many
 // sequences at once, and the chunks of prompts.
 //
 // A tile is 128 rows (token, query head of the group) of one KV head, a row per tensor memory lane; units of 64
@@ -31,8 +31,8 @@
 // (1,300 and 550 at hd 128): the product of a unit waits for its weights, whose place is free when the product before is
 // done, and each such hand-over from warp to warp and back is 150 to 300 clocks.  Deeper or shallower rings change
 // nothing.  Between two pieces pass 12,000 clocks at hd 256 (16,000 before Q's chunks came all at once): Q in, the masks,
-// the result out.  Two prompts of 4,096 tokens over 16 heads of 256 (8 KV heads): 286 us, 0.58 of the measured bf16
-// rate; of 128 (8 heads, 1 KV head): 123 us.
+// the result out.  Two prompts of 4,096 tokens over 16 heads of 256 (8 KV heads): 284 us, 0.58 of the measured bf16
+// rate; of 128 (8 heads, 1 KV head): 129 us, 0.32.
 #include "g4b_paged.cuh"
 #include "g4b_tcgen05.cuh"
 
@@ -125,7 +125,8 @@ __device__ __forceinline__ uint4 ld_shared(uint32_t at) {
 // Both halves of a pair added to an f32, an instruction each.  (Converted first they cost 8 % of a causal prompt's time at
 // hd 128; like this the sum of the rounded weights is as fast as that of the unrounded ones.)
 __device__ __forceinline__ void add_pair(float& sum, uint32_t h2) {
-    asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %1;\n\tadd.rn.f32.f16 %0, a, %0;\n\tadd.rn.f32.f16 %0, b, %0;\n\t}" : "+f"(sum) : "r"(h2));
+    asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %1;\n\tadd.rn.f32.f16 %0, a, %0;\n\tadd.rn.f32.f16 %0, b, %0;\n\t}"
+        : "+f"(sum) : "r"(h2));
 }
 // bit 15 of a half is set where the f16 value is not finite (its exponent field overflows by one)
 __device__ __forceinline__ uint32_t not_finite(uint32_t v) { return (v & 0x7fff7fffu) + 0x04000400u; }

@@ -577,9 +577,9 @@ G4B_API int g4b_paged_append(const void* qkv, int dtype, long long row_stride, c
  * A token that sees no key gets zeros.  q f16 [T, q_stride]; out f16 or f32 [T, out_stride]; strides multiples of 8.
  * f32 scores, maxima, sums and accumulators.  The weights enter as f16 hi + lo pairs; for an f16 result, where a sequence
  * (or the prefix) has more than 8 rows (16 at hd 128), as one f16 each, and their sum is of the rounded weights.
- * Weights down to 2^-40 of a row's largest count, 2^-29 where rows share a tile.  out may not overlap q or the caches (G4B_E_ARG);
- * columns of one buffer may hold both.  The workspace (g4b_paged_workspace_bytes: with a
- * prefix 8 bytes per element of out, and 22 to 50 MB for the SMs) needs no initialisation; calls that share one, or a plan, must be ordered. */
+ * Weights down to 2^-40 of a row's largest count, 2^-29 where rows share a tile.  out may not overlap q or the caches
+ * (G4B_E_ARG); columns of one buffer may hold both.  The workspace (g4b_paged_workspace_bytes: 22 to 50 MB for the SMs and,
+ * with a prefix, 8 bytes per element of out) needs no initialisation; calls that share one, or a plan, must be ordered. */
 G4B_API size_t g4b_paged_workspace_bytes(int T, int B, int nH, int nkv, int hd, int page_size, int table_pages,
                                          int prefix_pages, int window);
 G4B_API int g4b_paged_attn(const uint16_t* q, long long q_stride, const uint16_t* kc, const uint16_t* vc, int num_pages,
